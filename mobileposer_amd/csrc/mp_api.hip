@@ -5,14 +5,11 @@
 // finish_or_recover -> leave.  The rest of the host side: mp_host.h has the map.
 //
 // Launches are eager by default, or, opt-in, captured once per (shape, buffer set) into a hipGraph and replayed.
-// Why eager is the default: the multi-branch graph executor of the HIP runtime this image ships (libamdhip64 of
-// ROCm 7.0, hip::Graph::UpdateStreams) picks max_streams-1 of the max_streams internal streams a hipGraphExec_t owns,
-// skipping those that share a hardware queue with the launch stream, WITHOUT a bounds check: when two of them map to
-// the launch stream's queue (GPU_MAX_HW_QUEUES = 4 by default, so this depends on every stream the process has ever
-// created) it reads past the end of the vector and the process dies with SIGSEGV inside hipGraphLaunch
-// (profiles/r02_hipgraph_segv.md: backtrace, disassembly, and the GPU_MAX_HW_QUEUES experiment).  Eager launches on
-// the library's streams measure the same step time; graph mode 1 means mode 2 (single-branch) unless the environment asks
-// for the real thing (mp_handle.hip multibranch_graphs_allowed).
+// Why eager is the default: the multi-branch graph executor of the HIP runtime this image ships (ROCm 7.0) can die with SIGSEGV
+// inside hipGraphLaunch, depending on every stream the process has ever created (GPU_MAX_HW_QUEUES = 4 by default; with 8, or
+// with single-branch graphs, it does not: profiles/r02_hipgraph_segv.md).  Eager launches on the library's streams measure the
+// same step time; graph mode 1 means mode 2 (single-branch) unless the environment asks for the real thing (mp_handle.hip
+// multibranch_graphs_allowed).
 #include "mp_host.h"
 
 // ================================================================================================ C ABI
