@@ -40,6 +40,7 @@ def file_build_id(path=None):
 
 MP_OK = 0
 MP_ERR_INVALID, MP_ERR_HIP, MP_ERR_STATE_SHAPE, MP_ERR_NO_STREAMS, MP_ERR_LENGTHS, MP_ERR_DEVICE = -1, -2, -3, -4, -5, -6
+F32, BF16 = 0, 1
 MOD_JOINTS, MOD_POSE, MOD_FOOT_CONTACT, MOD_VELOCITY = 0, 1, 2, 3
 
 _vp, _i, _i64, _sz = C.c_void_p, C.c_int, C.c_int64, C.c_size_t
@@ -84,6 +85,11 @@ SIGNATURES = {
     "mp_live_form_frames": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, C.c_uint, _i, _vp, _vp]),
     "mp_stream_get_state": (_i, [_vp, _i, _vp, _fp, C.POINTER(C.c_double), _fp, C.POINTER(_i)]),
     "mp_stream_set_state": (_i, [_vp, _i, _vp, _fp, C.POINTER(C.c_double), _fp, C.POINTER(_i)]),
+    "mp_delta_rule": (_i, [_vp, _i] + [_vp] * 7 + [_i] * 6 + [C.c_float] + [_vp] * 4 + [_sz, _vp]),
+    "mp_delta_rule_workspace": (_sz, [_i, _i, _i]),
+    "mp_delta_rule_online": (_i, [_vp, _i] + [_vp] * 7 + [_i] * 6 + [C.c_float] + [_vp] * 3),
+    "mp_linear_adapted": (_i, [_vp, _i] + [_vp] * 8 + [_i] * 7 + [_vp, _vp, _sz, _vp]),
+    "mp_linear_adapted_workspace": (_sz, [_i, _i, _i]),
     "mp_timing_enable": (_i, [_vp, _i]),
     "mp_timing_read": (_i, [_vp, _i, C.POINTER(_i), _fp, C.POINTER(C.c_double)]),
     "mp_set_graph_mode": (_i, [_vp, _i]),

@@ -22,6 +22,7 @@ from .body_model import ParametricModel, eval_metrics_call, fk_call, upload_mesh
 from .config import joint_set, model_config, paths
 from .manifest import state_dict_manifest
 from .model_utils import blob_to_state_dict, state_dict_to_blob
+from .sequence import SequenceOps
 
 
 def _ptr(t):
@@ -136,7 +137,7 @@ class _PoserView(_ModuleView):
         return self._net._reduced_global_to_full(reduced_pose)
 
 
-class MobilePoserNet:
+class MobilePoserNet(SequenceOps):
     """Inputs: N IMUs.  Outputs: SMPL pose (rotation matrices) and translation.  (models/net.py:22-26)"""
 
     def __init__(self, poser=None, joints=None, foot_contact=None, velocity=None, finetune=False,
@@ -226,6 +227,7 @@ class MobilePoserNet:
         J = np.ascontiguousarray(self.bodymodel.J, dtype=np.float32).reshape(-1)
         h = C.c_void_p()
         idx = self.device.index if self.device.index is not None else torch.cuda.current_device()
+        self._device_index = idx
         if blob_dev is not None:
             assert blob_dev.is_cuda and blob_dev.dtype == torch.float32 and blob_dev.is_contiguous()
             rc = self._lib.mp_create_from_device(C.byref(h), idx, _ptr(blob_dev), blob_dev.numel(), parent,

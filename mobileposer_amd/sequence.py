@@ -1,0 +1,173 @@
+"""Sequence operators of the facade: the gated delta rule over ragged batches (``delta_rule``) and per tick of S streams
+(``delta_rule_online``), and a linear layer with a low-rank adapter per sequence (``linear_adapted``) -- the parts of a personalised
+recurrent block, over mp_delta_rule / mp_delta_rule_online / mp_linear_adapted (include/mobileposer_hip.h).
+
+They take torch tensors on the model's device, fp32 or bf16, run on the current stream, and return fresh tensors without waiting.
+Inference only, as the rest of the package: a tensor that requires a gradient is refused while gradients are recorded.
+No counterpart in the reference."""
+import ctypes as C
+
+import torch
+
+from . import _lib
+
+_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
+_INT_MAX = 2 ** 31 - 1
+
+
+def _no_grad(*tensors):
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError("the sequence operators have no backward pass: call them under torch.no_grad() or detach their inputs")
+
+
+def _rows(t):
+    """The tensor itself when its last dimension is contiguous, else a contiguous copy."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+class SequenceOps:
+    """Methods of ``MobilePoserNet`` (they use its native handle and device)."""
+
+    def _dtype(self, what, *tensors):
+        """The common type of the tensors, as the library numbers it; all of them on this model's device."""
+        first = tensors[0].dtype
+        if first not in _DTYPES:
+            raise RuntimeError("%s takes float32 or bfloat16 tensors, got %s" % (what, first))
+        for t in tensors:
+            if t.dtype != first:
+                raise RuntimeError("%s: tensors of one type expected, got %s and %s" % (what, first, t.dtype))
+            if t.device != self.device:
+                self._same_device(what, t)
+        return _DTYPES[first]
+
+    def _same_device(self, what, t):
+        if t.device.type != "cuda" or t.device.index != self._device_index:
+            raise RuntimeError("%s: a tensor on %s, the model is on %s" % (what, t.device, self.device))
+
+    def _indices(self, what, value, n, lo, hi):
+        """[n] int32 on the device.  A host sequence is checked against lo..hi; a device tensor is taken as it is (the kernels
+        hold its values to the range: nothing waits for the device here)."""
+        if torch.is_tensor(value) and value.is_cuda:
+            if tuple(value.shape) != (n,) or value.dtype not in (torch.int32, torch.int64):
+                raise RuntimeError("%s: expected [%d] int32, got %s %s" % (what, n, tuple(value.shape), value.dtype))
+            if value.device != self.device:
+                self._same_device(what, value)
+            if value.dtype == torch.int64:
+                value = value.clamp(-1, _INT_MAX).to(torch.int32)
+            return value if value.stride(0) == 1 or n == 1 else value.contiguous()
+        ints = [int(i) for i in value]
+        if len(ints) != n:
+            raise RuntimeError("%s: %d values for %d sequences" % (what, len(ints), n))
+        if any(i < lo or i > hi for i in ints):
+            raise RuntimeError("%s: values outside of %d..%d" % (what, lo, hi))
+        return torch.tensor(ints, dtype=torch.int32, device="cuda:%d" % self._device_index)
+
+    def _heads(self, what, q, k, v, g, beta, lead):
+        if q.dim() != lead + 2 or k.shape != q.shape or v.dim() != lead + 2 or v.shape[:lead] != q.shape[:lead]:
+            raise RuntimeError("%s: q, k [.., Hk, dk] and v [.., Hv, dv] expected, got %s, %s, %s" % (what, tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+        Hk, dk, Hv, dv = q.shape[-2], q.shape[-1], v.shape[-2], v.shape[-1]
+        if Hk < 1 or Hv < 1 or Hv % Hk or not 1 <= dk <= 256 or dv < 1:
+            raise RuntimeError("%s: %d value heads over %d key heads, head sizes %d / %d (Hv a multiple of Hk, dk at most 256)" % (what, Hv, Hk, dk, dv))
+        if g.shape != v.shape[:-1] or beta.shape != v.shape[:-1]:
+            raise RuntimeError("%s: g and beta %s expected, got %s and %s" % (what, tuple(v.shape[:-1]), tuple(g.shape), tuple(beta.shape)))
+        if g.dtype != torch.float32 or beta.dtype != torch.float32:
+            raise RuntimeError("%s: g and beta are float32, got %s and %s" % (what, g.dtype, beta.dtype))
+        return Hk, dk, Hv, dv
+
+    def delta_rule(self, q, k, v, g, beta, input_lengths=None, state=None, scale=None):
+        """The gated delta rule over B ragged sequences: per value head a state S [dk, dv] and per frame
+        ``S = exp(g) S; u = beta (v - S^T k); S = S + k u^T; o = scale S^T q``.
+
+        q, k [B, T, Hk, dk], v [B, T, Hv, dv] (fp32 or bf16; views of one projection's rows are fine), g (<= 0), beta [B, T, Hv]
+        fp32, ``input_lengths`` [B] (0..T; a list, or an int32 tensor on the device, whose values are clamped), ``state``
+        [B, Hv, dk, dv] fp32 or None (zeros), ``scale`` (default dk ** -0.5).
+        -> (o [B, T, Hv, dv], zeros behind a sequence's end; the state after each sequence's last frame, fp32)."""
+        self._require_weights()
+        _no_grad(q, k, v, g, beta, state)
+        dtype = self._dtype("delta_rule", q, k, v)
+        Hk, dk, Hv, dv = self._heads("delta_rule", q, k, v, g, beta, 2)
+        self._dtype("delta_rule", g, beta)
+        B, T = q.shape[0], q.shape[1]
+        if state is not None:
+            if state.shape != (B, Hv, dk, dv) or state.dtype != torch.float32:
+                raise RuntimeError("delta_rule: state [%d, %d, %d, %d] float32 expected, got %s %s" % (B, Hv, dk, dv, tuple(state.shape), state.dtype))
+            self._dtype("delta_rule", state)
+            state = state.contiguous()
+        lens = None if input_lengths is None else self._indices("delta_rule: input_lengths", input_lengths, B, 0, T)
+        q, k, v = _rows(q), _rows(k), _rows(v)
+        dev = q.device
+        o = torch.empty(B, T, Hv, dv, device=dev, dtype=q.dtype)
+        out = torch.empty(B, Hv, dk, dv, device=dev, dtype=torch.float32)
+        need = self._lib.mp_delta_rule_workspace(B, T, Hv)
+        ws = torch.empty(need, device=dev, dtype=torch.uint8)
+        st = (C.c_int64 * 15)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *g.stride(), *beta.stride())
+        self._check(self._lib.mp_delta_rule(
+            self._h, dtype, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), C.addressof(st),
+            0 if lens is None else lens.data_ptr(), B, T, Hk, Hv, dk, dv, dk ** -0.5 if scale is None else float(scale), o.data_ptr(),
+            0 if state is None else state.data_ptr(), out.data_ptr(), ws.data_ptr(), need, torch.cuda.current_stream(dev).cuda_stream))
+        return o, out
+
+    def delta_rule_online(self, q, k, v, g, beta, state, slots=None, scale=None):
+        """One frame of S streams on states that stay in place: q, k [S, Hk, dk], v [S, Hv, dv], g, beta [S, Hv], ``state``
+        [n, Hv, dk, dv] fp32 contiguous, updated; ``slots`` [S]: the state of each stream (None: stream s has state s).  A negative
+        slot is a stream without a frame (zeros, no state changes); a slot that is not there, or that an earlier stream of the
+        call has, gives a row of NaN and changes no state.  -> o [S, Hv, dv]."""
+        self._require_weights()
+        _no_grad(q, k, v, g, beta, state)
+        dtype = self._dtype("delta_rule_online", q, k, v)
+        Hk, dk, Hv, dv = self._heads("delta_rule_online", q, k, v, g, beta, 1)
+        self._dtype("delta_rule_online", g, beta, state)
+        S = q.shape[0]
+        if state.dim() != 4 or state.shape[1:] != (Hv, dk, dv) or not state.is_contiguous():
+            raise RuntimeError("delta_rule_online: contiguous state [n, %d, %d, %d] expected, got %s" % (Hv, dk, dv, tuple(state.shape)))
+        n = state.shape[0]
+        if slots is None:
+            if S > n:
+                raise RuntimeError("delta_rule_online: %d streams on %d states" % (S, n))
+        else:
+            slots = self._indices("delta_rule_online: slots", slots, S, -_INT_MAX, n - 1)
+        q, k, v = _rows(q), _rows(k), _rows(v)
+        o = torch.empty(S, Hv, dv, device=q.device, dtype=q.dtype)
+        st = (C.c_int64 * 10)(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *g.stride(), *beta.stride())
+        self._check(self._lib.mp_delta_rule_online(
+            self._h, dtype, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), C.addressof(st),
+            0 if slots is None else slots.data_ptr(), S, n, Hk, Hv, dk, dv, dk ** -0.5 if scale is None else float(scale), o.data_ptr(),
+            state.data_ptr(), torch.cuda.current_stream(q.device).cuda_stream))
+        return o
+
+    def linear_adapted(self, x, weight, bias, down, up, scale, ids, relu=False):
+        """``act(x W^T + b + scale[a] (x down[a]^T) up[a]^T)`` with a = ids[sequence]: a linear layer (nn.Linear's weight [M, K] and
+        bias [M] or None) with a low-rank adapter per sequence beside it.  x [B, T, K] or, one frame each, [B, K]; down [n, r, K],
+        up [n, M, r], r at most 128; ``scale`` [n] fp32 or None (1); ``ids`` [B]: negative = the shared layer alone (a list, or an
+        int32 tensor on the device: a value >= n gives rows of NaN); ``relu``: ReLU behind it.  -> [B, T, M] or [B, M]."""
+        self._require_weights()
+        _no_grad(x, weight, bias, down, up, scale)
+        dtype = self._dtype("linear_adapted", x, weight, down, up, *(() if bias is None else (bias,)))
+        if x.dim() not in (2, 3) or weight.dim() != 2 or weight.shape[1] != x.shape[-1]:
+            raise RuntimeError("linear_adapted: x [B, T, K] or [B, K] and weight [M, K] expected, got %s and %s" % (tuple(x.shape), tuple(weight.shape)))
+        M, K = weight.shape
+        if down.dim() != 3 or down.shape[2] != K or up.shape != (down.shape[0], M, down.shape[1]) or down.shape[0] < 1 or not 1 <= down.shape[1] <= 128:
+            raise RuntimeError("linear_adapted: down [n, r, %d] and up [n, %d, r] with r at most 128 expected, got %s and %s" % (K, M, tuple(down.shape), tuple(up.shape)))
+        n, r = down.shape[0], down.shape[1]
+        if bias is not None and bias.shape != (M,):
+            raise RuntimeError("linear_adapted: bias [%d] expected, got %s" % (M, tuple(bias.shape)))
+        if scale is not None:
+            if scale.shape != (n,) or scale.dtype != torch.float32:
+                raise RuntimeError("linear_adapted: scale [%d] float32 expected, got %s %s" % (n, tuple(scale.shape), scale.dtype))
+            self._dtype("linear_adapted", scale)
+            scale = scale.contiguous()
+        B, T = x.shape[0], x.shape[1] if x.dim() == 3 else 1
+        ids = self._indices("linear_adapted: ids", ids, B, -_INT_MAX, n - 1)
+        x, weight, down, up = _rows(x), weight.contiguous(), down.contiguous(), up.contiguous()
+        bias = None if bias is None else bias.contiguous()
+        y = torch.empty(*x.shape[:-1], M, device=x.device, dtype=x.dtype)
+        need = self._lib.mp_linear_adapted_workspace(B, T, r)
+        ws = torch.empty(need, device=x.device, dtype=torch.uint8)
+        st = (C.c_int64 * 2)(x.stride(0), x.stride(1) if x.dim() == 3 else 0)
+        self._check(self._lib.mp_linear_adapted(
+            self._h, dtype, x.data_ptr(), C.addressof(st), weight.data_ptr(), 0 if bias is None else bias.data_ptr(), down.data_ptr(),
+            up.data_ptr(), 0 if scale is None else scale.data_ptr(), ids.data_ptr(), B, T, K, M, n, r, int(bool(relu)), y.data_ptr(),
+            ws.data_ptr(), need, torch.cuda.current_stream(x.device).cuda_stream))
+        return y
