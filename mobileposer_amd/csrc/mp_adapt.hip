@@ -1,67 +1,293 @@
 // A linear layer over the rows of many sequences with a low-rank adapter per sequence beside the shared weight:
 //   y_n = act(W x_n + b + scale_a Up_a (Down_a x_n)),   a = ids[sequence of n]   (negative: the shared layer alone).
+// Two launches: z = scale Down x for all rows (mp_adapt_down, fp32 into the workspace), then the shared product with Up z joined
+// to it in its registers before the one rounding and the one store (mp_adapt_gemm).  Up to three operands of a product decide the arithmetic:
+// bf16 inputs go to the bf16 matrix instructions as they are; fp32 inputs as three bf16 terms each (hi + mid + lo, each the nearest
+// to what is left: all 24 bits), six products per fp32 product -- the three left out are below 2^-26 of it --, fp32 accumulation:
+// the accuracy of an fp32 sum at 16 / 6 times the rate of the fp32 matrix instructions.  (An infinite fp32 input gives NaN:
+// inf - inf in the split.)
 #include "mp_seq.h"
 
 namespace mpseq {
 
 size_t adapt_ws_floats(int B, int T, int r) { return (size_t)B * T * r; }
 
-// z [row][r] = scale_a Down_a x_row: a wave per (row, component)
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+template <class E> struct Arith;
+template <> struct Arith<bf16raw> { static constexpr int P = 1, BK = 64; };     // planes, K elements per staged tile
+template <> struct Arith<float> { static constexpr int P = 3, BK = 32; };
+
+// eight consecutive elements as P planes of bf16 (rows need no alignment: a row of odd length starts anywhere)
+template <class E> struct Oct;
+template <> struct Oct<bf16raw> {
+    u32x4 v;
+    __device__ __forceinline__ void load(const bf16raw* p) { __builtin_memcpy(&v, p, 16); }
+    __device__ __forceinline__ void load_guarded(const bf16raw* p, int n) {
+        bf16raw t[8];
+        for (int i = 0; i < 8; ++i) t[i] = i < n ? p[i] : (bf16raw)0;
+        __builtin_memcpy(&v, t, 16);
+    }
+    __device__ __forceinline__ void load_some(const bf16raw* p, int n) {
+        if (n >= 8) load(p); else load_guarded(p, n);
+    }
+    __device__ __forceinline__ float dot(const Oct<float>& z, float s) const;
+    __device__ __forceinline__ void planes(u32x4 (&o)[1]) const { o[0] = v; }
+};
+template <> struct Oct<float>;
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+// two floats -> their nearest bf16 (one word, a in the low half), and what is left of them (exact)
+static __device__ __forceinline__ unsigned take_bf16(float& a, float& b) {
+    const unsigned w = __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2){a, b}, bf16x2));
+    a -= __uint_as_float(w << 16);
+    b -= __uint_as_float(w & 0xffff0000u);
+    return w;
+}
+template <> struct Oct<float> {
+    float v[8];
+    __device__ __forceinline__ void load(const float* p) { __builtin_memcpy(v, p, 32); }
+    __device__ __forceinline__ void load_guarded(const float* p, int n) {
+        for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : 0.f;
+    }
+    __device__ __forceinline__ void load_some(const float* p, int n) {
+        if (n >= 8) load(p); else load_guarded(p, n);
+    }
+    __device__ __forceinline__ float dot(const Oct<float>& z, float s) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s = fmaf(z.v[i], v[i], s);
+        return s;
+    }
+    __device__ __forceinline__ void planes(u32x4 (&o)[3]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float a = v[2 * i], b = v[2 * i + 1];
+            o[0][i] = take_bf16(a, b);
+            o[1][i] = take_bf16(a, b);
+            o[2][i] = take_bf16(a, b);
+        }
+    }
+};
+__device__ __forceinline__ float Oct<bf16raw>::dot(const Oct<float>& z, float s) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s = fmaf(z.v[2 * i + 1], __uint_as_float(v[i] & 0xffff0000u), fmaf(z.v[2 * i], __uint_as_float(v[i] << 16), s));
+    return s;
+}
+static __device__ __forceinline__ void store4(float* p, const float (&y)[4]) { *(float4*)p = {y[0], y[1], y[2], y[3]}; }
+static __device__ __forceinline__ void store4(bf16raw* p, const float (&y)[4]) {
+    float a = y[0], b = y[1], c = y[2], d = y[3];
+    *(uint2*)p = {take_bf16(a, b), take_bf16(c, d)};
+}
+static __device__ __forceinline__ f32x4 mfma32(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+// sum of the products of planes whose orders add up to less than the number of planes that matter, the small ones first
+template <int PA, int PB>
+static __device__ __forceinline__ f32x4 mfma_planes(const u32x4 (&a)[PA], const u32x4 (&b)[PB], f32x4 c) {
+    constexpr int top = (PA > PB ? PA : PB) - 1;
+#pragma unroll
+    for (int s = top; s >= 0; --s)
+#pragma unroll
+        for (int i = 0; i <= s; ++i)
+            if (i < PA && s - i < PB) c = mfma32(a[i], b[s - i], c);
+    return c;
+}
+
+// ---------------------------------------------------------------- z = scale Down x
+// A workgroup takes up to 16 frames of one sequence -- one adapter, so the product runs on the matrix units even where the 16 rows
+// are one (a tick: the reads of Down bound it either way) --, K split over the four waves and joined through LDS.
 template <class E>
-MP_KERNEL __launch_bounds__(256) void mp_adapt_down(AdaptArgs a, long total) {
-    const long i = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (i >= total) return;
-    const int lane = threadIdx.x & 63, j = (int)(i % a.r);
-    const long row = i / a.r;
-    const int b = (int)(row / a.T), t = (int)(row % a.T), id = a.ids[b];
-    float z = 0.f;
-    if (id >= 0 && id < a.n) {
-        const E* x = (const E*)a.x + b * a.sx[0] + t * a.sx[1];
+MP_KERNEL __launch_bounds__(256) void mp_adapt_down(AdaptArgs a, int per_seq) {
+    constexpr int P = Arith<E>::P;
+    __shared__ float part[4][16][17];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, grp = lane >> 4;
+    const int b = blockIdx.x / per_seq, t0 = blockIdx.x % per_seq * 16, id = a.ids[b];
+    if (id < 0 || id >= a.n) return;                              // (the second launch reads no z of such rows)
+    const int t = t0 + col < a.T ? t0 + col : a.T - 1;
+    const E* x = (const E*)a.x + (size_t)b * a.sx[0] + (size_t)t * a.sx[1];
+    const float sc = a.scale ? a.scale[id] : 1.f;
+    for (int j0 = 0; j0 < a.r; j0 += 16) {
+        const int j = j0 + col < a.r ? j0 + col : a.r - 1;
         const E* d = (const E*)a.down + ((size_t)id * a.r + j) * a.K;
-        for (int k = lane; k < a.K; k += 64) z = fmaf(load_f(x + k), load_f(d + k), z);
-        for (int m = 1; m < 64; m <<= 1) z += __shfl_xor(z, m);
-        if (a.scale) z *= a.scale[id];
+        f32x4 acc = {};
+        int k = (wave * 4 + grp) * 8;
+#pragma unroll 2
+        for (; k - grp * 8 + 32 <= a.K; k += 128) {
+            Oct<E> ox, od;
+            u32x4 px[P], pd[P];
+            ox.load(x + k); od.load(d + k);
+            ox.planes(px); od.planes(pd);
+            acc = mfma_planes(pd, px, acc);
+        }
+        if (k - grp * 8 < a.K) {
+            const int left = a.K - k < 0 ? 0 : a.K - k;
+            Oct<E> ox, od;
+            u32x4 px[P], pd[P];
+            ox.load_some(x + k, left); od.load_some(d + k, left);
+            ox.planes(px); od.planes(pd);
+            acc = mfma_planes(pd, px, acc);
+        }
+        for (int r = 0; r < 4; ++r) part[wave][4 * grp + r][col] = acc[r];      // [component][row]
+        __syncthreads();
+        const int row = tid >> 4, c = tid & 15;
+        if (t0 + row < a.T && j0 + c < a.r)
+            a.ws[((size_t)b * a.T + t0 + row) * a.r + j0 + c] = sc * ((part[0][c][row] + part[1][c][row]) + (part[2][c][row] + part[3][c][row]));
+        __syncthreads();
     }
-    if (lane == 0) a.ws[i] = z;
 }
 
-template <class E>
-MP_KERNEL __launch_bounds__(256) void mp_adapt_rows(AdaptArgs a, long rows) {
-    __shared__ float xs[16][17], wsh[16][17];
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, m = blockIdx.y * 16 + tx;
-    const long row = (long)blockIdx.x * 16 + ty;
-    const bool rok = row < rows, mok = m < a.M;
-    const int b = rok ? (int)(row / a.T) : 0, t = rok ? (int)(row % a.T) : 0;
-    const E* x = (const E*)a.x + b * a.sx[0] + t * a.sx[1];
-    const int wm = blockIdx.y * 16 + ty;
-    const E* w = (const E*)a.w + (size_t)(wm < a.M ? wm : 0) * a.K;
-    float acc = 0.f;
-    for (int k0 = 0; k0 < a.K; k0 += 16) {
-        const int k = k0 + tx;
-        xs[ty][tx] = rok && k < a.K ? load_f(x + k) : 0.f;
-        wsh[ty][tx] = wm < a.M && k < a.K ? load_f(w + k) : 0.f;
-        __syncthreads();
-        for (int j = 0; j < 16; ++j) acc = fmaf(xs[ty][j], wsh[tx][j], acc);
-        __syncthreads();
+// ---------------------------------------------------------------- the shared product, the adapters' second half joined to it
+// A workgroup's tile is (32 MR rows of x) x (32 MC columns of y); four waves, 2 x 2, each MR x MC tiles of 16 x 16 with W as the A
+// operand (so that a lane ends with four consecutive columns of one row).  Tiles of K go through registers into LDS, rows padded by
+// 16 bytes (a 16-lane read of one K group covers every bank once); the next tile's loads are in flight while this one is
+// multiplied.
+template <class E, int MR, int MC>
+MP_KERNEL __launch_bounds__(256) void mp_adapt_gemm(AdaptArgs a, int rows, int ntr, int ntc) {
+    constexpr int P = Arith<E>::P, BK = Arith<E>::BK, UR = BK / 8, RN = 32 * MR, CM = 32 * MC, LS = BK + 8;
+    constexpr int NU = (RN + CM) * UR / 256;                      // units of eight elements that a thread stages
+    static_assert((RN + CM) * UR % 256 == 0, "whole units per thread");
+    __shared__ __align__(16) bf16raw lds[P][RN + CM][LS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, grp = lane >> 4;
+    // workgroups are dealt to the 8 XCDs in turn: a run of tiles (columns fastest: one panel of x) to each, so that an XCD's L2
+    // holds what its tiles share
+    const int nt = ntr * ntc, per = (nt + 7) / 8, tile = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
+    if (tile >= nt || (int)(blockIdx.x / 8) >= per) return;
+    const int n0 = tile / ntc * RN, m0 = tile % ntc * CM;
+    const E* src[NU];
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+        const int row = (tid + 256 * u) / UR, kk = (tid + 256 * u) % UR * 8;
+        if (row < RN) {
+            const int n = n0 + row < rows ? n0 + row : rows - 1, b = n / a.T;
+            src[u] = (const E*)a.x + (size_t)b * a.sx[0] + (size_t)(n - b * a.T) * a.sx[1] + kk;
+        } else {
+            const int m = m0 + row - RN < a.M ? m0 + row - RN : a.M - 1;
+            src[u] = (const E*)a.w + (size_t)m * a.K + kk;
+        }
     }
-    if (!rok || !mok) return;
-    if (a.bias) acc += load_f((const E*)a.bias + m);
-    const int id = a.ids[b];
-    if (id >= a.n) acc = __builtin_nanf("");
-    else if (id >= 0) {
-        const E* up = (const E*)a.up + ((size_t)id * a.M + m) * a.r;
-        const float* z = a.ws + row * a.r;
-        for (int j = 0; j < a.r; ++j) acc = fmaf(z[j], load_f(up + j), acc);
+    const int wr = wave & 1, wc = wave >> 1;
+    f32x4 acc[MC][MR] = {};
+    Oct<E> oct[NU];
+    auto fetch = [&](int k0) {
+        if (k0 + BK <= a.K) {
+#pragma unroll
+            for (int u = 0; u < NU; ++u) oct[u].load(src[u] + k0);
+        } else {
+#pragma unroll
+            for (int u = 0; u < NU; ++u) oct[u].load_guarded(src[u] + k0, a.K - k0 - (tid + 256 * u) % UR * 8);
+        }
+    };
+    fetch(0);
+    for (int k0 = 0; k0 < a.K; k0 += BK) {
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+            const int row = (tid + 256 * u) / UR, kk = (tid + 256 * u) % UR * 8;
+            u32x4 p[P];
+            oct[u].planes(p);
+#pragma unroll
+            for (int i = 0; i < P; ++i) *(u32x4*)&lds[i][row][kk] = p[i];
+        }
+        __syncthreads();
+        if (k0 + BK < a.K) fetch(k0 + BK);
+#pragma unroll
+        for (int ks = 0; ks < BK; ks += 32) {
+            u32x4 fx[MR][P];
+#pragma unroll
+            for (int i = 0; i < MR; ++i)
+#pragma unroll
+                for (int p = 0; p < P; ++p) fx[i][p] = *(const u32x4*)&lds[p][(wr * MR + i) * 16 + col][ks + 8 * grp];
+#pragma unroll
+            for (int j = 0; j < MC; ++j) {
+                u32x4 fw[P];
+#pragma unroll
+                for (int p = 0; p < P; ++p) fw[p] = *(const u32x4*)&lds[p][RN + (wc * MC + j) * 16 + col][ks + 8 * grp];
+#pragma unroll
+                for (int i = 0; i < MR; ++i) acc[j][i] = mfma_planes(fw, fx[i], acc[j][i]);
+            }
+        }
     }
-    if (a.relu) acc = relu_(acc);
-    store_f((E*)a.y + (size_t)row * a.M + m, acc);
+#pragma unroll
+    for (int i = 0; i < MR; ++i) {
+        const int nb = n0 + (wr * MR + i) * 16;                   // 16 rows, one per lane column
+        const int n = nb + col, nc = n < rows ? n : rows - 1;
+        const int id = a.ids[nc / a.T];
+        const bool use = id >= 0 && id < a.n;
+        const float* z = a.ws + (size_t)nc * a.r;
+        const int id0 = __builtin_amdgcn_readfirstlane(id);
+        if (__all(id == id0)) {
+            if (id0 >= 0 && id0 < a.n)                            // one adapter for the 16 rows: the matrix units again
+                for (int r0 = 0; r0 < a.r; r0 += 32) {
+                    const int k = r0 + 8 * grp, left = a.r - k < 0 ? 0 : a.r - k;
+                    Oct<float> oz;
+                    u32x4 p3[3], pz[P == 1 ? 2 : 3];              // z keeps 16 of its bits beside bf16 operands, all 24 beside fp32 ones
+                    oz.load_some(z + k, left);
+                    oz.planes(p3);
+#pragma unroll
+                    for (int p = 0; p < (P == 1 ? 2 : 3); ++p) pz[p] = p3[p];
+#pragma unroll
+                    for (int j = 0; j < MC; ++j) {
+                        const int m = m0 + (wc * MC + j) * 16 + col;
+                        Oct<E> ou;
+                        u32x4 pu[P];
+                        ou.load_some((const E*)a.up + ((size_t)id0 * a.M + (m < a.M ? m : 0)) * a.r + k, left);
+                        ou.planes(pu);
+                        acc[j][i] = mfma_planes(pu, pz, acc[j][i]);
+                    }
+                }
+        } else if (use) {                                         // a row of its own each: dot products of the lane's four columns
+            for (int q = 0; q < a.r; q += 8) {
+                Oct<float> oz;
+                oz.load_some(z + q, a.r - q);
+#pragma unroll
+                for (int j = 0; j < MC; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int m = m0 + (wc * MC + j) * 16 + 4 * grp + r;
+                        Oct<E> ou;
+                        ou.load_some((const E*)a.up + ((size_t)id * a.M + (m < a.M ? m : 0)) * a.r + q, a.r - q);
+                        acc[j][i][r] = ou.dot(oz, acc[j][i][r]);
+                    }
+            }
+        }
+        if (n >= rows) continue;
+#pragma unroll
+        for (int j = 0; j < MC; ++j) {
+            const int m = m0 + (wc * MC + j) * 16 + 4 * grp;
+            float y[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                y[r] = acc[j][i][r] + (a.bias && m + r < a.M ? load_f((const E*)a.bias + m + r) : 0.f);
+                if (id >= a.n) y[r] = __builtin_nanf("");
+                if (a.relu) y[r] = relu_(y[r]);
+            }
+            E* out = (E*)a.y + (size_t)n * a.M + m;
+            if (a.vec) {                                          // M a multiple of 4: whole groups of columns, aligned
+                if (m < a.M) store4(out, y);
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (m + r < a.M) store_f(out + r, y[r]);
+            }
+        }
+    }
 }
 
+template <class E, int MR, int MC>
+static void gemm_for(const AdaptArgs& a, int rows, hipStream_t s) {
+    const int ntr = (rows + 32 * MR - 1) / (32 * MR), ntc = (a.M + 32 * MC - 1) / (32 * MC);
+    hipLaunchKernelGGL((mp_adapt_gemm<E, MR, MC>), dim3((unsigned)((ntr * ntc + 7) / 8 * 8)), dim3(256), 0, s, a, rows, ntr, ntc);
+}
 template <class E>
-static bool launch_for(const AdaptArgs& a, hipStream_t s) {
-    const long rows = (long)a.B * a.T, total = rows * a.r;
-    hipLaunchKernelGGL(mp_adapt_down<E>, dim3((unsigned)((total + 3) / 4)), dim3(256), 0, s, a, total);
-    hipLaunchKernelGGL(mp_adapt_rows<E>, dim3((unsigned)((rows + 15) / 16), (unsigned)((a.M + 15) / 16)), dim3(256), 0, s, a, rows);
+static bool launch_for(AdaptArgs a, hipStream_t s) {
+    const int rows = a.B * a.T;
+    a.vec = a.M % 4 == 0 && (uintptr_t)a.y % (4 * sizeof(E)) == 0;
+    hipLaunchKernelGGL(mp_adapt_down<E>, dim3((unsigned)(a.B * ((a.T + 15) / 16))), dim3(256), 0, s, a, (a.T + 15) / 16);
+    auto tiles = [&](int t) { return ((long)rows + t - 1) / t * ((a.M + t - 1) / t); };
+    if (tiles(128) >= 192) gemm_for<E, 4, 4>(a, rows, s);
+    else if (tiles(64) >= 192) gemm_for<E, 2, 2>(a, rows, s);
+    else gemm_for<E, 1, 1>(a, rows, s);
     return hipGetLastError() == hipSuccess;
 }
 bool launch_adapt(const AdaptArgs& a, int dtype, hipStream_t s) {

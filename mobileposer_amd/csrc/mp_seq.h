@@ -58,6 +58,7 @@ struct AdaptArgs {
     int B, T, K, M, n, r, relu;
     void* y;                                     // [B][T][M] contiguous
     float* ws;                                   // [B*T][r] fp32
+    bool vec;                                    // (set by the launcher) groups of four columns of y can be stored at once
 };
 size_t adapt_ws_floats(int B, int T, int r);
 bool launch_adapt(const AdaptArgs& a, int dtype, hipStream_t s);
