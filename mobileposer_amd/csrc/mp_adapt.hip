@@ -6,93 +6,11 @@
 // to what is left: all 24 bits), six products per fp32 product -- the three left out are below 2^-26 of it --, fp32 accumulation:
 // the accuracy of an fp32 sum at 16 / 6 times the rate of the fp32 matrix instructions.  (An infinite fp32 input gives NaN:
 // inf - inf in the split.)
-#include "mp_seq.h"
+#include "mp_seq_dev.h"
 
 namespace mpseq {
 
 size_t adapt_ws_floats(int B, int T, int r) { return (size_t)B * T * r; }
-
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-
-template <class E> struct Arith;
-template <> struct Arith<bf16raw> { static constexpr int P = 1, BK = 64; };     // planes, K elements per staged tile
-template <> struct Arith<float> { static constexpr int P = 3, BK = 32; };
-
-// eight consecutive elements as P planes of bf16 (rows need no alignment: a row of odd length starts anywhere)
-template <class E> struct Oct;
-template <> struct Oct<bf16raw> {
-    u32x4 v;
-    __device__ __forceinline__ void load(const bf16raw* p) { __builtin_memcpy(&v, p, 16); }
-    __device__ __forceinline__ void load_guarded(const bf16raw* p, int n) {
-        bf16raw t[8];
-        for (int i = 0; i < 8; ++i) t[i] = i < n ? p[i] : (bf16raw)0;
-        __builtin_memcpy(&v, t, 16);
-    }
-    __device__ __forceinline__ void load_some(const bf16raw* p, int n) {
-        if (n >= 8) load(p); else load_guarded(p, n);
-    }
-    __device__ __forceinline__ float dot(const Oct<float>& z, float s) const;
-    __device__ __forceinline__ void planes(u32x4 (&o)[1]) const { o[0] = v; }
-};
-template <> struct Oct<float>;
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-// two floats -> their nearest bf16 (one word, a in the low half), and what is left of them (exact)
-static __device__ __forceinline__ unsigned take_bf16(float& a, float& b) {
-    const unsigned w = __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2){a, b}, bf16x2));
-    a -= __uint_as_float(w << 16);
-    b -= __uint_as_float(w & 0xffff0000u);
-    return w;
-}
-template <> struct Oct<float> {
-    float v[8];
-    __device__ __forceinline__ void load(const float* p) { __builtin_memcpy(v, p, 32); }
-    __device__ __forceinline__ void load_guarded(const float* p, int n) {
-        for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : 0.f;
-    }
-    __device__ __forceinline__ void load_some(const float* p, int n) {
-        if (n >= 8) load(p); else load_guarded(p, n);
-    }
-    __device__ __forceinline__ float dot(const Oct<float>& z, float s) const {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s = fmaf(z.v[i], v[i], s);
-        return s;
-    }
-    __device__ __forceinline__ void planes(u32x4 (&o)[3]) const {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float a = v[2 * i], b = v[2 * i + 1];
-            o[0][i] = take_bf16(a, b);
-            o[1][i] = take_bf16(a, b);
-            o[2][i] = take_bf16(a, b);
-        }
-    }
-};
-__device__ __forceinline__ float Oct<bf16raw>::dot(const Oct<float>& z, float s) const {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s = fmaf(z.v[2 * i + 1], __uint_as_float(v[i] & 0xffff0000u), fmaf(z.v[2 * i], __uint_as_float(v[i] << 16), s));
-    return s;
-}
-static __device__ __forceinline__ void store4(float* p, const float (&y)[4]) { *(float4*)p = {y[0], y[1], y[2], y[3]}; }
-static __device__ __forceinline__ void store4(bf16raw* p, const float (&y)[4]) {
-    float a = y[0], b = y[1], c = y[2], d = y[3];
-    *(uint2*)p = {take_bf16(a, b), take_bf16(c, d)};
-}
-static __device__ __forceinline__ f32x4 mfma32(u32x4 a, u32x4 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-// sum of the products of planes whose orders add up to less than the number of planes that matter, the small ones first
-template <int PA, int PB>
-static __device__ __forceinline__ f32x4 mfma_planes(const u32x4 (&a)[PA], const u32x4 (&b)[PB], f32x4 c) {
-    constexpr int top = (PA > PB ? PA : PB) - 1;
-#pragma unroll
-    for (int s = top; s >= 0; --s)
-#pragma unroll
-        for (int i = 0; i <= s; ++i)
-            if (i < PA && s - i < PB) c = mfma32(a[i], b[s - i], c);
-    return c;
-}
 
 // ---------------------------------------------------------------- z = scale Down x
 // A workgroup takes up to 16 frames of one sequence -- one adapter, so the product runs on the matrix units even where the 16 rows
@@ -144,7 +62,7 @@ MP_KERNEL __launch_bounds__(256) void mp_adapt_down(AdaptArgs a, int per_seq) {
 // multiplied.
 template <class E, int MR, int MC>
 MP_KERNEL __launch_bounds__(256) void mp_adapt_gemm(AdaptArgs a, int rows, int ntr, int ntc) {
-    constexpr int P = Arith<E>::P, BK = Arith<E>::BK, UR = BK / 8, RN = 32 * MR, CM = 32 * MC, LS = BK + 8;
+    constexpr int P = Arith<E>::P, BK = P == 1 ? 64 : 32, UR = BK / 8, RN = 32 * MR, CM = 32 * MC, LS = BK + 8;
     constexpr int NU = (RN + CM) * UR / 256;                      // units of eight elements that a thread stages
     static_assert((RN + CM) * UR % 256 == 0, "whole units per thread");
     __shared__ __align__(16) bf16raw lds[P][RN + CM][LS];

@@ -15,18 +15,24 @@
 // A value that is not finite reaches the frames behind it only, as in the recurrence: where a right-hand side holds one, the
 // rows from there on are taken out of the products (0 * NaN in a triangular matrix's zeros would reach the frames before it)
 // and their outputs and the column's state are NaN.
-#include "mp_seq.h"
+#include "mp_seq_dev.h"
 
 namespace mpseq {
 
 constexpr int kC = 32;                            // frames per chunk
-// workspace of one (sequence, value head, chunk), floats: T = (I + A)^{-1} and P = scale tril(Q K^T) o D as three 16 x 16 tiles
-// (0,0), (1,0), (1,1) each, in the order in which a lane of v_mfma_f32_16x16x4_f32 takes its A operand
-// ([tile][lane][4]: row lane & 15, columns 4 (lane >> 4) .. +3), then beta_i, e^{G_i}, e^{G_C - G_i}
-constexpr int kTile = 256;
-constexpr int kWsP = 3 * kTile, kWsBeta = 6 * kTile, kWsEg = kWsBeta + kC, kWsTail = kWsEg + kC, kWsUnit = kWsTail + kC;
+// Workspace of one (sequence, value head, chunk), bytes: T = (I + A)^{-1} as three terms and P = scale tril(Q K^T) o D as two (bf16
+// outputs) or three, in the order in which a lane of v_mfma_f32_16x16x32_bf16 takes its A operand, then beta, e^G, e^{G_C - G}.
+constexpr int kFrag = 1024;                       // one 16 x 32 operand: 64 lanes x 8 bf16
+constexpr int kWsP = 6 * kFrag, kWsBeta = 12 * kFrag, kWsEg = kWsBeta + 4 * kC, kWsTail = kWsEg + 4 * kC, kWsUnit = kWsTail + 4 * kC;
 
-size_t delta_ws_floats(int B, int T, int Hv) { return (size_t)B * Hv * ((T + kC - 1) / kC) * kWsUnit; }
+size_t delta_ws_floats(int B, int T, int Hv) { return (size_t)B * Hv * ((T + kC - 1) / kC) * (kWsUnit / 4); }
+
+// Which frame and which component of k a lane's registers stand for.  The accumulator layout of a 16 x 16 tile (lane: column
+// lane % 16, rows 4 (lane / 16) + r) becomes the B operand of a K = 32 instruction (lane: column lane % 16, k slots
+// 8 (lane / 16) + 0..7) by putting two tiles h = 0, 1 side by side: row 4 g + r of tile h is index 8 g + 4 h + r of 32.  So the
+// state (32 components per pair of tiles), the right-hand sides and U (32 frames per pair) go from one product into the next
+// without leaving their lanes; the A operands take their rows in the same order.
+static __device__ __forceinline__ int row_index(int h, int row) { return 8 * (row >> 2) + 4 * h + (row & 3); }
 
 static __device__ __forceinline__ int length_of(const int* lengths, int b, int T) {
     if (!lengths) return T;
@@ -36,237 +42,387 @@ static __device__ __forceinline__ int length_of(const int* lengths, int b, int T
 static __device__ __forceinline__ float clamp_g(float g) { return g < -1e4f ? -1e4f : g; }      // (NaN stays NaN)
 static __device__ __forceinline__ bool not_finite(float x) { return !(fabsf(x) <= 3.402823466e38f); }
 
-// 16 x 16 tile of X Y^T over dk: X rows x0 + l%16, Y rows y0 + l%16 of one head; any order of k serves as long as both take it
 template <class E>
-static __device__ __forceinline__ float4 row4(const E* p, int d, int dk, bool on) {
-    float4 r;
-    r.x = on && d + 0 < dk ? load_f(p + d + 0) : 0.f;
-    r.y = on && d + 1 < dk ? load_f(p + d + 1) : 0.f;
-    r.z = on && d + 2 < dk ? load_f(p + d + 2) : 0.f;
-    r.w = on && d + 3 < dk ? load_f(p + d + 3) : 0.f;
-    return r;
-}
-static __device__ __forceinline__ f32x4 mfma4(float4 a, float4 b, f32x4 c) {
-    c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.x, b.x, c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.y, b.y, c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.z, b.z, c, 0, 0, 0);
-    return __builtin_amdgcn_mfma_f32_16x16x4f32(a.w, b.w, c, 0, 0, 0);
+static __device__ __forceinline__ void load_row(Oct<E>& o, const E* p, int d, int dk, bool on) {      // components d .. d + 7 of a row
+    if (on && d < dk) o.load_some(p + d, dk - d); else o.zero();
 }
 
-// One wave per (sequence, key head, chunk): K K^T and Q K^T once, then the value heads that share the key head.
-template <class E>
+// One wave per (sequence, key head, chunk): K K^T and Q K^T once, then the value heads that share the key head, two at a time --
+// a lane of either half solves a column of (I + A) T = I by forward substitution (stable where keys repeat and A is far from
+// small; products of powers of A are not).
+template <class E, int PO>
 MP_KERNEL __launch_bounds__(64) void mp_delta_prep(DeltaArgs a) {
-    __shared__ float A[kC][kC + 1];
+    constexpr int P = Arith<E>::P, LS = kC + 4;
+    __shared__ __align__(16) float A[2][kC][LS], W[kC][LS];
     const int unit = blockIdx.x, c = unit % a.nchunk, hk = unit / a.nchunk % a.Hk, b = unit / a.nchunk / a.Hk;
-    const int lane = threadIdx.x, col = lane & 15, grp = lane >> 4, t0 = c * kC;
+    const int lane = threadIdx.x, col = lane & 15, grp = lane >> 4, half = lane >> 5, i = lane & 31, t0 = c * kC;
     const int len = length_of(a.lengths, b, a.T);
     if (t0 >= len) return;
     const E* q = (const E*)a.q + b * a.sq[0] + hk * a.sq[2];
     const E* k = (const E*)a.k + b * a.sk[0] + hk * a.sk[2];
-    f32x4 kk[3] = {}, qk[3] = {};
-    for (int d = 4 * grp; d - 4 * grp < a.dk; d += 16) {
-        float4 fk[2], fq[2];
+    f32x4 kk[3] = {}, qk[3] = {};                 // tiles (0,0), (1,0), (1,1) of frames 16 I + row, 16 J + column
+    for (int d0 = 0; d0 < a.dk; d0 += 32) {
+        u32x4 fk[2][P], fq[2][P];
+#pragma unroll
         for (int I = 0; I < 2; ++I) {
             const int t = t0 + 16 * I + col;
             const bool on = t < len;
-            fk[I] = row4(k + (on ? t : 0) * a.sk[1], d, a.dk, on);
-            fq[I] = row4(q + (on ? t : 0) * a.sq[1], d, a.dk, on);
+            Oct<E> ok, oq;
+            load_row(ok, k + (on ? t : 0) * a.sk[1], d0 + 8 * grp, a.dk, on);
+            load_row(oq, q + (on ? t : 0) * a.sq[1], d0 + 8 * grp, a.dk, on);
+            ok.planes(fk[I]);
+            oq.planes(fq[I]);
         }
-        kk[0] = mfma4(fk[0], fk[0], kk[0]);
-        kk[1] = mfma4(fk[1], fk[0], kk[1]);
-        kk[2] = mfma4(fk[1], fk[1], kk[2]);
-        qk[0] = mfma4(fq[0], fk[0], qk[0]);
-        qk[1] = mfma4(fq[1], fk[0], qk[1]);
-        qk[2] = mfma4(fq[1], fk[1], qk[2]);
+#pragma unroll
+        for (int n = 0; n < 3; ++n) {
+            kk[n] = mfma_planes(fk[n > 0], fk[n > 1], kk[n]);
+            qk[n] = mfma_planes(fq[n > 0], fk[n > 1], qk[n]);
+        }
     }
-    const int rep = a.Hv / a.Hk;
-    for (int e = 0; e < rep; ++e) {
-        const int hv = hk * rep + e;
-        float* ws = a.ws + ((size_t)(b * a.Hv + hv) * a.nchunk + c) * kWsUnit;
-        const int i = lane & 31, t = t0 + i;
-        const bool on = t < len;
-        const float beta = on ? a.beta[b * a.sb[0] + t * a.sb[1] + hv * a.sb[2]] : 0.f;
-        double G = on ? (double)clamp_g(a.g[b * a.sg[0] + t * a.sg[1] + hv * a.sg[2]]) : 0.0;
+    const int rep = a.Hv / a.Hk, t = t0 + i;
+    const bool on = t < len;
+    for (int e0 = 0; e0 < rep; e0 += 2) {
+        const int two = min(2, rep - e0), hh = hk * rep + e0 + min(half, two - 1);
+        const float beta = on ? a.beta[b * a.sb[0] + t * a.sb[1] + hh * a.sb[2]] : 0.f;
+        double G = on ? (double)clamp_g(a.g[b * a.sg[0] + t * a.sg[1] + hh * a.sg[2]]) : 0.0;
+#pragma unroll
         for (int s = 1; s < kC; s <<= 1) {
             const double up = __shfl_up(G, s, 32);
             if (i >= s) G += up;
         }
         const double last = __shfl(G, kC - 1, 32);
-        if (lane < kC) {
-            ws[kWsBeta + i] = beta;
-            ws[kWsEg + i] = expf((float)G);
-            ws[kWsTail + i] = expf((float)(last - G));
+        if (half < two) {
+            char* ws = (char*)a.ws + ((size_t)(b * a.Hv + hh) * a.nchunk + c) * kWsUnit;
+            ((float*)(ws + kWsBeta))[i] = beta;
+            ((float*)(ws + kWsEg))[i] = expf((float)G);
+            ((float*)(ws + kWsTail))[i] = expf((float)(last - G));
         }
-        // D layout of an accumulator: row 4 grp + r, column col
-        for (int tile = 0; tile < 3; ++tile) {
-            const int I = tile > 0, J = tile > 1;
-            const double Gj = __shfl(G, 16 * J + col, 64);
-            for (int r = 0; r < 4; ++r) {
-                const int ri = 16 * I + 4 * grp + r, cj = 16 * J + col;
-                const float D = expf((float)(__shfl(G, ri, 64) - Gj));
-                const float bi = __shfl(beta, ri, 64);
-                A[ri][cj] = cj < ri ? bi * D * kk[tile][r] : 0.f;
-                // P in operand order: lane (row & 15) + 16 (column / 4 within the tile), element column % 4
-                ws[kWsP + tile * kTile + ((ri & 15) + 16 * (col >> 2)) * 4 + (col & 3)] = cj <= ri ? a.scale * D * qk[tile][r] : 0.f;
+        for (int e = 0; e < two; ++e) {
+            char* ws = (char*)a.ws + ((size_t)(b * a.Hv + hk * rep + e0 + e) * a.nchunk + c) * kWsUnit;
+            __syncthreads();
+#pragma unroll
+            for (int tile = 0; tile < 3; ++tile) {
+                const double Gj = __shfl(G, 32 * e + 16 * (tile > 1) + col);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int ri = 16 * (tile > 0) + 4 * grp + r, cj = 16 * (tile > 1) + col;
+                    const float D = expf((float)(__shfl(G, 32 * e + ri) - Gj));
+                    const float bi = __shfl(beta, 32 * e + ri);
+                    A[e][cj][ri] = cj < ri ? bi * D * kk[tile][r] : 0.f;
+                    W[ri][cj] = cj <= ri ? a.scale * D * qk[tile][r] : 0.f;
+                }
+            }
+            for (int r = 0; r < 4; ++r) W[4 * grp + r][16 + col] = 0.f;
+            __syncthreads();
+#pragma unroll
+            for (int I = 0; I < 2; ++I) {
+                Oct<float> o;
+                u32x4 p[3];
+                o.load(&W[row_index(I, col)][8 * grp]);
+                o.planes(p);
+#pragma unroll
+                for (int n = 0; n < PO; ++n) *(u32x4*)(ws + kWsP + (I * PO + n) * kFrag + lane * 16) = p[n];
             }
         }
-        __syncthreads();
-        // T = (I + A)^{-1} by forward substitution, lane = column
+        const int mine = min(half, two - 1);
         float x[kC];
-        for (int n = 0; n < kC; ++n) {
-            float s = n == i ? 1.f : 0.f;
-            for (int j = 0; j < n; ++j) s -= j < i ? 0.f : A[n][j] * x[j];
-            x[n] = n < i ? 0.f : s;
+#pragma unroll
+        for (int n = 0; n < kC; ++n) x[n] = n == i ? 1.f : 0.f;
+        float4 now[kC / 4], next[kC / 4];         // column n of A, rows n + 1 .. : on its way while column n - 1 is used
+#pragma unroll
+        for (int m = 0; m < kC / 4; ++m) next[m] = *(const float4*)&A[mine][0][4 * m];
+#pragma unroll
+        for (int n = 0; n < kC - 1; ++n) {
+
+#pragma unroll
+            for (int m = n / 4; m < kC / 4; ++m) now[m] = next[m];
+#pragma unroll
+            for (int m = (n + 1) / 4; m < kC / 4; ++m) next[m] = *(const float4*)&A[mine][n + 1][4 * m];
+            if (n < i) x[n] = 0.f;                // (not 0 * NaN where an earlier frame's row is not finite)
+#pragma unroll
+            for (int j = n + 1; j < kC; ++j) x[j] = fmaf(-((const float*)now)[j], x[n], x[j]);
         }
-        if (lane < kC) {
-            const int J = i >> 4, cc = i & 15;
-            for (int n = 0; n < kC; ++n) {
-                const int I = n >> 4;
-                if (I >= J) ws[(I + J) * kTile + ((n & 15) + 16 * (cc >> 2)) * 4 + (cc & 3)] = x[n];
+        if (kC - 1 < i) x[kC - 1] = 0.f;
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < kC; ++n) A[half][n][i] = x[n];        // (with one head left, the other half's copy is not read)
+        __syncthreads();
+        for (int e = 0; e < two; ++e) {
+            char* ws = (char*)a.ws + ((size_t)(b * a.Hv + hk * rep + e0 + e) * a.nchunk + c) * kWsUnit;
+#pragma unroll
+            for (int I = 0; I < 2; ++I) {
+                Oct<float> o;
+                u32x4 p[3];
+                o.load(&A[e][row_index(I, col)][8 * grp]);
+                o.planes(p);
+#pragma unroll
+                for (int n = 0; n < 3; ++n) *(u32x4*)(ws + (I * 3 + n) * kFrag + lane * 16) = p[n];
             }
         }
-        __syncthreads();
     }
 }
 
-// One wave per (sequence, value head, 16 columns of the state): the walk over the chunks.  NK = dk / 16 rounded up.
-// The accumulator layout (row 4 grp + r, column col) of a tile IS the B operand of four v_mfma_f32_16x16x4_f32 when their k
-// slots are taken as rows 4 grp + r of step r, so the state, the right-hand sides and U never leave their registers.
+// The walk over the chunks: a workgroup per (sequence, value head, 64 columns of the state), a wave per 16 columns; NK = dk / 32
+// rounded up.  The workgroup stages K, Q and K^T of a chunk in LDS as ready operands (bf16 terms, one 16-byte read per lane and
+// operand), the next chunk's rows are on their way through registers meanwhile.
 template <class E, int NK>
-MP_KERNEL __launch_bounds__(64) void mp_delta_scan(DeltaArgs a, int ncol) {
-    const int lane = threadIdx.x, col = lane & 15, grp = lane >> 4;
-    const int ct = blockIdx.x % ncol, hv = blockIdx.x / ncol % a.Hv, b = blockIdx.x / ncol / a.Hv;
-    const int hk = hv / (a.Hv / a.Hk);
-    const int cv = 16 * ct + col;
-    const bool cok = cv < a.dv;
+struct ScanLds {
+    static constexpr int P = Arith<E>::P, kPlane = 2 * NK * kFrag, kOne = 3 * P * kPlane;      // K | Q | K^T, P planes each
+    static constexpr bool kTwo = 2 * kOne <= 160 * 1024;
+    static constexpr int kBytes = kTwo ? 2 * kOne : kOne;
+};
+template <class E, int NK>
+struct Rows {                                     // what a thread stages of a chunk
+    static constexpr int P = Arith<E>::P, NO = (4 * NK + 7) / 8, NP = (16 * NK + 63) / 64;
+    Oct<E> k[NO], q[NO];
+    E kt[NP][2][8];
+    __device__ __forceinline__ void load(const DeltaArgs& a, const E* kp, const E* qp, int t0, int len) {
+        const int tid = threadIdx.x, t = t0 + (tid & 31);
+        const bool on = t < len;
+#pragma unroll
+        for (int n = 0; n < NO; ++n) {
+            const int d = 8 * ((tid >> 5) + 8 * n);
+            load_row(k[n], kp + (on ? t : 0) * a.sk[1], d, a.dk, on);
+            load_row(q[n], qp + (on ? t : 0) * a.sq[1], d, a.dk, on);
+        }
+#pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            const int d = 2 * ((tid >> 2) + 64 * n), tt = t0 + 8 * (tid & 3);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const E* p = kp + (tt + j < len ? tt + j : 0) * a.sk[1] + d;
+                E two[2] = {0, 0};
+                if (tt + j < len && d + 1 < a.dk) __builtin_memcpy(two, p, sizeof(two));
+                else if (tt + j < len && d < a.dk) two[0] = *p;
+                kt[n][0][j] = two[0];
+                kt[n][1][j] = two[1];
+            }
+        }
+    }
+    __device__ __forceinline__ void store(char* lds) const {
+        using L = ScanLds<E, NK>;
+        const int tid = threadIdx.x, t = tid & 31, row = 4 * (t >> 3) + (t & 3), I = t >> 2 & 1;
+#pragma unroll
+        for (int n = 0; n < NO; ++n) {
+            const int o = (tid >> 5) + 8 * n;
+            if (o < 4 * NK) {
+                u32x4 pk[P], pq[P];
+                k[n].planes(pk);
+                q[n].planes(pq);
+                char* at = lds + (2 * (o >> 2) + I) * kFrag + (row + 16 * (o & 3)) * 16;
+#pragma unroll
+                for (int p = 0; p < P; ++p) {
+                    *(u32x4*)(at + p * L::kPlane) = pk[p];
+                    *(u32x4*)(at + (P + p) * L::kPlane) = pq[p];
+                }
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            const int d = 2 * ((tid >> 2) + 64 * n);
+            if (d < 32 * NK)
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const int dd = d + x, tile = 2 * (dd >> 5) + (dd >> 2 & 1), rw = 4 * (dd >> 3 & 3) + (dd & 3);
+                    Oct<E> o;
+                    u32x4 pt[P];
+                    __builtin_memcpy(&o.v, kt[n][x], sizeof(o.v));
+                    o.planes(pt);
+#pragma unroll
+                    for (int p = 0; p < P; ++p) *(u32x4*)(lds + (2 * P + p) * L::kPlane + tile * kFrag + (rw + 16 * (tid & 3)) * 16) = pt[p];
+                }
+        }
+    }
+};
+static __device__ __forceinline__ u32x4 operand(const char* p, int lane) { return *(const u32x4*)(p + lane * 16); }
+
+template <class E, int NK>
+MP_KERNEL __launch_bounds__(256) void mp_delta_scan(DeltaArgs a, int ncol) {
+    using L = ScanLds<E, NK>;
+    constexpr int P = Arith<E>::P, PO = P == 1 ? 2 : 3;
+    extern __shared__ __align__(16) char scan_lds[];
+    char* const lds = scan_lds;
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, grp = lane >> 4;
+    // the workgroups that read the same K and Q on one XCD (workgroups are dealt to the 8 of them in turn)
+    const int rep = a.Hv / a.Hk, inner = rep * ncol, rest = blockIdx.x >> 3, unit = rest / inner * 8 + (blockIdx.x & 7);
+    if (unit >= a.B * a.Hk) return;
+    const int hk = unit % a.Hk, b = unit / a.Hk, hv = hk * rep + rest % inner / ncol;
+    const int cv = 64 * (rest % ncol) + 16 * (tid >> 6) + col;
+    const bool cok = cv < a.dv, live = 64 * (rest % ncol) + 16 * (tid >> 6) < a.dv;      // (live: the wave has a column)
     const int len = length_of(a.lengths, b, a.T);
     const E* q = (const E*)a.q + b * a.sq[0] + hk * a.sq[2];
     const E* k = (const E*)a.k + b * a.sk[0] + hk * a.sk[2];
-    const E* v = (const E*)a.v + b * a.sv[0] + hv * a.sv[2] + cv;
+    const E* v = (const E*)a.v + b * a.sv[0] + hv * a.sv[2] + (cok ? cv : 0);
     E* o = (E*)a.o + ((size_t)b * a.T * a.Hv + hv) * a.dv + cv;
     const size_t so = (size_t)a.Hv * a.dv;
     const size_t sbase = (size_t)(b * a.Hv + hv) * a.dk * a.dv + cv;
-    f32x4 S[NK];
+    f32x4 S[2 * NK];
 #pragma unroll
-    for (int n = 0; n < NK; ++n)
+    for (int n = 0; n < 2 * NK; ++n)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int d = 16 * n + 4 * grp + r;
+            const int d = 32 * (n >> 1) + row_index(n & 1, 4 * grp + r);
             S[n][r] = a.s_in && cok && d < a.dk ? a.s_in[sbase + (size_t)d * a.dv] : 0.f;
         }
-    const float nan = __builtin_nanf("");
-    for (int c = 0; c * kC < len; ++c) {
-        const float* ws = a.ws + ((size_t)(b * a.Hv + hv) * a.nchunk + c) * kWsUnit;
-        const int t0 = c * kC;
-        f32x4 ks[2] = {}, qs[2] = {};
+    auto load_v = [&](float (&vv)[8], int t0) {
 #pragma unroll
-        for (int n = 0; n < NK; ++n) {
-            const float4 s4 = {S[n][0], S[n][1], S[n][2], S[n][3]};
+        for (int j = 0; j < 8; ++j) {
+            const int t = t0 + 8 * grp + j;
+            vv[j] = cok && t < len ? load_f(v + (size_t)t * a.sv[1]) : 0.f;
+        }
+    };
+    const float nan = __builtin_nanf("");
+    Rows<E, NK> rows;
+    float vnext[8];
+    if (len > 0) {
+        rows.load(a, k, q, 0, len);
+        load_v(vnext, 0);
+        rows.store(lds);
+    }
+    __syncthreads();
+    for (int c = 0; c * kC < len; ++c) {
+        const char* ws = (const char*)a.ws + ((size_t)(b * a.Hv + hv) * a.nchunk + c) * kWsUnit;
+        const int t0 = c * kC;
+        const bool more = t0 + kC < len;
+        float vv[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) vv[j] = vnext[j];
+        if (more) {
+            rows.load(a, k, q, t0 + kC, len);
+            load_v(vnext, t0 + kC);
+        }
+        const char* buf = lds + (L::kTwo ? (c & 1) * L::kOne : 0);
+        if (live) {
+            u32x4 T[2][3], Pm[2][PO];
+            float beta[8], eg[8], tail[8];
+#pragma unroll
             for (int I = 0; I < 2; ++I) {
-                const int t = t0 + 16 * I + col;
-                const bool on = t < len;
-                ks[I] = mfma4(row4(k + (on ? t : 0) * a.sk[1], 16 * n + 4 * grp, a.dk, on), s4, ks[I]);
-                qs[I] = mfma4(row4(q + (on ? t : 0) * a.sq[1], 16 * n + 4 * grp, a.dk, on), s4, qs[I]);
+#pragma unroll
+                for (int p = 0; p < 3; ++p) T[I][p] = operand(ws + (I * 3 + p) * kFrag, lane);
+#pragma unroll
+                for (int p = 0; p < PO; ++p) Pm[I][p] = operand(ws + kWsP + (I * PO + p) * kFrag, lane);
             }
-        }
-        float4 R[2];
-        bool bad = false;
-        for (int I = 0; I < 2; ++I) {
-            float rr[4];
-            for (int r = 0; r < 4; ++r) {
-                const int i = 16 * I + 4 * grp + r, t = t0 + i;
-                const float vv = cok && t < len ? load_f(v + (size_t)t * a.sv[1]) : 0.f;
-                rr[r] = ws[kWsBeta + i] * (vv - ws[kWsEg + i] * ks[I][r]);
-                bad |= not_finite(rr[r]);
+            __builtin_memcpy(beta, __builtin_assume_aligned(ws + kWsBeta + 32 * grp, 16), 32);
+            __builtin_memcpy(eg, __builtin_assume_aligned(ws + kWsEg + 32 * grp, 16), 32);
+            __builtin_memcpy(tail, __builtin_assume_aligned(ws + kWsTail + 32 * grp, 16), 32);
+            const float whole = *(const float*)(ws + kWsEg + 4 * (kC - 1));
+            f32x4 ks[2] = {}, qs[2] = {};
+#pragma unroll
+            for (int m = 0; m < NK; ++m) {
+                Oct<float> os;
+                u32x4 sp[3], s2[PO];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) os.v[j] = S[2 * m + (j >> 2)][j & 3];
+                os.planes(sp);
+#pragma unroll
+                for (int p = 0; p < PO; ++p) s2[p] = sp[p];
+#pragma unroll
+                for (int I = 0; I < 2; ++I) {
+                    u32x4 fk[P], fq[P];
+#pragma unroll
+                    for (int p = 0; p < P; ++p) {
+                        fk[p] = operand(buf + p * L::kPlane + (2 * m + I) * kFrag, lane);
+                        fq[p] = operand(buf + (P + p) * L::kPlane + (2 * m + I) * kFrag, lane);
+                    }
+                    ks[I] = mfma_planes(fk, sp, ks[I]);
+                    qs[I] = mfma_planes(fq, s2, qs[I]);
+                }
             }
-            R[I] = {rr[0], rr[1], rr[2], rr[3]};
-        }
-        int first = kC;                                            // this column's first row that is not finite
-        const bool any_bad = __any(bad);
-        if (any_bad) {
-            for (int I = 1; I >= 0; --I)
-                for (int r = 3; r >= 0; --r)
-                    if (not_finite(((const float*)&R[I])[r])) first = 16 * I + 4 * grp + r;
-            first = min(first, __shfl_xor(first, 16));
-            first = min(first, __shfl_xor(first, 32));
-            for (int I = 0; I < 2; ++I)
-                for (int r = 0; r < 4; ++r)
-                    if (16 * I + 4 * grp + r >= first) ((float*)&R[I])[r] = 0.f;
-        }
-        const float4* T4 = (const float4*)ws;
-        const float4* P4 = (const float4*)(ws + kWsP);
-        f32x4 u[2] = {}, w[2] = {};
-        u[0] = mfma4(T4[lane], R[0], u[0]);
-        u[1] = mfma4(T4[64 + lane], R[0], u[1]);
-        u[1] = mfma4(T4[128 + lane], R[1], u[1]);
-        if (any_bad)
-            for (int I = 0; I < 2; ++I)
-                for (int r = 0; r < 4; ++r)
-                    if (16 * I + 4 * grp + r >= first) u[I][r] = 0.f;
-        const float4 u0 = {u[0][0], u[0][1], u[0][2], u[0][3]}, u1 = {u[1][0], u[1][1], u[1][2], u[1][3]};
-        w[0] = mfma4(P4[lane], u0, w[0]);
-        w[1] = mfma4(P4[64 + lane], u0, w[1]);
-        w[1] = mfma4(P4[128 + lane], u1, w[1]);
-        for (int I = 0; I < 2; ++I)
-            for (int r = 0; r < 4; ++r) {
-                const int i = 16 * I + 4 * grp + r, t = t0 + i;
-                float ov = a.scale * ws[kWsEg + i] * qs[I][r] + w[I][r];
-                if (i >= first) ov = nan;
+            Oct<float> R;
+            bool bad = false;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                R.v[j] = beta[j] * fmaf(-eg[j], ks[j >> 2][j & 3], vv[j]);
+                bad |= not_finite(R.v[j]);
+            }
+            int first = kC;                                        // this column's first row that is not finite
+            const bool any_bad = __any(bad);
+            if (any_bad) {
+#pragma unroll
+                for (int j = 7; j >= 0; --j)
+                    if (not_finite(R.v[j])) first = 8 * grp + j;
+                first = min(first, __shfl_xor(first, 16));
+                first = min(first, __shfl_xor(first, 32));
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (8 * grp + j >= first) R.v[j] = 0.f;
+            }
+            u32x4 rp[3];
+            R.planes(rp);
+            f32x4 u[2] = {}, w[2] = {};
+            u[0] = mfma_planes(T[0], rp, u[0]);
+            u[1] = mfma_planes(T[1], rp, u[1]);
+            Oct<float> U, Ut;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                U.v[j] = u[j >> 2][j & 3];
+                if (any_bad && 8 * grp + j >= first) U.v[j] = 0.f;
+                Ut.v[j] = tail[j] * U.v[j];
+            }
+            u32x4 up[3], ut[3], u2[PO];
+            U.planes(up);
+            Ut.planes(ut);
+#pragma unroll
+            for (int p = 0; p < PO; ++p) u2[p] = up[p];
+            w[0] = mfma_planes(Pm[0], u2, w[0]);
+            w[1] = mfma_planes(Pm[1], u2, w[1]);
+            // S' = e^{G_C} S0 + K^T (e^{G_C - G} U)
+#pragma unroll
+            for (int n = 0; n < 2 * NK; ++n) {
+                u32x4 ft[P];
+#pragma unroll
+                for (int p = 0; p < P; ++p) ft[p] = operand(buf + (2 * P + p) * L::kPlane + n * kFrag, lane);
+                S[n] = mfma_planes(ft, ut, S[n] * whole);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int t = t0 + 8 * grp + j;
+                float ov = fmaf(a.scale * eg[j], qs[j >> 2][j & 3], w[j >> 2][j & 3]);
+                if (any_bad && 8 * grp + j >= first) ov = nan;
                 if (cok && t < len) store_f(o + (size_t)t * so, ov);
             }
-        // S' = e^{G_C} S0 + K^T (e^{G_C - G} U)
-        const float whole = ws[kWsEg + kC - 1];
-        float4 ut[2];
-        for (int I = 0; I < 2; ++I) {
-            float x[4];
-            for (int r = 0; r < 4; ++r) x[r] = ws[kWsTail + 16 * I + 4 * grp + r] * u[I][r];
-            ut[I] = {x[0], x[1], x[2], x[3]};
-        }
+            if (any_bad && first < kC)
 #pragma unroll
-        for (int n = 0; n < NK; ++n) {
-            S[n] *= whole;
-            const int d = 16 * n + col;
-            for (int I = 0; I < 2; ++I) {
-                float kt[4];
-                for (int r = 0; r < 4; ++r) {
-                    const int t = t0 + 16 * I + 4 * grp + r;
-                    kt[r] = d < a.dk && t < len ? load_f(k + (size_t)t * a.sk[1] + d) : 0.f;
-                }
-                S[n] = mfma4({kt[0], kt[1], kt[2], kt[3]}, ut[I], S[n]);
-            }
-            if (first < kC)
-                for (int r = 0; r < 4; ++r) S[n][r] = nan;
+                for (int n = 0; n < 2 * NK; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) S[n][r] = nan;
         }
+        if (!L::kTwo) __syncthreads();
+        if (more) rows.store(lds + (L::kTwo ? (c + 1 & 1) * L::kOne : 0));
+        __syncthreads();
     }
     if (cok)
         for (int t = len + grp; t < a.T; t += 4) store_f(o + (size_t)t * so, 0.f);
     if (a.s_out && cok)
 #pragma unroll
-        for (int n = 0; n < NK; ++n)
+        for (int n = 0; n < 2 * NK; ++n)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int d = 16 * n + 4 * grp + r;
+                const int d = 32 * (n >> 1) + row_index(n & 1, 4 * grp + r);
                 if (d < a.dk) a.s_out[sbase + (size_t)d * a.dv] = S[n][r];
             }
 }
 
 template <class E, int NK>
-static void scan_for(const DeltaArgs& a, hipStream_t s) {
-    const int ncol = (a.dv + 15) / 16;
-    hipLaunchKernelGGL((mp_delta_scan<E, NK>), dim3((unsigned)(a.B * a.Hv * ncol)), dim3(64), 0, s, a, ncol);
+static bool scan_for(const DeltaArgs& a, hipStream_t s) {
+    constexpr int bytes = ScanLds<E, NK>::kBytes;
+    static_assert(bytes <= 160 * 1024, "LDS of a CU");
+    // (per device: an attribute of the function on the current device; setting it again costs a microsecond)
+    if (bytes > 64 * 1024 && hipFuncSetAttribute((const void*)mp_delta_scan<E, NK>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return false;
+    const int ncol = (a.dv + 63) / 64, units = a.B * a.Hk;
+    hipLaunchKernelGGL((mp_delta_scan<E, NK>), dim3((unsigned)((units + 7) / 8 * 8 * (a.Hv / a.Hk) * ncol)), dim3(256), bytes, s, a, ncol);
+    return true;
 }
-template <class E>
+template <class E, int PO>
 static bool launch_for(const DeltaArgs& a, hipStream_t s) {
-    if (a.nchunk) hipLaunchKernelGGL(mp_delta_prep<E>, dim3((unsigned)(a.B * a.Hk * a.nchunk)), dim3(64), 0, s, a);
-    const int nk = (a.dk + 15) / 16;
-    if (nk <= 2) scan_for<E, 2>(a, s);
-    else if (nk <= 4) scan_for<E, 4>(a, s);
-    else if (nk <= 8) scan_for<E, 8>(a, s);
-    else scan_for<E, 16>(a, s);
-    return hipGetLastError() == hipSuccess;
+    if (a.nchunk) hipLaunchKernelGGL((mp_delta_prep<E, PO>), dim3((unsigned)(a.B * a.Hk * a.nchunk)), dim3(64), 0, s, a);
+    const int nk = (a.dk + 31) / 32;
+    const bool ok = nk == 1 ? scan_for<E, 1>(a, s) : nk == 2 ? scan_for<E, 2>(a, s) : nk == 3 ? scan_for<E, 3>(a, s) : nk == 4 ? scan_for<E, 4>(a, s)
+                  : nk <= 6 ? scan_for<E, 6>(a, s) : scan_for<E, 8>(a, s);
+    return hipGetLastError() == hipSuccess && ok;
 }
 bool launch_delta(const DeltaArgs& a, int dtype, hipStream_t s) {
-    return dtype == kBF16 ? launch_for<bf16raw>(a, s) : launch_for<float>(a, s);
+    return dtype == kBF16 ? launch_for<bf16raw, 2>(a, s) : launch_for<float, 3>(a, s);
 }
 
 // ---------------------------------------------------------------- one frame per stream
@@ -275,7 +431,7 @@ bool launch_delta(const DeltaArgs& a, int dtype, hipStream_t s) {
 // state is written once.  HBM-bound: 8 dk dv bytes per stream and head.
 template <class E, int VEC, int NR>
 MP_KERNEL __launch_bounds__(256) void mp_delta_online(DeltaOnlineArgs a, int ntile, int log_lanes) {
-    extern __shared__ float lds[];               // k [dk] | q [dk] | partial sums [4 waves][2][lanes * VEC]
+    extern __shared__ float tick_lds[];               // k [dk] | q [dk] | partial sums [4 waves][2][lanes * VEC]
     const int tid = threadIdx.x, lanes = 1 << log_lanes, cl = tid & (lanes - 1), rl = tid >> log_lanes, rows = 256 >> log_lanes;
     const int ct = blockIdx.x % ntile, hv = blockIdx.x / ntile % a.Hv, st = blockIdx.x / ntile / a.Hv;
     const int hk = hv / (a.Hv / a.Hk);
@@ -308,7 +464,7 @@ MP_KERNEL __launch_bounds__(256) void mp_delta_online(DeltaOnlineArgs a, int nti
         for (int i = tid; i < st; i += 256) twice |= a.slots[i] == slot;
         refuse |= __syncthreads_or(twice) != 0;
     }
-    float *lk = lds, *lq = lds + a.dk, *part = lds + 2 * a.dk;
+    float *lk = tick_lds, *lq = lk + a.dk, *part = lq + a.dk;
     const E* q = (const E*)a.q + st * a.sq[0] + hk * a.sq[1];
     const E* k = (const E*)a.k + st * a.sk[0] + hk * a.sk[1];
     for (int d = tid; d < a.dk; d += 256) { lk[d] = load_f(k + d); lq[d] = load_f(q + d); }

@@ -37,7 +37,7 @@ int mp_delta_rule(mp_handle* h, int dtype, const void* q_dev, const void* k_dev,
     if (need && (!ws_dev || ws_bytes < need || (uintptr_t)ws_dev % 16))
         return fail(h, MP_ERR_INVALID, "mp_delta_rule: workspace of %zu bytes, %zu needed (16-byte aligned)", ws_bytes, need);
     const int64_t nchunk = ((int64_t)T + 31) / 32;
-    if ((int64_t)B * Hk * nchunk > kMaxBlocks || (int64_t)B * Hv * (((int64_t)dv + 15) / 16) > kMaxBlocks)
+    if ((int64_t)B * Hk * nchunk > kMaxBlocks || ((int64_t)B * Hk + 7) * (Hv / Hk) * (((int64_t)dv + 63) / 64) > kMaxBlocks)
         return fail(h, MP_ERR_INVALID, "mp_delta_rule: batch of %d x %d frames, %d heads is too large for one call", B, T, Hv);
     ON_DEVICE(h);
     mpseq::DeltaArgs a;
