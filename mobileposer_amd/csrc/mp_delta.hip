@@ -21,11 +21,12 @@ namespace mpseq {
 
 constexpr int kC = 32;                            // frames per chunk
 // Workspace of one (sequence, value head, chunk), bytes: T = (I + A)^{-1} as three terms and P = scale tril(Q K^T) o D as two (bf16
-// outputs) or three, in the order in which a lane of v_mfma_f32_16x16x32_bf16 takes its A operand, then beta, e^G, e^{G_C - G}.
+// outputs) or three, in the order in which a lane of v_mfma_f32_16x16x32_bf16 takes its A operand, behind beta, e^G, e^{G_C - G}.
 constexpr int kFrag = 1024;                       // one 16 x 32 operand: 64 lanes x 8 bf16
-constexpr int kWsP = 6 * kFrag, kWsBeta = 12 * kFrag, kWsEg = kWsBeta + 4 * kC, kWsTail = kWsEg + 4 * kC, kWsUnit = kWsTail + 4 * kC;
+constexpr int kWsBeta = 0, kWsEg = 4 * kC, kWsTail = 8 * kC, kWsT = 512, kWsP = kWsT + 6 * kFrag;
+constexpr int ws_unit(int po) { return kWsP + 2 * po * kFrag; }
 
-size_t delta_ws_floats(int B, int T, int Hv) { return (size_t)B * Hv * ((T + kC - 1) / kC) * (kWsUnit / 4); }
+size_t delta_ws_floats(int B, int T, int Hv) { return (size_t)B * Hv * ((T + kC - 1) / kC) * (ws_unit(3) / 4); }
 
 // Which frame and which component of k a lane's registers stand for.  The accumulator layout of a 16 x 16 tile (lane: column
 // lane % 16, rows 4 (lane / 16) + r) becomes the B operand of a K = 32 instruction (lane: column lane % 16, k slots
@@ -42,15 +43,26 @@ static __device__ __forceinline__ int length_of(const int* lengths, int b, int T
 static __device__ __forceinline__ float clamp_g(float g) { return g < -1e4f ? -1e4f : g; }      // (NaN stays NaN)
 static __device__ __forceinline__ bool not_finite(float x) { return !(fabsf(x) <= 3.402823466e38f); }
 
-template <class E>
-static __device__ __forceinline__ void load_row(Oct<E>& o, const E* p, int d, int dk, bool on) {      // components d .. d + 7 of a row
-    if (on && d < dk) o.load_some(p + d, dk - d); else o.zero();
+// Components d .. d + 7 of a row of q or k, without a branch around the load (a branch would make the loads wait for each other):
+// the address is moved inside the row, fix() puts zeros where the row or the sequence has ended.  MODE 0: dk is a multiple of 8;
+// 1: it is not, but at least 8 -- the last eight components are loaded and shifted down; 2: dk < 8, component by component.
+template <class E, int MODE>
+static __device__ __forceinline__ void load_oct(Oct<E>& o, const E* row, int d, int dk) {
+    if (MODE == 0) o.load(row + (d < dk ? d : 0));
+    else if (MODE == 1) o.load(row + min(d, dk - 8));
+    else o.load_clamped(row, d, dk);
+}
+template <class E, int MODE>
+static __device__ __forceinline__ void fix_oct(Oct<E>& o, int d, int dk, bool on) {
+    if (MODE == 1) o.shift(d - min(d, dk - 8));
+    if (MODE == 2) o.keep(dk - d);
+    if (!on || d >= dk) o.zero();
 }
 
 // One wave per (sequence, key head, chunk): K K^T and Q K^T once, then the value heads that share the key head, two at a time --
 // a lane of either half solves a column of (I + A) T = I by forward substitution (stable where keys repeat and A is far from
 // small; products of powers of A are not).
-template <class E, int PO>
+template <class E, int PO, int MODE>
 MP_KERNEL __launch_bounds__(64) void mp_delta_prep(DeltaArgs a) {
     constexpr int P = Arith<E>::P, LS = kC + 4;
     __shared__ __align__(16) float A[2][kC][LS], W[kC][LS];
@@ -61,17 +73,22 @@ MP_KERNEL __launch_bounds__(64) void mp_delta_prep(DeltaArgs a) {
     const E* q = (const E*)a.q + b * a.sq[0] + hk * a.sq[2];
     const E* k = (const E*)a.k + b * a.sk[0] + hk * a.sk[2];
     f32x4 kk[3] = {}, qk[3] = {};                 // tiles (0,0), (1,0), (1,1) of frames 16 I + row, 16 J + column
+    const int tl[2] = {min(t0 + col, len - 1), min(t0 + 16 + col, len - 1)};
     for (int d0 = 0; d0 < a.dk; d0 += 32) {
         u32x4 fk[2][P], fq[2][P];
+        Oct<E> ok[2], oq[2];
+        const int d = d0 + 8 * grp;
 #pragma unroll
         for (int I = 0; I < 2; ++I) {
-            const int t = t0 + 16 * I + col;
-            const bool on = t < len;
-            Oct<E> ok, oq;
-            load_row(ok, k + (on ? t : 0) * a.sk[1], d0 + 8 * grp, a.dk, on);
-            load_row(oq, q + (on ? t : 0) * a.sq[1], d0 + 8 * grp, a.dk, on);
-            ok.planes(fk[I]);
-            oq.planes(fq[I]);
+            load_oct<E, MODE>(ok[I], k + tl[I] * a.sk[1], d, a.dk);
+            load_oct<E, MODE>(oq[I], q + tl[I] * a.sq[1], d, a.dk);
+        }
+#pragma unroll
+        for (int I = 0; I < 2; ++I) {
+            fix_oct<E, MODE>(ok[I], d, a.dk, t0 + 16 * I + col < len);
+            fix_oct<E, MODE>(oq[I], d, a.dk, t0 + 16 * I + col < len);
+            ok[I].planes(fk[I]);
+            oq[I].planes(fq[I]);
         }
 #pragma unroll
         for (int n = 0; n < 3; ++n) {
@@ -92,13 +109,13 @@ MP_KERNEL __launch_bounds__(64) void mp_delta_prep(DeltaArgs a) {
         }
         const double last = __shfl(G, kC - 1, 32);
         if (half < two) {
-            char* ws = (char*)a.ws + ((size_t)(b * a.Hv + hh) * a.nchunk + c) * kWsUnit;
+            char* ws = (char*)a.ws + ((size_t)(b * a.Hv + hh) * a.nchunk + c) * ws_unit(PO);
             ((float*)(ws + kWsBeta))[i] = beta;
             ((float*)(ws + kWsEg))[i] = expf((float)G);
             ((float*)(ws + kWsTail))[i] = expf((float)(last - G));
         }
         for (int e = 0; e < two; ++e) {
-            char* ws = (char*)a.ws + ((size_t)(b * a.Hv + hk * rep + e0 + e) * a.nchunk + c) * kWsUnit;
+            char* ws = (char*)a.ws + ((size_t)(b * a.Hv + hk * rep + e0 + e) * a.nchunk + c) * ws_unit(PO);
             __syncthreads();
 #pragma unroll
             for (int tile = 0; tile < 3; ++tile) {
@@ -148,7 +165,7 @@ MP_KERNEL __launch_bounds__(64) void mp_delta_prep(DeltaArgs a) {
         for (int n = 0; n < kC; ++n) A[half][n][i] = x[n];        // (with one head left, the other half's copy is not read)
         __syncthreads();
         for (int e = 0; e < two; ++e) {
-            char* ws = (char*)a.ws + ((size_t)(b * a.Hv + hk * rep + e0 + e) * a.nchunk + c) * kWsUnit;
+            char* ws = (char*)a.ws + ((size_t)(b * a.Hv + hk * rep + e0 + e) * a.nchunk + c) * ws_unit(PO);
 #pragma unroll
             for (int I = 0; I < 2; ++I) {
                 Oct<float> o;
@@ -156,7 +173,7 @@ MP_KERNEL __launch_bounds__(64) void mp_delta_prep(DeltaArgs a) {
                 o.load(&A[e][row_index(I, col)][8 * grp]);
                 o.planes(p);
 #pragma unroll
-                for (int n = 0; n < 3; ++n) *(u32x4*)(ws + (I * 3 + n) * kFrag + lane * 16) = p[n];
+                for (int n = 0; n < 3; ++n) *(u32x4*)(ws + kWsT + (I * 3 + n) * kFrag + lane * 16) = p[n];
             }
         }
     }
@@ -164,49 +181,57 @@ MP_KERNEL __launch_bounds__(64) void mp_delta_prep(DeltaArgs a) {
 
 // The walk over the chunks: a workgroup per (sequence, value head, 64 columns of the state), a wave per 16 columns; NK = dk / 32
 // rounded up.  The workgroup stages K, Q and K^T of a chunk in LDS as ready operands (bf16 terms, one 16-byte read per lane and
-// operand), the next chunk's rows are on their way through registers meanwhile.
+// operand) beside the chunk's workspace; the next chunk's rows are on their way through registers meanwhile, with no use of them --
+// not even a conversion -- before this chunk's products are done.
 template <class E, int NK>
 struct ScanLds {
-    static constexpr int P = Arith<E>::P, kPlane = 2 * NK * kFrag, kOne = 3 * P * kPlane;      // K | Q | K^T, P planes each
-    static constexpr bool kTwo = 2 * kOne <= 160 * 1024;
-    static constexpr int kBytes = kTwo ? 2 * kOne : kOne;
+    static constexpr int P = Arith<E>::P, PO = P == 1 ? 2 : 3, kPlane = 2 * NK * kFrag, kWs = 3 * P * kPlane;      // K | Q | K^T | workspace
+    static constexpr int kBytes = kWs + ws_unit(PO);
 };
-template <class E, int NK>
+template <class E, int NK, int MODE>
 struct Rows {                                     // what a thread stages of a chunk
-    static constexpr int P = Arith<E>::P, NO = (4 * NK + 7) / 8, NP = (16 * NK + 63) / 64;
+    static constexpr int P = Arith<E>::P, NO = (4 * NK + 7) / 8, NP = (16 * NK + 63) / 64, kUnit = ws_unit(ScanLds<E, NK>::PO), NW = (kUnit + 4095) / 4096;
     Oct<E> k[NO], q[NO];
-    E kt[NP][2][8];
-    __device__ __forceinline__ void load(const DeltaArgs& a, const E* kp, const E* qp, int t0, int len) {
-        const int tid = threadIdx.x, t = t0 + (tid & 31);
-        const bool on = t < len;
+    E kt[NP][8][2];                               // components d, d + 1 of eight frames
+    E v[8];                                       // the lane's column of eight frames
+    u32x4 ws[NW];
+    __device__ __forceinline__ void load(const DeltaArgs& a, const E* kp, const E* qp, const E* vp, const char* wp, int t0, int len) {
+        const int tid = threadIdx.x, t = min(t0 + (tid & 31), len - 1);
+#pragma unroll
+        for (int n = 0; n < NW; ++n) ws[n] = *(const u32x4*)(wp + min(4096 * n + 16 * tid, kUnit - 16));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = vp[min(t0 + 8 * (tid >> 4 & 3) + j, len - 1) * a.sv[1]];
 #pragma unroll
         for (int n = 0; n < NO; ++n) {
             const int d = 8 * ((tid >> 5) + 8 * n);
-            load_row(k[n], kp + (on ? t : 0) * a.sk[1], d, a.dk, on);
-            load_row(q[n], qp + (on ? t : 0) * a.sq[1], d, a.dk, on);
+            load_oct<E, MODE>(k[n], kp + t * a.sk[1], d, a.dk);
+            load_oct<E, MODE>(q[n], qp + t * a.sq[1], d, a.dk);
         }
 #pragma unroll
         for (int n = 0; n < NP; ++n) {
-            const int d = 2 * ((tid >> 2) + 64 * n), tt = t0 + 8 * (tid & 3);
+            const int d = 2 * ((tid >> 2) + 64 * n);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const E* p = kp + (tt + j < len ? tt + j : 0) * a.sk[1] + d;
-                E two[2] = {0, 0};
-                if (tt + j < len && d + 1 < a.dk) __builtin_memcpy(two, p, sizeof(two));
-                else if (tt + j < len && d < a.dk) two[0] = *p;
-                kt[n][0][j] = two[0];
-                kt[n][1][j] = two[1];
+                const E* row = kp + min(t0 + 8 * (tid & 3) + j, len - 1) * a.sk[1];
+                if (MODE == 0) __builtin_memcpy(kt[n][j], row + (d < a.dk ? d : 0), 2 * sizeof(E));
+                else if (MODE == 1) __builtin_memcpy(kt[n][j], row + min(d, a.dk - 2), 2 * sizeof(E));
+                else { kt[n][j][0] = row[min(d, a.dk - 1)]; kt[n][j][1] = row[min(d + 1, a.dk - 1)]; }
             }
         }
     }
-    __device__ __forceinline__ void store(char* lds) const {
+    __device__ __forceinline__ void store(const DeltaArgs& a, char* lds, int t0, int len) {
         using L = ScanLds<E, NK>;
         const int tid = threadIdx.x, t = tid & 31, row = 4 * (t >> 3) + (t & 3), I = t >> 2 & 1;
+#pragma unroll
+        for (int n = 0; n < NW; ++n)
+            if (4096 * n + 16 * tid < kUnit) *(u32x4*)(lds + L::kWs + 4096 * n + 16 * tid) = ws[n];
 #pragma unroll
         for (int n = 0; n < NO; ++n) {
             const int o = (tid >> 5) + 8 * n;
             if (o < 4 * NK) {
                 u32x4 pk[P], pq[P];
+                fix_oct<E, MODE>(k[n], 8 * o, a.dk, t0 + t < len);
+                fix_oct<E, MODE>(q[n], 8 * o, a.dk, t0 + t < len);
                 k[n].planes(pk);
                 q[n].planes(pq);
                 char* at = lds + (2 * (o >> 2) + I) * kFrag + (row + 16 * (o & 3)) * 16;
@@ -224,9 +249,13 @@ struct Rows {                                     // what a thread stages of a c
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                     const int dd = d + x, tile = 2 * (dd >> 5) + (dd >> 2 & 1), rw = 4 * (dd >> 3 & 3) + (dd & 3);
+                    const bool last = MODE == 1 && d == a.dk - 1;               // (the pair was loaded one component early)
+                    E col[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) col[j] = dd < a.dk && t0 + 8 * (tid & 3) + j < len ? (last ? kt[n][j][1] : kt[n][j][x]) : (E)0;
                     Oct<E> o;
                     u32x4 pt[P];
-                    __builtin_memcpy(&o.v, kt[n][x], sizeof(o.v));
+                    __builtin_memcpy(&o.v, col, sizeof(o.v));
                     o.planes(pt);
 #pragma unroll
                     for (int p = 0; p < P; ++p) *(u32x4*)(lds + (2 * P + p) * L::kPlane + tile * kFrag + (rw + 16 * (tid & 3)) * 16) = pt[p];
@@ -236,159 +265,165 @@ struct Rows {                                     // what a thread stages of a c
 };
 static __device__ __forceinline__ u32x4 operand(const char* p, int lane) { return *(const u32x4*)(p + lane * 16); }
 
-template <class E, int NK>
+template <class E, int NK, int MODE>
 MP_KERNEL __launch_bounds__(256) void mp_delta_scan(DeltaArgs a, int ncol) {
     using L = ScanLds<E, NK>;
-    constexpr int P = Arith<E>::P, PO = P == 1 ? 2 : 3;
+    constexpr int P = L::P, PO = L::PO;
     extern __shared__ __align__(16) char scan_lds[];
     char* const lds = scan_lds;
+    const char* const ws = lds + L::kWs;
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, grp = lane >> 4;
     // the workgroups that read the same K and Q on one XCD (workgroups are dealt to the 8 of them in turn)
     const int rep = a.Hv / a.Hk, inner = rep * ncol, rest = blockIdx.x >> 3, unit = rest / inner * 8 + (blockIdx.x & 7);
     if (unit >= a.B * a.Hk) return;
     const int hk = unit % a.Hk, b = unit / a.Hk, hv = hk * rep + rest % inner / ncol;
     const int cv = 64 * (rest % ncol) + 16 * (tid >> 6) + col;
-    const bool cok = cv < a.dv, live = 64 * (rest % ncol) + 16 * (tid >> 6) < a.dv;      // (live: the wave has a column)
+    const bool cok = cv < a.dv;
+    const int cc = cok ? cv : a.dv - 1;
     const int len = length_of(a.lengths, b, a.T);
     const E* q = (const E*)a.q + b * a.sq[0] + hk * a.sq[2];
     const E* k = (const E*)a.k + b * a.sk[0] + hk * a.sk[2];
-    const E* v = (const E*)a.v + b * a.sv[0] + hv * a.sv[2] + (cok ? cv : 0);
-    E* o = (E*)a.o + ((size_t)b * a.T * a.Hv + hv) * a.dv + cv;
+    const E* v = (const E*)a.v + b * a.sv[0] + hv * a.sv[2] + cc;
+    const char* wsg = (const char*)a.ws + (size_t)(b * a.Hv + hv) * a.nchunk * ws_unit(PO);
+    E* o = (E*)a.o + ((size_t)b * a.T * a.Hv + hv) * a.dv + cc;
     const size_t so = (size_t)a.Hv * a.dv;
-    const size_t sbase = (size_t)(b * a.Hv + hv) * a.dk * a.dv + cv;
+    const size_t sbase = (size_t)(b * a.Hv + hv) * a.dk * a.dv + cc;
     f32x4 S[2 * NK];
 #pragma unroll
-    for (int n = 0; n < 2 * NK; ++n)
+    for (int n = 0; n < 2 * NK; ++n) S[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    if (a.s_in)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int d = 32 * (n >> 1) + row_index(n & 1, 4 * grp + r);
-            S[n][r] = a.s_in && cok && d < a.dk ? a.s_in[sbase + (size_t)d * a.dv] : 0.f;
-        }
-    auto load_v = [&](float (&vv)[8], int t0) {
+        for (int n = 0; n < 2 * NK; ++n)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int t = t0 + 8 * grp + j;
-            vv[j] = cok && t < len ? load_f(v + (size_t)t * a.sv[1]) : 0.f;
-        }
-    };
+            for (int r = 0; r < 4; ++r) {
+                const int d = 32 * (n >> 1) + row_index(n & 1, 4 * grp + r);
+                const float x = a.s_in[sbase + (size_t)min(d, a.dk - 1) * a.dv];
+                S[n][r] = d < a.dk ? x : 0.f;
+            }
     const float nan = __builtin_nanf("");
-    Rows<E, NK> rows;
-    float vnext[8];
-    if (len > 0) {
-        rows.load(a, k, q, 0, len);
-        load_v(vnext, 0);
-        rows.store(lds);
+    const int nc = (len + kC - 1) / kC;
+    Rows<E, NK, MODE> rows;
+    if (nc > 0) {
+        rows.load(a, k, q, v, wsg, 0, len);
+        rows.store(a, lds, 0, len);
     }
     __syncthreads();
-    for (int c = 0; c * kC < len; ++c) {
-        const char* ws = (const char*)a.ws + ((size_t)(b * a.Hv + hv) * a.nchunk + c) * kWsUnit;
+    for (int c = 0; c < nc; ++c) {
         const int t0 = c * kC;
-        const bool more = t0 + kC < len;
-        float vv[8];
+        E vv[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) vv[j] = vnext[j];
-        if (more) {
-            rows.load(a, k, q, t0 + kC, len);
-            load_v(vnext, t0 + kC);
-        }
-        const char* buf = lds + (L::kTwo ? (c & 1) * L::kOne : 0);
-        if (live) {
-            u32x4 T[2][3], Pm[2][PO];
-            float beta[8], eg[8], tail[8];
+        for (int j = 0; j < 8; ++j) vv[j] = rows.v[j];
+        const int cn = min(c + 1, nc - 1);
+        rows.load(a, k, q, v, wsg + (size_t)cn * ws_unit(PO), cn * kC, len);
+        __builtin_amdgcn_sched_barrier(0);                         // (the loads are issued here, not where their values are used)
+        f32x4 ks[2] = {}, qs[2] = {};
+#pragma unroll
+        for (int m = 0; m < NK; ++m) {
+            Oct<float> os;
+            u32x4 sp[3], s2[PO];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) os.v[j] = S[2 * m + (j >> 2)][j & 3];
+            os.planes(sp);
+#pragma unroll
+            for (int p = 0; p < PO; ++p) s2[p] = sp[p];
 #pragma unroll
             for (int I = 0; I < 2; ++I) {
+                u32x4 fk[P], fq[P];
 #pragma unroll
-                for (int p = 0; p < 3; ++p) T[I][p] = operand(ws + (I * 3 + p) * kFrag, lane);
-#pragma unroll
-                for (int p = 0; p < PO; ++p) Pm[I][p] = operand(ws + kWsP + (I * PO + p) * kFrag, lane);
-            }
-            __builtin_memcpy(beta, __builtin_assume_aligned(ws + kWsBeta + 32 * grp, 16), 32);
-            __builtin_memcpy(eg, __builtin_assume_aligned(ws + kWsEg + 32 * grp, 16), 32);
-            __builtin_memcpy(tail, __builtin_assume_aligned(ws + kWsTail + 32 * grp, 16), 32);
-            const float whole = *(const float*)(ws + kWsEg + 4 * (kC - 1));
-            f32x4 ks[2] = {}, qs[2] = {};
-#pragma unroll
-            for (int m = 0; m < NK; ++m) {
-                Oct<float> os;
-                u32x4 sp[3], s2[PO];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) os.v[j] = S[2 * m + (j >> 2)][j & 3];
-                os.planes(sp);
-#pragma unroll
-                for (int p = 0; p < PO; ++p) s2[p] = sp[p];
-#pragma unroll
-                for (int I = 0; I < 2; ++I) {
-                    u32x4 fk[P], fq[P];
-#pragma unroll
-                    for (int p = 0; p < P; ++p) {
-                        fk[p] = operand(buf + p * L::kPlane + (2 * m + I) * kFrag, lane);
-                        fq[p] = operand(buf + (P + p) * L::kPlane + (2 * m + I) * kFrag, lane);
-                    }
-                    ks[I] = mfma_planes(fk, sp, ks[I]);
-                    qs[I] = mfma_planes(fq, s2, qs[I]);
+                for (int p = 0; p < P; ++p) {
+                    fk[p] = operand(lds + p * L::kPlane + (2 * m + I) * kFrag, lane);
+                    fq[p] = operand(lds + (P + p) * L::kPlane + (2 * m + I) * kFrag, lane);
                 }
+                ks[I] = mfma_planes(fk, sp, ks[I]);
+                qs[I] = mfma_planes(fq, s2, qs[I]);
             }
-            Oct<float> R;
-            bool bad = false;
+        }
+        float beta[8], eg[8], tail[8];
+        __builtin_memcpy(beta, __builtin_assume_aligned(ws + kWsBeta + 32 * grp, 16), 32);
+        __builtin_memcpy(eg, __builtin_assume_aligned(ws + kWsEg + 32 * grp, 16), 32);
+        __builtin_memcpy(tail, __builtin_assume_aligned(ws + kWsTail + 32 * grp, 16), 32);
+        const float whole = *(const float*)(ws + kWsEg + 4 * (kC - 1));
+        Oct<float> R;
+        bool bad = false;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                R.v[j] = beta[j] * fmaf(-eg[j], ks[j >> 2][j & 3], vv[j]);
-                bad |= not_finite(R.v[j]);
-            }
-            int first = kC;                                        // this column's first row that is not finite
-            const bool any_bad = __any(bad);
-            if (any_bad) {
+        for (int j = 0; j < 8; ++j) {
+            const float vj = cok && t0 + 8 * grp + j < len ? load_f(&vv[j]) : 0.f;
+            R.v[j] = beta[j] * fmaf(-eg[j], ks[j >> 2][j & 3], vj);
+            bad |= not_finite(R.v[j]);
+        }
+        int first = kC;                                            // this column's first row that is not finite
+        const bool any_bad = __any(bad);
+        if (any_bad) {
 #pragma unroll
-                for (int j = 7; j >= 0; --j)
-                    if (not_finite(R.v[j])) first = 8 * grp + j;
-                first = min(first, __shfl_xor(first, 16));
-                first = min(first, __shfl_xor(first, 32));
+            for (int j = 7; j >= 0; --j)
+                if (not_finite(R.v[j])) first = 8 * grp + j;
+            first = min(first, __shfl_xor(first, 16));
+            first = min(first, __shfl_xor(first, 32));
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (8 * grp + j >= first) R.v[j] = 0.f;
+        }
+        u32x4 rp[3];
+        R.planes(rp);
+        f32x4 u[2] = {}, w[2] = {};
+#pragma unroll
+        for (int I = 0; I < 2; ++I) {
+            u32x4 T[3];
+#pragma unroll
+            for (int p = 0; p < 3; ++p) T[p] = operand(ws + kWsT + (I * 3 + p) * kFrag, lane);
+            u[I] = mfma_planes(T, rp, u[I]);
+        }
+        Oct<float> U, Ut;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            U.v[j] = u[j >> 2][j & 3];
+            if (any_bad && 8 * grp + j >= first) U.v[j] = 0.f;
+            Ut.v[j] = tail[j] * U.v[j];
+        }
+        u32x4 up[3], ut[3], u2[PO];
+        U.planes(up);
+        Ut.planes(ut);
+#pragma unroll
+        for (int p = 0; p < PO; ++p) u2[p] = up[p];
+#pragma unroll
+        for (int I = 0; I < 2; ++I) {
+            u32x4 Pm[PO];
+#pragma unroll
+            for (int p = 0; p < PO; ++p) Pm[p] = operand(ws + kWsP + (I * PO + p) * kFrag, lane);
+            w[I] = mfma_planes(Pm, u2, w[I]);
+        }
+        // S' = e^{G_C} S0 + K^T (e^{G_C - G} U)
+#pragma unroll
+        for (int n = 0; n < 2 * NK; ++n) {
+            u32x4 ft[P];
+#pragma unroll
+            for (int p = 0; p < P; ++p) ft[p] = operand(lds + (2 * P + p) * L::kPlane + n * kFrag, lane);
+            S[n] = mfma_planes(ft, ut, S[n] * whole);
+        }
+        float ov[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            ov[j] = fmaf(a.scale * eg[j], qs[j >> 2][j & 3], w[j >> 2][j & 3]);
+            if (any_bad && 8 * grp + j >= first) ov[j] = nan;
+        }
+        E* out = o + (size_t)(t0 + 8 * grp) * so;
+        if (cok) {
+            if (t0 + kC <= len) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) store_f(out + j * so, ov[j]);
+            } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    if (8 * grp + j >= first) R.v[j] = 0.f;
+                    if (t0 + 8 * grp + j < len) store_f(out + j * so, ov[j]);
             }
-            u32x4 rp[3];
-            R.planes(rp);
-            f32x4 u[2] = {}, w[2] = {};
-            u[0] = mfma_planes(T[0], rp, u[0]);
-            u[1] = mfma_planes(T[1], rp, u[1]);
-            Oct<float> U, Ut;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                U.v[j] = u[j >> 2][j & 3];
-                if (any_bad && 8 * grp + j >= first) U.v[j] = 0.f;
-                Ut.v[j] = tail[j] * U.v[j];
-            }
-            u32x4 up[3], ut[3], u2[PO];
-            U.planes(up);
-            Ut.planes(ut);
-#pragma unroll
-            for (int p = 0; p < PO; ++p) u2[p] = up[p];
-            w[0] = mfma_planes(Pm[0], u2, w[0]);
-            w[1] = mfma_planes(Pm[1], u2, w[1]);
-            // S' = e^{G_C} S0 + K^T (e^{G_C - G} U)
-#pragma unroll
-            for (int n = 0; n < 2 * NK; ++n) {
-                u32x4 ft[P];
-#pragma unroll
-                for (int p = 0; p < P; ++p) ft[p] = operand(buf + (2 * P + p) * L::kPlane + n * kFrag, lane);
-                S[n] = mfma_planes(ft, ut, S[n] * whole);
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int t = t0 + 8 * grp + j;
-                float ov = fmaf(a.scale * eg[j], qs[j >> 2][j & 3], w[j >> 2][j & 3]);
-                if (any_bad && 8 * grp + j >= first) ov = nan;
-                if (cok && t < len) store_f(o + (size_t)t * so, ov);
-            }
-            if (any_bad && first < kC)
-#pragma unroll
-                for (int n = 0; n < 2 * NK; ++n)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) S[n][r] = nan;
         }
-        if (!L::kTwo) __syncthreads();
-        if (more) rows.store(lds + (L::kTwo ? (c + 1 & 1) * L::kOne : 0));
+        if (any_bad && first < kC)
+#pragma unroll
+            for (int n = 0; n < 2 * NK; ++n)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) S[n][r] = nan;
+        __syncthreads();
+        if (c + 1 < nc) rows.store(a, lds, t0 + kC, len);
         __syncthreads();
     }
     if (cok)
@@ -403,22 +438,28 @@ MP_KERNEL __launch_bounds__(256) void mp_delta_scan(DeltaArgs a, int ncol) {
             }
 }
 
-template <class E, int NK>
+template <class E, int NK, int MODE>
 static bool scan_for(const DeltaArgs& a, hipStream_t s) {
     constexpr int bytes = ScanLds<E, NK>::kBytes;
     static_assert(bytes <= 160 * 1024, "LDS of a CU");
-    // (per device: an attribute of the function on the current device; setting it again costs a microsecond)
-    if (bytes > 64 * 1024 && hipFuncSetAttribute((const void*)mp_delta_scan<E, NK>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return false;
+    // (an attribute of the function on the current device: set at every launch, a call may come from any device's handle)
+    if (bytes > 64 * 1024 && hipFuncSetAttribute((const void*)mp_delta_scan<E, NK, MODE>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return false;
     const int ncol = (a.dv + 63) / 64, units = a.B * a.Hk;
-    hipLaunchKernelGGL((mp_delta_scan<E, NK>), dim3((unsigned)((units + 7) / 8 * 8 * (a.Hv / a.Hk) * ncol)), dim3(256), bytes, s, a, ncol);
+    hipLaunchKernelGGL((mp_delta_scan<E, NK, MODE>), dim3((unsigned)((units + 7) / 8 * 8 * (a.Hv / a.Hk) * ncol)), dim3(256), bytes, s, a, ncol);
     return true;
+}
+template <class E, int PO, int MODE>
+static bool launch_mode(const DeltaArgs& a, hipStream_t s) {
+    if (a.nchunk) hipLaunchKernelGGL((mp_delta_prep<E, PO, MODE>), dim3((unsigned)(a.B * a.Hk * a.nchunk)), dim3(64), 0, s, a);
+    if (MODE == 2) return scan_for<E, 1, MODE>(a, s);
+    constexpr int M = MODE == 2 ? 1 : MODE;
+    const int nk = (a.dk + 31) / 32;
+    return nk == 1 ? scan_for<E, 1, M>(a, s) : nk == 2 ? scan_for<E, 2, M>(a, s) : nk == 3 ? scan_for<E, 3, M>(a, s) : nk == 4 ? scan_for<E, 4, M>(a, s)
+         : nk <= 6 ? scan_for<E, 6, M>(a, s) : scan_for<E, 8, M>(a, s);
 }
 template <class E, int PO>
 static bool launch_for(const DeltaArgs& a, hipStream_t s) {
-    if (a.nchunk) hipLaunchKernelGGL((mp_delta_prep<E, PO>), dim3((unsigned)(a.B * a.Hk * a.nchunk)), dim3(64), 0, s, a);
-    const int nk = (a.dk + 31) / 32;
-    const bool ok = nk == 1 ? scan_for<E, 1>(a, s) : nk == 2 ? scan_for<E, 2>(a, s) : nk == 3 ? scan_for<E, 3>(a, s) : nk == 4 ? scan_for<E, 4>(a, s)
-                  : nk <= 6 ? scan_for<E, 6>(a, s) : scan_for<E, 8>(a, s);
+    const bool ok = a.dk % 8 == 0 ? launch_mode<E, PO, 0>(a, s) : a.dk >= 8 ? launch_mode<E, PO, 1>(a, s) : launch_mode<E, PO, 2>(a, s);
     return hipGetLastError() == hipSuccess && ok;
 }
 bool launch_delta(const DeltaArgs& a, int dtype, hipStream_t s) {

@@ -27,6 +27,19 @@ template <> struct Oct<bf16raw> {
         for (int i = 0; i < 8; ++i) t[i] = i < n ? p[i] : (bf16raw)0;
         __builtin_memcpy(&v, t, 16);
     }
+    __device__ __forceinline__ void load_clamped(const bf16raw* row, int d, int n) {
+        bf16raw t[8];
+        for (int i = 0; i < 8; ++i) t[i] = row[min(d + i, n - 1)];
+        __builtin_memcpy(&v, t, 16);
+    }
+    __device__ __forceinline__ void shift(int s) {                // element i <- element i + s, zeros behind the last (s < 8)
+        if (s & 4) { v[0] = v[2]; v[1] = v[3]; v[2] = v[3] = 0; }
+        if (s & 2) { v[0] = v[1]; v[1] = v[2]; v[2] = v[3]; v[3] = 0; }
+        if (s & 1) { v[0] = v[0] >> 16 | v[1] << 16; v[1] = v[1] >> 16 | v[2] << 16; v[2] = v[2] >> 16 | v[3] << 16; v[3] >>= 16; }
+    }
+    __device__ __forceinline__ void keep(int n) {                 // zeros from element n on
+        for (int i = 0; i < 4; ++i) v[i] = 2 * i >= n ? 0 : 2 * i + 1 >= n ? v[i] & 0xffffu : v[i];
+    }
     __device__ __forceinline__ void load_some(const bf16raw* p, int n) {
         if (n >= 8) load(p); else load_guarded(p, n);
     }
@@ -50,6 +63,16 @@ template <> struct Oct<float> {
     __device__ __forceinline__ void load_guarded(const float* p, int n) {
         for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : 0.f;
     }
+    __device__ __forceinline__ void load_clamped(const float* row, int d, int n) {
+        for (int i = 0; i < 8; ++i) v[i] = row[min(d + i, n - 1)];
+    }
+    __device__ __forceinline__ void shift(int s) {
+#pragma unroll
+        for (int m = 4; m > 0; m >>= 1)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = s & m ? (i + m < 8 ? v[i + m < 8 ? i + m : 0] : 0.f) : v[i];
+    }
+    __device__ __forceinline__ void keep(int n) { for (int i = 0; i < 8; ++i) v[i] = i < n ? v[i] : 0.f; }
     __device__ __forceinline__ void load_some(const float* p, int n) {
         if (n >= 8) load(p); else load_guarded(p, n);
     }
