@@ -21,9 +21,10 @@ namespace mpseq {
 
 constexpr int kC = 32;                            // frames per chunk
 // Workspace of one (sequence, value head, chunk), bytes: T = (I + A)^{-1} as three terms and P = scale tril(Q K^T) o D as two (bf16
-// outputs) or three, in the order in which a lane of v_mfma_f32_16x16x32_bf16 takes its A operand, behind beta, e^G, e^{G_C - G}.
+// outputs) or three, in the order in which a lane of v_mfma_f32_16x16x32_bf16 takes its A operand, behind beta, beta e^G, scale e^G,
+// e^{G_C - G} of the 32 frames and e^{G_C}.
 constexpr int kFrag = 1024;                       // one 16 x 32 operand: 64 lanes x 8 bf16
-constexpr int kWsBeta = 0, kWsEg = 4 * kC, kWsTail = 8 * kC, kWsT = 512, kWsP = kWsT + 6 * kFrag;
+constexpr int kWsBeta = 0, kWsBetaEg = 4 * kC, kWsScaleEg = 8 * kC, kWsTail = 12 * kC, kWsWhole = 16 * kC, kWsT = kWsWhole + 16, kWsP = kWsT + 6 * kFrag;
 constexpr int ws_unit(int po) { return kWsP + 2 * po * kFrag; }
 
 size_t delta_ws_floats(int B, int T, int Hv) { return (size_t)B * Hv * ((T + kC - 1) / kC) * (ws_unit(3) / 4); }
@@ -111,8 +112,11 @@ MP_KERNEL __launch_bounds__(64) void mp_delta_prep(DeltaArgs a) {
         if (half < two) {
             char* ws = (char*)a.ws + ((size_t)(b * a.Hv + hh) * a.nchunk + c) * ws_unit(PO);
             ((float*)(ws + kWsBeta))[i] = beta;
-            ((float*)(ws + kWsEg))[i] = expf((float)G);
+            const float eg = expf((float)G);
+            ((float*)(ws + kWsBetaEg))[i] = beta * eg;
+            ((float*)(ws + kWsScaleEg))[i] = a.scale * eg;
             ((float*)(ws + kWsTail))[i] = expf((float)(last - G));
+            if (i == kC - 1) *(float*)(ws + kWsWhole) = eg;
         }
         for (int e = 0; e < two; ++e) {
             char* ws = (char*)a.ws + ((size_t)(b * a.Hv + hk * rep + e0 + e) * a.nchunk + c) * ws_unit(PO);
@@ -195,33 +199,58 @@ struct Rows {                                     // what a thread stages of a c
     E kt[NP][8][2];                               // components d, d + 1 of eight frames
     E v[8];                                       // the lane's column of eight frames
     u32x4 ws[NW];
-    __device__ __forceinline__ void load(const DeltaArgs& a, const E* kp, const E* qp, const E* vp, const char* wp, int t0, int len) {
-        const int tid = threadIdx.x, t = min(t0 + (tid & 31), len - 1);
-#pragma unroll
-        for (int n = 0; n < NW; ++n) ws[n] = *(const u32x4*)(wp + min(4096 * n + 16 * tid, kUnit - 16));
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = vp[min(t0 + 8 * (tid >> 4 & 3) + j, len - 1) * a.sv[1]];
+    // byte offsets from the chunk's first row (uniform pointer + 32-bit lane offset: no address arithmetic per chunk)
+    unsigned ok[NO], oq[NO], okt[NP][8], ov[8];
+    __device__ __forceinline__ void place(const DeltaArgs& a, int last_row) {
+        const int tid = threadIdx.x, t = min(tid & 31, last_row);
+        const int sk = (int)a.sk[1], sq = (int)a.sq[1], sv = (int)a.sv[1];
 #pragma unroll
         for (int n = 0; n < NO; ++n) {
-            const int d = 8 * ((tid >> 5) + 8 * n);
-            load_oct<E, MODE>(k[n], kp + t * a.sk[1], d, a.dk);
-            load_oct<E, MODE>(q[n], qp + t * a.sq[1], d, a.dk);
+            const int d = 8 * ((tid >> 5) + 8 * n), at = MODE == 0 ? (d < a.dk ? d : 0) : MODE == 1 ? min(d, a.dk - 8) : 0;
+            ok[n] = (unsigned)(t * sk + at) * sizeof(E);
+            oq[n] = (unsigned)(t * sq + at) * sizeof(E);
+        }
+#pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            const int d = 2 * ((tid >> 2) + 64 * n), at = MODE == 0 ? (d < a.dk ? d : 0) : MODE == 1 ? min(d, a.dk - 2) : 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) okt[n][j] = (unsigned)(min(8 * (tid & 3) + j, last_row) * sk + at) * sizeof(E);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ov[j] = (unsigned)(min(8 * (tid >> 4 & 3) + j, last_row) * sv) * sizeof(E);
+    }
+    __device__ __forceinline__ void load(const DeltaArgs& a, const E* kp, const E* qp, const E* vp, unsigned vcol, const char* wp, int t0) {
+        const int tid = threadIdx.x;
+        const char *kb = (const char*)(kp + t0 * a.sk[1]), *qb = (const char*)(qp + t0 * a.sq[1]), *vb = (const char*)(vp + t0 * a.sv[1]);
+#pragma unroll
+        for (int n = 0; n < NW; ++n) ws[n] = *(const u32x4*)(wp + (unsigned)min(4096 * n + 16 * tid, kUnit - 16));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = *(const E*)(vb + (ov[j] + vcol));
+#pragma unroll
+        for (int n = 0; n < NO; ++n) {
+            if (MODE == 2) {
+                k[n].load_clamped((const E*)(kb + ok[n]), 8 * ((tid >> 5) + 8 * n), a.dk);
+                q[n].load_clamped((const E*)(qb + oq[n]), 8 * ((tid >> 5) + 8 * n), a.dk);
+            } else {
+                k[n].load((const E*)(kb + ok[n]));
+                q[n].load((const E*)(qb + oq[n]));
+            }
         }
 #pragma unroll
         for (int n = 0; n < NP; ++n) {
             const int d = 2 * ((tid >> 2) + 64 * n);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const E* row = kp + min(t0 + 8 * (tid & 3) + j, len - 1) * a.sk[1];
-                if (MODE == 0) __builtin_memcpy(kt[n][j], row + (d < a.dk ? d : 0), 2 * sizeof(E));
-                else if (MODE == 1) __builtin_memcpy(kt[n][j], row + min(d, a.dk - 2), 2 * sizeof(E));
-                else { kt[n][j][0] = row[min(d, a.dk - 1)]; kt[n][j][1] = row[min(d + 1, a.dk - 1)]; }
+                const E* row = (const E*)(kb + okt[n][j]);
+                if (MODE == 2) { kt[n][j][0] = row[min(d, a.dk - 1)]; kt[n][j][1] = row[min(d + 1, a.dk - 1)]; }
+                else __builtin_memcpy(kt[n][j], row, 2 * sizeof(E));
             }
         }
     }
     __device__ __forceinline__ void store(const DeltaArgs& a, char* lds, int t0, int len) {
         using L = ScanLds<E, NK>;
         const int tid = threadIdx.x, t = tid & 31, row = 4 * (t >> 3) + (t & 3), I = t >> 2 & 1;
+        const bool edge = t0 + kC > len || a.dk != 32 * NK;       // (uniform) something of the 32 x 32 NK block is not there
 #pragma unroll
         for (int n = 0; n < NW; ++n)
             if (4096 * n + 16 * tid < kUnit) *(u32x4*)(lds + L::kWs + 4096 * n + 16 * tid) = ws[n];
@@ -230,8 +259,10 @@ struct Rows {                                     // what a thread stages of a c
             const int o = (tid >> 5) + 8 * n;
             if (o < 4 * NK) {
                 u32x4 pk[P], pq[P];
-                fix_oct<E, MODE>(k[n], 8 * o, a.dk, t0 + t < len);
-                fix_oct<E, MODE>(q[n], 8 * o, a.dk, t0 + t < len);
+                if (MODE != 0 || edge) {
+                    fix_oct<E, MODE>(k[n], 8 * o, a.dk, t0 + t < len);
+                    fix_oct<E, MODE>(q[n], 8 * o, a.dk, t0 + t < len);
+                }
                 k[n].planes(pk);
                 q[n].planes(pq);
                 char* at = lds + (2 * (o >> 2) + I) * kFrag + (row + 16 * (o & 3)) * 16;
@@ -252,7 +283,11 @@ struct Rows {                                     // what a thread stages of a c
                     const bool last = MODE == 1 && d == a.dk - 1;               // (the pair was loaded one component early)
                     E col[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) col[j] = dd < a.dk && t0 + 8 * (tid & 3) + j < len ? (last ? kt[n][j][1] : kt[n][j][x]) : (E)0;
+                    for (int j = 0; j < 8; ++j) col[j] = last ? kt[n][j][1] : kt[n][j][x];
+                    if (edge)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (dd >= a.dk || t0 + 8 * (tid & 3) + j >= len) col[j] = 0;
                     Oct<E> o;
                     u32x4 pt[P];
                     __builtin_memcpy(&o.v, col, sizeof(o.v));
@@ -283,10 +318,12 @@ MP_KERNEL __launch_bounds__(256) void mp_delta_scan(DeltaArgs a, int ncol) {
     const int len = length_of(a.lengths, b, a.T);
     const E* q = (const E*)a.q + b * a.sq[0] + hk * a.sq[2];
     const E* k = (const E*)a.k + b * a.sk[0] + hk * a.sk[2];
-    const E* v = (const E*)a.v + b * a.sv[0] + hv * a.sv[2] + cc;
+    const E* v = (const E*)a.v + b * a.sv[0] + hv * a.sv[2];
+    const unsigned vcol = cc * sizeof(E);
     const char* wsg = (const char*)a.ws + (size_t)(b * a.Hv + hv) * a.nchunk * ws_unit(PO);
-    E* o = (E*)a.o + ((size_t)b * a.T * a.Hv + hv) * a.dv + cc;
+    E* o = (E*)a.o + ((size_t)b * a.T * a.Hv + hv) * a.dv;
     const size_t so = (size_t)a.Hv * a.dv;
+    const unsigned olane = (unsigned)(8 * grp * so + cc) * sizeof(E);
     const size_t sbase = (size_t)(b * a.Hv + hv) * a.dk * a.dv + cc;
     f32x4 S[2 * NK];
 #pragma unroll
@@ -304,7 +341,8 @@ MP_KERNEL __launch_bounds__(256) void mp_delta_scan(DeltaArgs a, int ncol) {
     const int nc = (len + kC - 1) / kC;
     Rows<E, NK, MODE> rows;
     if (nc > 0) {
-        rows.load(a, k, q, v, wsg, 0, len);
+        rows.place(a, min(kC, a.T) - 1);
+        rows.load(a, k, q, v, vcol, wsg, 0);
         rows.store(a, lds, 0, len);
     }
     __syncthreads();
@@ -314,45 +352,70 @@ MP_KERNEL __launch_bounds__(256) void mp_delta_scan(DeltaArgs a, int ncol) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) vv[j] = rows.v[j];
         const int cn = min(c + 1, nc - 1);
-        rows.load(a, k, q, v, wsg + (size_t)cn * ws_unit(PO), cn * kC, len);
+        if (cn * kC + kC > a.T) rows.place(a, a.T - 1 - cn * kC);   // (rows behind the tensor's end)
+        rows.load(a, k, q, v, vcol, wsg + (size_t)cn * ws_unit(PO), cn * kC);
         __builtin_amdgcn_sched_barrier(0);                         // (the loads are issued here, not where their values are used)
+        // K S0 and Q S0, one pair of state tiles (32 components) a step: the operands and the terms of the next step are made while
+        // this one is multiplied
         f32x4 ks[2] = {}, qs[2] = {};
-#pragma unroll
-        for (int m = 0; m < NK; ++m) {
+        u32x4 fk[2][2][P], fq[2][2][P], sp[2][3];
+        auto step = [&](int m) {
             Oct<float> os;
-            u32x4 sp[3], s2[PO];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) os.v[j] = S[2 * m + (j >> 2)][j & 3];
-            os.planes(sp);
-#pragma unroll
-            for (int p = 0; p < PO; ++p) s2[p] = sp[p];
-#pragma unroll
-            for (int I = 0; I < 2; ++I) {
-                u32x4 fk[P], fq[P];
+            for (int I = 0; I < 2; ++I)
 #pragma unroll
                 for (int p = 0; p < P; ++p) {
-                    fk[p] = operand(lds + p * L::kPlane + (2 * m + I) * kFrag, lane);
-                    fq[p] = operand(lds + (P + p) * L::kPlane + (2 * m + I) * kFrag, lane);
+                    fk[m & 1][I][p] = operand(lds + p * L::kPlane + (2 * m + I) * kFrag, lane);
+                    fq[m & 1][I][p] = operand(lds + (P + p) * L::kPlane + (2 * m + I) * kFrag, lane);
                 }
-                ks[I] = mfma_planes(fk, sp, ks[I]);
-                qs[I] = mfma_planes(fq, s2, qs[I]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) os.v[j] = S[2 * m + (j >> 2)][j & 3];
+            os.planes(sp[m & 1]);
+        };
+        step(0);
+#pragma unroll
+        for (int m = 0; m < NK; ++m) {
+            if (m + 1 < NK) step(m + 1);
+            u32x4 s2[PO];
+#pragma unroll
+            for (int p = 0; p < PO; ++p) s2[p] = sp[m & 1][p];
+            constexpr int kProducts = P == 1 ? 3 + PO : 12;
+            ks[0] = mfma_planes(fk[m & 1][0], sp[m & 1], ks[0]);
+            ks[1] = mfma_planes(fk[m & 1][1], sp[m & 1], ks[1]);
+            qs[0] = mfma_planes(fq[m & 1][0], s2, qs[0]);
+            qs[1] = mfma_planes(fq[m & 1][1], s2, qs[1]);
+            if (m + 1 < NK) {
+#pragma unroll
+                for (int i = 0; i < 2 * kProducts; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);       // an LDS read,
+                    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);         // a matrix instruction,
+                    __builtin_amdgcn_sched_group_barrier(0x2, P == 1 ? 5 : 2, 0);   // vector instructions that fit behind it
+                }
             }
         }
-        float beta[8], eg[8], tail[8];
+        float beta[8], beg[8], seg[8], tail[8];
         __builtin_memcpy(beta, __builtin_assume_aligned(ws + kWsBeta + 32 * grp, 16), 32);
-        __builtin_memcpy(eg, __builtin_assume_aligned(ws + kWsEg + 32 * grp, 16), 32);
+        __builtin_memcpy(beg, __builtin_assume_aligned(ws + kWsBetaEg + 32 * grp, 16), 32);
+        __builtin_memcpy(seg, __builtin_assume_aligned(ws + kWsScaleEg + 32 * grp, 16), 32);
         __builtin_memcpy(tail, __builtin_assume_aligned(ws + kWsTail + 32 * grp, 16), 32);
-        const float whole = *(const float*)(ws + kWsEg + 4 * (kC - 1));
+        const float whole = *(const float*)(ws + kWsWhole);
+        u32x4 T[2][3];
+#pragma unroll
+        for (int I = 0; I < 2; ++I)
+#pragma unroll
+            for (int p = 0; p < 3; ++p) T[I][p] = operand(ws + kWsT + (I * 3 + p) * kFrag, lane);
+        const bool part = t0 + kC > len;                           // (uniform)
         Oct<float> R;
-        bool bad = false;
+        float odd = 0.f;                                           // stays 0 while everything is finite
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float vj = cok && t0 + 8 * grp + j < len ? load_f(&vv[j]) : 0.f;
-            R.v[j] = beta[j] * fmaf(-eg[j], ks[j >> 2][j & 3], vj);
-            bad |= not_finite(R.v[j]);
+            float vj = load_f(&vv[j]);
+            if (part && t0 + 8 * grp + j >= len) vj = 0.f;
+            R.v[j] = fmaf(-beg[j], ks[j >> 2][j & 3], beta[j] * vj);
+            odd = fmaf(0.f, R.v[j], odd);
         }
+        const bool any_bad = __any(odd != 0.f);
         int first = kC;                                            // this column's first row that is not finite
-        const bool any_bad = __any(bad);
         if (any_bad) {
 #pragma unroll
             for (int j = 7; j >= 0; --j)
@@ -366,55 +429,57 @@ MP_KERNEL __launch_bounds__(256) void mp_delta_scan(DeltaArgs a, int ncol) {
         u32x4 rp[3];
         R.planes(rp);
         f32x4 u[2] = {}, w[2] = {};
-#pragma unroll
-        for (int I = 0; I < 2; ++I) {
-            u32x4 T[3];
-#pragma unroll
-            for (int p = 0; p < 3; ++p) T[p] = operand(ws + kWsT + (I * 3 + p) * kFrag, lane);
-            u[I] = mfma_planes(T, rp, u[I]);
-        }
+        u[0] = mfma_planes(T[0], rp, u[0]);
+        u[1] = mfma_planes(T[1], rp, u[1]);
         Oct<float> U, Ut;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            U.v[j] = u[j >> 2][j & 3];
-            if (any_bad && 8 * grp + j >= first) U.v[j] = 0.f;
-            Ut.v[j] = tail[j] * U.v[j];
-        }
+        for (int j = 0; j < 8; ++j) U.v[j] = u[j >> 2][j & 3];
+        if (any_bad)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (8 * grp + j >= first) U.v[j] = 0.f;
+        // S' = e^{G_C} S0 + K^T (e^{G_C - G} U), and P U beside it
+        u32x4 Pm[2][PO], ft[4][P];
+        auto transposed = [&](int n) {
+#pragma unroll
+            for (int p = 0; p < P; ++p) ft[n & 3][p] = operand(lds + (2 * P + p) * L::kPlane + n * kFrag, lane);
+        };
+#pragma unroll
+        for (int n = 0; n < 3 && n < 2 * NK; ++n) transposed(n);
+#pragma unroll
+        for (int I = 0; I < 2; ++I)
+#pragma unroll
+            for (int p = 0; p < PO; ++p) Pm[I][p] = operand(ws + kWsP + (I * PO + p) * kFrag, lane);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) Ut.v[j] = tail[j] * U.v[j];
         u32x4 up[3], ut[3], u2[PO];
-        U.planes(up);
         Ut.planes(ut);
+        U.planes(up);
 #pragma unroll
         for (int p = 0; p < PO; ++p) u2[p] = up[p];
 #pragma unroll
-        for (int I = 0; I < 2; ++I) {
-            u32x4 Pm[PO];
-#pragma unroll
-            for (int p = 0; p < PO; ++p) Pm[p] = operand(ws + kWsP + (I * PO + p) * kFrag, lane);
-            w[I] = mfma_planes(Pm, u2, w[I]);
-        }
-        // S' = e^{G_C} S0 + K^T (e^{G_C - G} U)
-#pragma unroll
         for (int n = 0; n < 2 * NK; ++n) {
-            u32x4 ft[P];
-#pragma unroll
-            for (int p = 0; p < P; ++p) ft[p] = operand(lds + (2 * P + p) * L::kPlane + n * kFrag, lane);
-            S[n] = mfma_planes(ft, ut, S[n] * whole);
+            if (n + 3 < 2 * NK) transposed(n + 3);
+            S[n] = mfma_planes(ft[n & 3], ut, S[n] * whole);
         }
+        w[0] = mfma_planes(Pm[0], u2, w[0]);
+        w[1] = mfma_planes(Pm[1], u2, w[1]);
         float ov[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            ov[j] = fmaf(a.scale * eg[j], qs[j >> 2][j & 3], w[j >> 2][j & 3]);
+            ov[j] = fmaf(seg[j], qs[j >> 2][j & 3], w[j >> 2][j & 3]);
             if (any_bad && 8 * grp + j >= first) ov[j] = nan;
         }
-        E* out = o + (size_t)(t0 + 8 * grp) * so;
+        char* out = (char*)(o + (size_t)t0 * so);
+        const size_t sb = so * sizeof(E);
         if (cok) {
-            if (t0 + kC <= len) {
+            if (!part) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) store_f(out + j * so, ov[j]);
+                for (int j = 0; j < 8; ++j) store_f((E*)(out + j * sb + olane), ov[j]);
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    if (t0 + 8 * grp + j < len) store_f(out + j * so, ov[j]);
+                    if (t0 + 8 * grp + j < len) store_f((E*)(out + j * sb + olane), ov[j]);
             }
         }
         if (any_bad && first < kC)
@@ -427,7 +492,7 @@ MP_KERNEL __launch_bounds__(256) void mp_delta_scan(DeltaArgs a, int ncol) {
         __syncthreads();
     }
     if (cok)
-        for (int t = len + grp; t < a.T; t += 4) store_f(o + (size_t)t * so, 0.f);
+        for (int t = len + grp; t < a.T; t += 4) store_f(o + (size_t)t * so + cc, 0.f);
     if (a.s_out && cok)
 #pragma unroll
         for (int n = 0; n < 2 * NK; ++n)

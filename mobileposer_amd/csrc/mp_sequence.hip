@@ -37,7 +37,8 @@ int mp_delta_rule(mp_handle* h, int dtype, const void* q_dev, const void* k_dev,
     if (need && (!ws_dev || ws_bytes < need || (uintptr_t)ws_dev % 16))
         return fail(h, MP_ERR_INVALID, "mp_delta_rule: workspace of %zu bytes, %zu needed (16-byte aligned)", ws_bytes, need);
     const int64_t nchunk = ((int64_t)T + 31) / 32;
-    if ((int64_t)B * Hk * nchunk > kMaxBlocks || ((int64_t)B * Hk + 7) * (Hv / Hk) * (((int64_t)dv + 63) / 64) > kMaxBlocks)
+    if ((int64_t)B * Hk * nchunk > kMaxBlocks || ((int64_t)B * Hk + 7) * (Hv / Hk) * (((int64_t)dv + 63) / 64) > kMaxBlocks ||
+        (int64_t)Hv * dv > (1 << 24) - 1)
         return fail(h, MP_ERR_INVALID, "mp_delta_rule: batch of %d x %d frames, %d heads is too large for one call", B, T, Hv);
     ON_DEVICE(h);
     mpseq::DeltaArgs a;
@@ -45,6 +46,9 @@ int mp_delta_rule(mp_handle* h, int dtype, const void* q_dev, const void* k_dev,
     a.q = q_dev; a.k = k_dev; a.v = v_dev; a.g = g_dev; a.beta = beta_dev;
     if (strides)
         for (int i = 0; i < 3; ++i) {
+            // 32 frames are addressed with 32-bit byte offsets
+            if (T > 1 && (strides[3 * i + 1] < 0 || strides[3 * i + 1] > (1 << 24) - 1))
+                return fail(h, MP_ERR_INVALID, "mp_delta_rule: frame stride of %lld elements (0..2^24 - 1)", (long long)strides[3 * i + 1]);
             a.sq[i] = strides[i]; a.sk[i] = strides[3 + i]; a.sv[i] = strides[6 + i]; a.sg[i] = strides[9 + i]; a.sb[i] = strides[12 + i];
         }
     a.lengths = lengths_dev; a.B = B; a.T = T; a.Hk = Hk; a.Hv = Hv; a.dk = dk; a.dv = dv; a.scale = scale;
