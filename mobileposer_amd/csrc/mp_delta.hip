@@ -184,117 +184,84 @@ MP_KERNEL __launch_bounds__(64) void mp_delta_prep(DeltaArgs a) {
 }
 
 // The walk over the chunks: a workgroup per (sequence, value head, 64 columns of the state), a wave per 16 columns; NK = dk / 32
-// rounded up.  The workgroup stages K, Q and K^T of a chunk in LDS as ready operands (bf16 terms, one 16-byte read per lane and
-// operand) beside the chunk's workspace; the next chunk's rows are on their way through registers meanwhile, with no use of them --
-// not even a conversion -- before this chunk's products are done.
+// rounded up.  The workgroup stages a chunk in LDS -- K and Q as ready operands (bf16 terms, one 16-byte read per lane and operand;
+// K^T comes from K's operands by the turning reads), the chunk's workspace, the 64 columns of V, whose place the outputs take --
+// and the next chunk is on its way through registers meanwhile, with no use of its values before this chunk's products are done.
+constexpr int kFragK = kFrag + 256;               // K's operands: 64 bytes between the groups of eight components, or the 16 lanes of a
+                                                  // turning read would meet in a quarter of the banks
 template <class E, int NK>
 struct ScanLds {
-    static constexpr int P = Arith<E>::P, PO = P == 1 ? 2 : 3, kPlane = 2 * NK * kFrag, kWs = 3 * P * kPlane;      // K | Q | K^T | workspace
-    static constexpr int kBytes = kWs + ws_unit(PO);
+    static constexpr int P = Arith<E>::P, PO = P == 1 ? 2 : 3, kPlaneK = 2 * NK * kFragK, kPlaneQ = 2 * NK * kFrag;
+    static constexpr int kQ = P * kPlaneK, kWs = kQ + P * kPlaneQ, kV = kWs + (ws_unit(PO) + 15) / 16 * 16, kRowV = (64 + 16 / sizeof(E)) * sizeof(E);
+    static constexpr int kBytes = kV + kC * kRowV;
 };
 template <class E, int NK, int MODE>
 struct Rows {                                     // what a thread stages of a chunk
-    static constexpr int P = Arith<E>::P, NO = (4 * NK + 7) / 8, NP = (16 * NK + 63) / 64, kUnit = ws_unit(ScanLds<E, NK>::PO), NW = (kUnit + 4095) / 4096;
-    Oct<E> k[NO], q[NO];
-    E kt[NP][8][2];                               // components d, d + 1 of eight frames
-    E v[8];                                       // the lane's column of eight frames
+    using L = ScanLds<E, NK>;
+    static constexpr int P = L::P, NF = (2 * NK + 3) / 4, kUnit = ws_unit(L::PO), NW = (kUnit + 4095) / 4096;
+    Oct<E> k[NF], q[NF], v;
     u32x4 ws[NW];
-    // byte offsets from the chunk's first row (uniform pointer + 32-bit lane offset: no address arithmetic per chunk)
-    unsigned ok[NO], oq[NO], okt[NP][8], ov[8];
-    __device__ __forceinline__ void place(const DeltaArgs& a, int last_row) {
-        const int tid = threadIdx.x, t = min(tid & 31, last_row);
-        const int sk = (int)a.sk[1], sq = (int)a.sq[1], sv = (int)a.sv[1];
+    unsigned ok[NF], oq[NF], ov;                  // byte offsets from the chunk's first row
+    static __device__ __forceinline__ int frame(int f) { return row_index(f & 1, threadIdx.x & 15); }
+    static __device__ __forceinline__ int component(int f) { return 32 * (f >> 1) + 8 * (threadIdx.x >> 4 & 3); }
+    __device__ __forceinline__ void place(const DeltaArgs& a, int last_row, int c0) {
+        const int wave = threadIdx.x >> 6;
 #pragma unroll
-        for (int n = 0; n < NO; ++n) {
-            const int d = 8 * ((tid >> 5) + 8 * n), at = MODE == 0 ? (d < a.dk ? d : 0) : MODE == 1 ? min(d, a.dk - 8) : 0;
-            ok[n] = (unsigned)(t * sk + at) * sizeof(E);
-            oq[n] = (unsigned)(t * sq + at) * sizeof(E);
+        for (int n = 0; n < NF; ++n) {
+            const int f = min(wave + 4 * n, 2 * NK - 1), t = min(frame(f), last_row), d = component(f);
+            const int at = MODE == 0 ? (d < a.dk ? d : 0) : MODE == 1 ? min(d, a.dk - 8) : 0;
+            ok[n] = (unsigned)(t * (int)a.sk[1] + at) * sizeof(E);
+            oq[n] = (unsigned)(t * (int)a.sq[1] + at) * sizeof(E);
         }
-#pragma unroll
-        for (int n = 0; n < NP; ++n) {
-            const int d = 2 * ((tid >> 2) + 64 * n), at = MODE == 0 ? (d < a.dk ? d : 0) : MODE == 1 ? min(d, a.dk - 2) : 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) okt[n][j] = (unsigned)(min(8 * (tid & 3) + j, last_row) * sk + at) * sizeof(E);
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) ov[j] = (unsigned)(min(8 * (tid >> 4 & 3) + j, last_row) * sv) * sizeof(E);
+        const int col = c0 + 8 * (threadIdx.x & 7);
+        ov = (unsigned)(min((int)threadIdx.x >> 3, last_row) * (int)a.sv[1] + (a.dv < 8 ? 0 : min(col, a.dv - 8))) * sizeof(E);
     }
-    __device__ __forceinline__ void load(const DeltaArgs& a, const E* kp, const E* qp, const E* vp, unsigned vcol, const char* wp, int t0) {
-        const int tid = threadIdx.x;
+    __device__ __forceinline__ void load(const DeltaArgs& a, const E* kp, const E* qp, const E* vp, const char* wp, int t0, int c0) {
+        const int tid = threadIdx.x, wave = tid >> 6;
         const char *kb = (const char*)(kp + t0 * a.sk[1]), *qb = (const char*)(qp + t0 * a.sq[1]), *vb = (const char*)(vp + t0 * a.sv[1]);
 #pragma unroll
         for (int n = 0; n < NW; ++n) ws[n] = *(const u32x4*)(wp + (unsigned)min(4096 * n + 16 * tid, kUnit - 16));
+        if (a.dv >= 8) v.load((const E*)(vb + ov));
+        else v.load_clamped((const E*)(vb + ov), c0 + 8 * (tid & 7), a.dv);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = *(const E*)(vb + (ov[j] + vcol));
-#pragma unroll
-        for (int n = 0; n < NO; ++n) {
+        for (int n = 0; n < NF; ++n) {
             if (MODE == 2) {
-                k[n].load_clamped((const E*)(kb + ok[n]), 8 * ((tid >> 5) + 8 * n), a.dk);
-                q[n].load_clamped((const E*)(qb + oq[n]), 8 * ((tid >> 5) + 8 * n), a.dk);
+                const int d = component(min(wave + 4 * n, 2 * NK - 1));
+                k[n].load_clamped((const E*)(kb + ok[n]), d, a.dk);
+                q[n].load_clamped((const E*)(qb + oq[n]), d, a.dk);
             } else {
                 k[n].load((const E*)(kb + ok[n]));
                 q[n].load((const E*)(qb + oq[n]));
             }
         }
-#pragma unroll
-        for (int n = 0; n < NP; ++n) {
-            const int d = 2 * ((tid >> 2) + 64 * n);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const E* row = (const E*)(kb + okt[n][j]);
-                if (MODE == 2) { kt[n][j][0] = row[min(d, a.dk - 1)]; kt[n][j][1] = row[min(d + 1, a.dk - 1)]; }
-                else __builtin_memcpy(kt[n][j], row, 2 * sizeof(E));
-            }
-        }
     }
-    __device__ __forceinline__ void store(const DeltaArgs& a, char* lds, int t0, int len) {
-        using L = ScanLds<E, NK>;
-        const int tid = threadIdx.x, t = tid & 31, row = 4 * (t >> 3) + (t & 3), I = t >> 2 & 1;
+    __device__ __forceinline__ void store(const DeltaArgs& a, char* lds, int t0, int len, int c0) {
+        const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
         const bool edge = t0 + kC > len || a.dk != 32 * NK;       // (uniform) something of the 32 x 32 NK block is not there
 #pragma unroll
         for (int n = 0; n < NW; ++n)
             if (4096 * n + 16 * tid < kUnit) *(u32x4*)(lds + L::kWs + 4096 * n + 16 * tid) = ws[n];
+        const int col = c0 + 8 * (tid & 7);
+        if (a.dv % 8 && a.dv >= 8) v.shift(col - min(col, a.dv - 8));
+        if (t0 + (tid >> 3) >= len) v.zero();
+        __builtin_memcpy(__builtin_assume_aligned(lds + L::kV + (tid >> 3) * L::kRowV + 8 * (tid & 7) * sizeof(E), 16), &v.v, sizeof(v.v));
 #pragma unroll
-        for (int n = 0; n < NO; ++n) {
-            const int o = (tid >> 5) + 8 * n;
-            if (o < 4 * NK) {
+        for (int n = 0; n < NF; ++n) {
+            const int f = wave + 4 * n;
+            if (f < 2 * NK) {
                 u32x4 pk[P], pq[P];
                 if (MODE != 0 || edge) {
-                    fix_oct<E, MODE>(k[n], 8 * o, a.dk, t0 + t < len);
-                    fix_oct<E, MODE>(q[n], 8 * o, a.dk, t0 + t < len);
+                    fix_oct<E, MODE>(k[n], component(f), a.dk, t0 + frame(f) < len);
+                    fix_oct<E, MODE>(q[n], component(f), a.dk, t0 + frame(f) < len);
                 }
                 k[n].planes(pk);
                 q[n].planes(pq);
-                char* at = lds + (2 * (o >> 2) + I) * kFrag + (row + 16 * (o & 3)) * 16;
 #pragma unroll
                 for (int p = 0; p < P; ++p) {
-                    *(u32x4*)(at + p * L::kPlane) = pk[p];
-                    *(u32x4*)(at + (P + p) * L::kPlane) = pq[p];
+                    *(u32x4*)(lds + p * L::kPlaneK + f * kFragK + lane * 16 + (lane >> 4) * 64) = pk[p];
+                    *(u32x4*)(lds + L::kQ + p * L::kPlaneQ + f * kFrag + lane * 16) = pq[p];
                 }
             }
-        }
-#pragma unroll
-        for (int n = 0; n < NP; ++n) {
-            const int d = 2 * ((tid >> 2) + 64 * n);
-            if (d < 32 * NK)
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const int dd = d + x, tile = 2 * (dd >> 5) + (dd >> 2 & 1), rw = 4 * (dd >> 3 & 3) + (dd & 3);
-                    const bool last = MODE == 1 && d == a.dk - 1;               // (the pair was loaded one component early)
-                    E col[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) col[j] = last ? kt[n][j][1] : kt[n][j][x];
-                    if (edge)
-#pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            if (dd >= a.dk || t0 + 8 * (tid & 3) + j >= len) col[j] = 0;
-                    Oct<E> o;
-                    u32x4 pt[P];
-                    __builtin_memcpy(&o.v, col, sizeof(o.v));
-                    o.planes(pt);
-#pragma unroll
-                    for (int p = 0; p < P; ++p) *(u32x4*)(lds + (2 * P + p) * L::kPlane + tile * kFrag + (rw + 16 * (tid & 3)) * 16) = pt[p];
-                }
         }
     }
 };
@@ -312,19 +279,20 @@ MP_KERNEL __launch_bounds__(256) void mp_delta_scan(DeltaArgs a, int ncol) {
     const int rep = a.Hv / a.Hk, inner = rep * ncol, rest = blockIdx.x >> 3, unit = rest / inner * 8 + (blockIdx.x & 7);
     if (unit >= a.B * a.Hk) return;
     const int hk = unit % a.Hk, b = unit / a.Hk, hv = hk * rep + rest % inner / ncol;
-    const int cv = 64 * (rest % ncol) + 16 * (tid >> 6) + col;
+    const int c0 = 64 * (rest % ncol), cv = c0 + 16 * (tid >> 6) + col;
     const bool cok = cv < a.dv;
-    const int cc = cok ? cv : a.dv - 1;
     const int len = length_of(a.lengths, b, a.T);
     const E* q = (const E*)a.q + b * a.sq[0] + hk * a.sq[2];
     const E* k = (const E*)a.k + b * a.sk[0] + hk * a.sk[2];
     const E* v = (const E*)a.v + b * a.sv[0] + hv * a.sv[2];
-    const unsigned vcol = cc * sizeof(E);
     const char* wsg = (const char*)a.ws + (size_t)(b * a.Hv + hv) * a.nchunk * ws_unit(PO);
-    E* o = (E*)a.o + ((size_t)b * a.T * a.Hv + hv) * a.dv;
-    const size_t so = (size_t)a.Hv * a.dv;
-    const unsigned olane = (unsigned)(8 * grp * so + cc) * sizeof(E);
-    const size_t sbase = (size_t)(b * a.Hv + hv) * a.dk * a.dv + cc;
+    const size_t so = (size_t)a.Hv * a.dv, sbase = (size_t)(b * a.Hv + hv) * a.dk * a.dv + (cok ? cv : a.dv - 1);
+    // outputs leave as eight columns of a frame per thread, from the place of V
+    const int ocol = c0 + 8 * (tid & 7), ofull = a.dv - ocol;
+    E* o = (E*)a.o + ((size_t)b * a.T * a.Hv + hv) * a.dv + (size_t)(tid >> 3) * so + ocol;
+    char* const oplace = lds + L::kV + (tid >> 3) * L::kRowV + 8 * (tid & 7) * sizeof(E);
+    char* const vplace = lds + L::kV + 8 * grp * L::kRowV + (16 * (tid >> 6) + col) * sizeof(E);
+    const int turned = (4 * grp + (col >> 2)) * 16 + (col & 3) * 320;      // this lane's piece of a turning read of K's operands
     f32x4 S[2 * NK];
 #pragma unroll
     for (int n = 0; n < 2 * NK; ++n) S[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -341,32 +309,29 @@ MP_KERNEL __launch_bounds__(256) void mp_delta_scan(DeltaArgs a, int ncol) {
     const int nc = (len + kC - 1) / kC;
     Rows<E, NK, MODE> rows;
     if (nc > 0) {
-        rows.place(a, min(kC, a.T) - 1);
-        rows.load(a, k, q, v, vcol, wsg, 0);
-        rows.store(a, lds, 0, len);
+        rows.place(a, min(kC, a.T) - 1, c0);
+        rows.load(a, k, q, v, wsg, 0, c0);
+        rows.store(a, lds, 0, len, c0);
     }
     __syncthreads();
     for (int c = 0; c < nc; ++c) {
         const int t0 = c * kC;
-        E vv[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) vv[j] = rows.v[j];
         const int cn = min(c + 1, nc - 1);
-        if (cn * kC + kC > a.T) rows.place(a, a.T - 1 - cn * kC);   // (rows behind the tensor's end)
-        rows.load(a, k, q, v, vcol, wsg + (size_t)cn * ws_unit(PO), cn * kC);
+        if (cn * kC + kC > a.T) rows.place(a, a.T - 1 - cn * kC, c0);      // (rows behind the tensor's end)
+        rows.load(a, k, q, v, wsg + (size_t)cn * ws_unit(PO), cn * kC, c0);
         __builtin_amdgcn_sched_barrier(0);                         // (the loads are issued here, not where their values are used)
         // K S0 and Q S0, one pair of state tiles (32 components) a step: the operands and the terms of the next step are made while
         // this one is multiplied
-        f32x4 ks[2] = {}, qs[2] = {};
-        u32x4 fk[2][2][P], fq[2][2][P], sp[2][3];
+        f32x4 kq[4] = {};                                          // K S0: 0, 1, Q S0: 2, 3
+        u32x4 f[2][4][P], sp[2][3];
         auto step = [&](int m) {
             Oct<float> os;
 #pragma unroll
             for (int I = 0; I < 2; ++I)
 #pragma unroll
                 for (int p = 0; p < P; ++p) {
-                    fk[m & 1][I][p] = operand(lds + p * L::kPlane + (2 * m + I) * kFrag, lane);
-                    fq[m & 1][I][p] = operand(lds + (P + p) * L::kPlane + (2 * m + I) * kFrag, lane);
+                    f[m & 1][I][p] = *(const u32x4*)(lds + p * L::kPlaneK + (2 * m + I) * kFragK + lane * 16 + grp * 64);
+                    f[m & 1][2 + I][p] = operand(lds + L::kQ + p * L::kPlaneQ + (2 * m + I) * kFrag, lane);
                 }
 #pragma unroll
             for (int j = 0; j < 8; ++j) os.v[j] = S[2 * m + (j >> 2)][j & 3];
@@ -376,20 +341,24 @@ MP_KERNEL __launch_bounds__(256) void mp_delta_scan(DeltaArgs a, int ncol) {
 #pragma unroll
         for (int m = 0; m < NK; ++m) {
             if (m + 1 < NK) step(m + 1);
-            u32x4 s2[PO];
-#pragma unroll
-            for (int p = 0; p < PO; ++p) s2[p] = sp[m & 1][p];
-            constexpr int kProducts = P == 1 ? 3 + PO : 12;
-            ks[0] = mfma_planes(fk[m & 1][0], sp[m & 1], ks[0]);
-            ks[1] = mfma_planes(fk[m & 1][1], sp[m & 1], ks[1]);
-            qs[0] = mfma_planes(fq[m & 1][0], s2, qs[0]);
-            qs[1] = mfma_planes(fq[m & 1][1], s2, qs[1]);
+            if (P == 1) {                                          // Q S0 with the state's first two terms: its rounding is bf16's
+                u32x4 fk[2][P] = {{f[m & 1][0][0]}, {f[m & 1][1][0]}};
+                f32x4 lowest[2] = {kq[0], kq[1]};
+                u32x4 third[1] = {sp[m & 1][2]};
+                mfma_planes_n<2, P, 1>(fk, third, lowest);
+                kq[0] = lowest[0];
+                kq[1] = lowest[1];
+                u32x4 two[2] = {sp[m & 1][0], sp[m & 1][1]};
+                mfma_planes_n<4, P, 2>(f[m & 1], two, kq);
+            } else {
+                mfma_planes_n<4, P, 3>(f[m & 1], sp[m & 1], kq);
+            }
             if (m + 1 < NK) {
 #pragma unroll
-                for (int i = 0; i < 2 * kProducts; ++i) {
-                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);       // an LDS read,
-                    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);         // a matrix instruction,
-                    __builtin_amdgcn_sched_group_barrier(0x2, P == 1 ? 5 : 2, 0);   // vector instructions that fit behind it
+                for (int i = 0; i < (P == 1 ? 10 : 24); ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);               // an LDS read,
+                    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);                 // a matrix instruction,
+                    __builtin_amdgcn_sched_group_barrier(0x2, P == 1 ? 5 : 2, 0);    // vector instructions that fit behind it
                 }
             }
         }
@@ -404,17 +373,14 @@ MP_KERNEL __launch_bounds__(256) void mp_delta_scan(DeltaArgs a, int ncol) {
         for (int I = 0; I < 2; ++I)
 #pragma unroll
             for (int p = 0; p < 3; ++p) T[I][p] = operand(ws + kWsT + (I * 3 + p) * kFrag, lane);
-        const bool part = t0 + kC > len;                           // (uniform)
         Oct<float> R;
         float odd = 0.f;                                           // stays 0 while everything is finite
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            float vj = load_f(&vv[j]);
-            if (part && t0 + 8 * grp + j >= len) vj = 0.f;
-            R.v[j] = fmaf(-beg[j], ks[j >> 2][j & 3], beta[j] * vj);
+            R.v[j] = fmaf(-beg[j], kq[j >> 2][j & 3], beta[j] * load_f((const E*)(vplace + j * L::kRowV)));
             odd = fmaf(0.f, R.v[j], odd);
         }
-        const bool any_bad = __any(odd != 0.f);
+        const bool any_bad = __any(cok && odd != 0.f);
         int first = kC;                                            // this column's first row that is not finite
         if (any_bad) {
 #pragma unroll
@@ -429,8 +395,7 @@ MP_KERNEL __launch_bounds__(256) void mp_delta_scan(DeltaArgs a, int ncol) {
         u32x4 rp[3];
         R.planes(rp);
         f32x4 u[2] = {}, w[2] = {};
-        u[0] = mfma_planes(T[0], rp, u[0]);
-        u[1] = mfma_planes(T[1], rp, u[1]);
+        mfma_planes_n<2, 3, 3>(T, rp, u);
         Oct<float> U, Ut;
 #pragma unroll
         for (int j = 0; j < 8; ++j) U.v[j] = u[j >> 2][j & 3];
@@ -438,14 +403,19 @@ MP_KERNEL __launch_bounds__(256) void mp_delta_scan(DeltaArgs a, int ncol) {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 if (8 * grp + j >= first) U.v[j] = 0.f;
-        // S' = e^{G_C} S0 + K^T (e^{G_C - G} U), and P U beside it
-        u32x4 Pm[2][PO], ft[4][P];
-        auto transposed = [&](int n) {
+        // S' = e^{G_C} S0 + K^T (e^{G_C - G} U), four tiles a step, and P U beside it
+        u32x4 Pm[2][PO], ft[2][4][P];
+        auto turn = [&](int m) {
 #pragma unroll
-            for (int p = 0; p < P; ++p) ft[n & 3][p] = operand(lds + (2 * P + p) * L::kPlane + n * kFrag, lane);
+            for (int n = 0; n < 4 && 4 * m + n < 2 * NK; ++n)
+#pragma unroll
+                for (int p = 0; p < P; ++p) {
+                    const char* at = lds + p * L::kPlaneK + ((4 * m + n) & ~1) * kFragK + turned + 8 * (n & 1);
+                    const uint2 lo = read_turned(at), hi = read_turned(at + kFragK);
+                    ft[m & 1][n][p] = (u32x4){lo.x, lo.y, hi.x, hi.y};
+                }
         };
-#pragma unroll
-        for (int n = 0; n < 3 && n < 2 * NK; ++n) transposed(n);
+        turn(0);
 #pragma unroll
         for (int I = 0; I < 2; ++I)
 #pragma unroll
@@ -458,29 +428,26 @@ MP_KERNEL __launch_bounds__(256) void mp_delta_scan(DeltaArgs a, int ncol) {
 #pragma unroll
         for (int p = 0; p < PO; ++p) u2[p] = up[p];
 #pragma unroll
-        for (int n = 0; n < 2 * NK; ++n) {
-            if (n + 3 < 2 * NK) transposed(n + 3);
-            S[n] = mfma_planes(ft[n & 3], ut, S[n] * whole);
-        }
-        w[0] = mfma_planes(Pm[0], u2, w[0]);
-        w[1] = mfma_planes(Pm[1], u2, w[1]);
-        float ov[8];
+        for (int m = 0; m < (NK + 1) / 2; ++m) {
+            if (4 * m + 4 < 2 * NK) turn(m + 1);
+            if (4 * m + 4 <= 2 * NK) {
+                f32x4 s4[4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            ov[j] = fmaf(seg[j], qs[j >> 2][j & 3], w[j >> 2][j & 3]);
-            if (any_bad && 8 * grp + j >= first) ov[j] = nan;
-        }
-        char* out = (char*)(o + (size_t)t0 * so);
-        const size_t sb = so * sizeof(E);
-        if (cok) {
-            if (!part) {
+                for (int n = 0; n < 4; ++n) s4[n] = S[4 * m + n] * whole;
+                mfma_planes_n<4, P, 3>(ft[m & 1], ut, s4);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) store_f((E*)(out + j * sb + olane), ov[j]);
+                for (int n = 0; n < 4; ++n) S[4 * m + n] = s4[n];
             } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (t0 + 8 * grp + j < len) store_f((E*)(out + j * sb + olane), ov[j]);
+                for (int n = 0; n < 2; ++n) S[4 * m + n] = mfma_planes(ft[m & 1][n], ut, S[4 * m + n] * whole);
             }
+        }
+        mfma_planes_n<2, PO, PO>(Pm, u2, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float ov = fmaf(seg[j], kq[2 + (j >> 2)][j & 3], w[j >> 2][j & 3]);
+            if (any_bad && 8 * grp + j >= first) ov = nan;
+            store_f((E*)(vplace + j * L::kRowV), ov);
         }
         if (any_bad && first < kC)
 #pragma unroll
@@ -488,11 +455,26 @@ MP_KERNEL __launch_bounds__(256) void mp_delta_scan(DeltaArgs a, int ncol) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) S[n][r] = nan;
         __syncthreads();
-        if (c + 1 < nc) rows.store(a, lds, t0 + kC, len);
+        Oct<E> out;
+        __builtin_memcpy(&out.v, __builtin_assume_aligned(oplace, 16), sizeof(out.v));
+        if (c + 1 < nc) rows.store(a, lds, t0 + kC, len, c0);
         __syncthreads();
+        if (t0 + (tid >> 3) < len) {
+            E* at = o + (size_t)t0 * so;
+            if (ofull >= 8) __builtin_memcpy(at, &out.v, sizeof(out.v));
+            else {
+                E e[8];
+                __builtin_memcpy(e, &out.v, sizeof(e));
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (i < ofull) at[i] = e[i];
+            }
+        }
     }
-    if (cok)
-        for (int t = len + grp; t < a.T; t += 4) store_f(o + (size_t)t * so + cc, 0.f);
+    for (int t = len + (tid >> 3); t < a.T; t += 32) {
+        E* at = o + (size_t)(t - (tid >> 3)) * so;
+        for (int i = 0; i < min(8, ofull); ++i) at[i] = 0;
+    }
     if (a.s_out && cok)
 #pragma unroll
         for (int n = 0; n < 2 * NK; ++n)

@@ -104,6 +104,12 @@ static __device__ __forceinline__ void store4(bf16raw* p, const float (&y)[4]) {
 static __device__ __forceinline__ f32x4 mfma32(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
+// 4 x 16 blocks of 16-bit elements turned over on the way out of LDS: of 16 lanes each, lane 4 s + u reads elements 4 u .. 4 u + 3 of
+// row s and receives element 16-lane index of rows 0..3
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+static __device__ __forceinline__ uint2 read_turned(const char* lds_piece) {
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)lds_piece));
+}
 // sum of the products of planes whose orders add up to less than the number of planes that matter, the small ones first
 template <int PA, int PB>
 static __device__ __forceinline__ f32x4 mfma_planes(const u32x4 (&a)[PA], const u32x4 (&b)[PB], f32x4 c) {
@@ -114,6 +120,18 @@ static __device__ __forceinline__ f32x4 mfma_planes(const u32x4 (&a)[PA], const 
         for (int i = 0; i <= s; ++i)
             if (i < PA && s - i < PB) c = mfma32(a[i], b[s - i], c);
     return c;
+}
+// the same for N accumulators in turn, so that no product waits for the one before it
+template <int N, int PA, int PB>
+static __device__ __forceinline__ void mfma_planes_n(const u32x4 (&a)[N][PA], const u32x4 (&b)[PB], f32x4 (&c)[N]) {
+    constexpr int top = (PA > PB ? PA : PB) - 1;
+#pragma unroll
+    for (int s = top; s >= 0; --s)
+#pragma unroll
+        for (int i = 0; i <= s; ++i)
+            if (i < PA && s - i < PB)
+#pragma unroll
+                for (int n = 0; n < N; ++n) c[n] = mfma32(a[n][i], b[s - i], c[n]);
 }
 
 }  // namespace mpseq
