@@ -216,9 +216,8 @@ struct Rows {                                     // what a thread stages of a c
         const int col = c0 + 8 * (threadIdx.x & 7);
         ov = (unsigned)(min((int)threadIdx.x >> 3, last_row) * (int)a.sv[1] + (a.dv < 8 ? 0 : min(col, a.dv - 8))) * sizeof(E);
     }
-    __device__ __forceinline__ void load(const DeltaArgs& a, const E* kp, const E* qp, const E* vp, const char* wp, int t0, int c0) {
+    __device__ __forceinline__ void load(const DeltaArgs& a, const char* kb, const char* qb, const char* vb, const char* wp, int c0) {
         const int tid = threadIdx.x, wave = tid >> 6;
-        const char *kb = (const char*)(kp + t0 * a.sk[1]), *qb = (const char*)(qp + t0 * a.sq[1]), *vb = (const char*)(vp + t0 * a.sv[1]);
 #pragma unroll
         for (int n = 0; n < NW; ++n) ws[n] = *(const u32x4*)(wp + (unsigned)min(4096 * n + 16 * tid, kUnit - 16));
         if (a.dv >= 8) v.load((const E*)(vb + ov));
@@ -268,7 +267,7 @@ struct Rows {                                     // what a thread stages of a c
 static __device__ __forceinline__ u32x4 operand(const char* p, int lane) { return *(const u32x4*)(p + lane * 16); }
 
 template <class E, int NK, int MODE>
-MP_KERNEL __launch_bounds__(256) void mp_delta_scan(DeltaArgs a, int ncol) {
+MP_KERNEL __launch_bounds__(256, (Arith<E>::P == 1 ? NK <= 4 : NK <= 2) ? 2 : 1) void mp_delta_scan(DeltaArgs a, int ncol) {
     using L = ScanLds<E, NK>;
     constexpr int P = L::P, PO = L::PO;
     extern __shared__ __align__(16) char scan_lds[];
@@ -282,9 +281,10 @@ MP_KERNEL __launch_bounds__(256) void mp_delta_scan(DeltaArgs a, int ncol) {
     const int c0 = 64 * (rest % ncol), cv = c0 + 16 * (tid >> 6) + col;
     const bool cok = cv < a.dv;
     const int len = length_of(a.lengths, b, a.T);
-    const E* q = (const E*)a.q + b * a.sq[0] + hk * a.sq[2];
-    const E* k = (const E*)a.k + b * a.sk[0] + hk * a.sk[2];
-    const E* v = (const E*)a.v + b * a.sv[0] + hv * a.sv[2];
+    const char* q = (const char*)((const E*)a.q + b * a.sq[0] + hk * a.sq[2]);
+    const char* k = (const char*)((const E*)a.k + b * a.sk[0] + hk * a.sk[2]);
+    const char* v = (const char*)((const E*)a.v + b * a.sv[0] + hv * a.sv[2]);
+    const long kstep = kC * a.sk[1] * sizeof(E), qstep = kC * a.sq[1] * sizeof(E), vstep = kC * a.sv[1] * sizeof(E);
     const char* wsg = (const char*)a.ws + (size_t)(b * a.Hv + hv) * a.nchunk * ws_unit(PO);
     const size_t so = (size_t)a.Hv * a.dv, sbase = (size_t)(b * a.Hv + hv) * a.dk * a.dv + (cok ? cv : a.dv - 1);
     // outputs leave as eight columns of a frame per thread, from the place of V
@@ -310,15 +310,17 @@ MP_KERNEL __launch_bounds__(256) void mp_delta_scan(DeltaArgs a, int ncol) {
     Rows<E, NK, MODE> rows;
     if (nc > 0) {
         rows.place(a, min(kC, a.T) - 1, c0);
-        rows.load(a, k, q, v, wsg, 0, c0);
+        rows.load(a, k, q, v, wsg, c0);
         rows.store(a, lds, 0, len, c0);
     }
     __syncthreads();
     for (int c = 0; c < nc; ++c) {
         const int t0 = c * kC;
-        const int cn = min(c + 1, nc - 1);
-        if (cn * kC + kC > a.T) rows.place(a, a.T - 1 - cn * kC, c0);      // (rows behind the tensor's end)
-        rows.load(a, k, q, v, wsg + (size_t)cn * ws_unit(PO), cn * kC, c0);
+        if (c + 1 < nc) {                                          // (the last chunk asks for itself again: no branch around the loads)
+            k += kstep; q += qstep; v += vstep; wsg += ws_unit(PO);
+            if (t0 + 2 * kC > a.T) rows.place(a, a.T - 1 - t0 - kC, c0);   // (rows behind the tensor's end)
+        }
+        rows.load(a, k, q, v, wsg, c0);
         __builtin_amdgcn_sched_barrier(0);                         // (the loads are issued here, not where their values are used)
         // K S0 and Q S0, one pair of state tiles (32 components) a step: the operands and the terms of the next step are made while
         // this one is multiplied

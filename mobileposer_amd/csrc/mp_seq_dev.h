@@ -1,7 +1,7 @@
 // Device helpers of the sequence operators: operands of the bf16 matrix instructions from bf16 or fp32 data.
 //
-// An fp32 value as three bf16 terms -- hi + mid + lo, each the nearest to what is left -- keeps all 24 bits, and a product of two
-// such values is six products of terms: the three left out are below 2^-26 of it.  With fp32 accumulation that is the accuracy of
+// An fp32 value as three bf16 terms -- hi the nearest, mid the next eight bits, lo the rest -- keeps all 24 bits, and a product of
+// two such values is six products of terms: the three left out are below 2^-24 of it.  With fp32 accumulation that is the accuracy of
 // an fp32 sum at 16 / 6 times the rate of the fp32 matrix instructions; beside a bf16 operand, which is its own only term, it is
 // three products.  (An infinite value gives NaN: inf - inf in the split.)
 #pragma once
@@ -49,12 +49,24 @@ template <> struct Oct<bf16raw> {
 template <> struct Oct<float>;
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
-// two floats -> their nearest bf16 (one word, a in the low half), and what is left of them (exact)
+// two floats -> their nearest bf16 (one word, a in the low half)
+static __device__ __forceinline__ unsigned nearest_bf16(float a, float b) {
+    return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2){a, b}, bf16x2));
+}
+// the same, and what is left of them (exact).  Halves are rounded away from zero by integer arithmetic and cut: three instructions
+// of full rate a value where v_cvt_pk_bf16_f32 has a quarter of it
 static __device__ __forceinline__ unsigned take_bf16(float& a, float& b) {
-    const unsigned w = __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2){a, b}, bf16x2));
-    a -= __uint_as_float(w << 16);
-    b -= __uint_as_float(w & 0xffff0000u);
-    return w;
+    const unsigned x = __float_as_uint(a) + 0x8000u, y = __float_as_uint(b) + 0x8000u;
+    a -= __uint_as_float(x & 0xffff0000u);
+    b -= __uint_as_float(y & 0xffff0000u);
+    return __builtin_amdgcn_perm(y, x, 0x07060302u);
+}
+// the upper eight bits of what is left, cut, and the rest of it (exact)
+static __device__ __forceinline__ unsigned cut_bf16(float& a, float& b) {
+    const unsigned x = __float_as_uint(a), y = __float_as_uint(b);
+    a -= __uint_as_float(x & 0xffff0000u);
+    b -= __uint_as_float(y & 0xffff0000u);
+    return __builtin_amdgcn_perm(y, x, 0x07060302u);
 }
 template <> struct Oct<float> {
     float v[8];
@@ -86,8 +98,8 @@ template <> struct Oct<float> {
         for (int i = 0; i < 4; ++i) {
             float a = v[2 * i], b = v[2 * i + 1];
             o[0][i] = take_bf16(a, b);
-            o[1][i] = take_bf16(a, b);
-            o[2][i] = take_bf16(a, b);
+            o[1][i] = cut_bf16(a, b);
+            o[2][i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
         }
     }
 };
@@ -98,8 +110,7 @@ __device__ __forceinline__ float Oct<bf16raw>::dot(const Oct<float>& z, float s)
 }
 static __device__ __forceinline__ void store4(float* p, const float (&y)[4]) { *(float4*)p = {y[0], y[1], y[2], y[3]}; }
 static __device__ __forceinline__ void store4(bf16raw* p, const float (&y)[4]) {
-    float a = y[0], b = y[1], c = y[2], d = y[3];
-    *(uint2*)p = {take_bf16(a, b), take_bf16(c, d)};
+    *(uint2*)p = {nearest_bf16(y[0], y[1]), nearest_bf16(y[2], y[3])};
 }
 static __device__ __forceinline__ f32x4 mfma32(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
