@@ -20,11 +20,11 @@
 namespace mpseq {
 
 constexpr int kC = 32;                            // frames per chunk
-// Workspace of one (sequence, value head, chunk), bytes: T = (I + A)^{-1} as three terms and P = scale tril(Q K^T) o D as two (bf16
-// outputs) or three, in the order in which a lane of v_mfma_f32_16x16x32_bf16 takes its A operand, behind beta, beta e^G, scale e^G,
-// e^{G_C - G} of the 32 frames and e^{G_C}.
+// Workspace of one (sequence, value head, chunk), bytes: T = (I + A)^{-1} diag(beta) as three terms and P = scale tril(Q K^T) o D as two (bf16
+// outputs) or three, in the order in which a lane of v_mfma_f32_16x16x32_bf16 takes its A operand, behind e^G and e^{G_C - G} of the
+// 32 frames.
 constexpr int kFrag = 1024;                       // one 16 x 32 operand: 64 lanes x 8 bf16
-constexpr int kWsBeta = 0, kWsBetaEg = 4 * kC, kWsScaleEg = 8 * kC, kWsTail = 12 * kC, kWsWhole = 16 * kC, kWsT = kWsWhole + 16, kWsP = kWsT + 6 * kFrag;
+constexpr int kWsEg = 0, kWsTail = 4 * kC, kWsT = 8 * kC, kWsP = kWsT + 6 * kFrag;
 constexpr int ws_unit(int po) { return kWsP + 2 * po * kFrag; }
 
 size_t delta_ws_floats(int B, int T, int Hv) { return (size_t)B * Hv * ((T + kC - 1) / kC) * (ws_unit(3) / 4); }
@@ -111,12 +111,8 @@ MP_KERNEL __launch_bounds__(64) void mp_delta_prep(DeltaArgs a) {
         const double last = __shfl(G, kC - 1, 32);
         if (half < two) {
             char* ws = (char*)a.ws + ((size_t)(b * a.Hv + hh) * a.nchunk + c) * ws_unit(PO);
-            ((float*)(ws + kWsBeta))[i] = beta;
-            const float eg = expf((float)G);
-            ((float*)(ws + kWsBetaEg))[i] = beta * eg;
-            ((float*)(ws + kWsScaleEg))[i] = a.scale * eg;
+            ((float*)(ws + kWsEg))[i] = expf((float)G);
             ((float*)(ws + kWsTail))[i] = expf((float)(last - G));
-            if (i == kC - 1) *(float*)(ws + kWsWhole) = eg;
         }
         for (int e = 0; e < two; ++e) {
             char* ws = (char*)a.ws + ((size_t)(b * a.Hv + hk * rep + e0 + e) * a.nchunk + c) * ws_unit(PO);
@@ -166,7 +162,7 @@ MP_KERNEL __launch_bounds__(64) void mp_delta_prep(DeltaArgs a) {
         if (kC - 1 < i) x[kC - 1] = 0.f;
         __syncthreads();
 #pragma unroll
-        for (int n = 0; n < kC; ++n) A[half][n][i] = x[n];        // (with one head left, the other half's copy is not read)
+        for (int n = 0; n < kC; ++n) A[half][n][i] = n < i ? 0.f : x[n] * beta;        // (with one head left, the other half's copy is not read)
         __syncthreads();
         for (int e = 0; e < two; ++e) {
             char* ws = (char*)a.ws + ((size_t)(b * a.Hv + hk * rep + e0 + e) * a.nchunk + c) * ws_unit(PO);
@@ -322,6 +318,23 @@ MP_KERNEL __launch_bounds__(256, (Arith<E>::P == 1 ? NK <= 4 : NK <= 2) ? 2 : 1)
         }
         rows.load(a, k, q, v, wsg, c0);
         __builtin_amdgcn_sched_barrier(0);                         // (the loads are issued here, not where their values are used)
+        // (requested in front of the products that they wait for)
+        float eg[8], tail[8];
+        __builtin_memcpy(eg, __builtin_assume_aligned(ws + kWsEg + 32 * grp, 16), 32);
+        u32x4 T[2][3];
+#pragma unroll
+        for (int I = 0; I < 2; ++I)
+#pragma unroll
+            for (int p = 0; p < 3; ++p) T[I][p] = operand(ws + kWsT + (I * 3 + p) * kFrag, lane);
+        E vv[8];
+        if (P == 1) {
+            const char* at = lds + L::kV + (8 * grp + (col >> 2)) * L::kRowV + (16 * (tid >> 6) + 4 * (col & 3)) * sizeof(E);
+            const uint2 x[2] = {read_turned(at), read_turned(at + 4 * L::kRowV)};
+            __builtin_memcpy(vv, x, 16);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) vv[j] = *(const E*)(vplace + j * L::kRowV);
+        }
         // K S0 and Q S0, one pair of state tiles (32 components) a step: the operands and the terms of the next step are made while
         // this one is multiplied
         f32x4 kq[4] = {};                                          // K S0: 0, 1, Q S0: 2, 3
@@ -364,32 +377,26 @@ MP_KERNEL __launch_bounds__(256, (Arith<E>::P == 1 ? NK <= 4 : NK <= 2) ? 2 : 1)
                 }
             }
         }
-        float beta[8], beg[8], seg[8], tail[8];
-        __builtin_memcpy(beta, __builtin_assume_aligned(ws + kWsBeta + 32 * grp, 16), 32);
-        __builtin_memcpy(beg, __builtin_assume_aligned(ws + kWsBetaEg + 32 * grp, 16), 32);
-        __builtin_memcpy(seg, __builtin_assume_aligned(ws + kWsScaleEg + 32 * grp, 16), 32);
         __builtin_memcpy(tail, __builtin_assume_aligned(ws + kWsTail + 32 * grp, 16), 32);
-        const float whole = *(const float*)(ws + kWsWhole);
-        u32x4 T[2][3];
-#pragma unroll
-        for (int I = 0; I < 2; ++I)
-#pragma unroll
-            for (int p = 0; p < 3; ++p) T[I][p] = operand(ws + kWsT + (I * 3 + p) * kFrag, lane);
+        const float whole = *(const float*)(ws + kWsEg + 4 * (kC - 1));
         Oct<float> R;
         float odd = 0.f;                                           // stays 0 while everything is finite
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            R.v[j] = fmaf(-beg[j], kq[j >> 2][j & 3], beta[j] * load_f((const E*)(vplace + j * L::kRowV)));
+            R.v[j] = fmaf(-eg[j], kq[j >> 2][j & 3], load_f(&vv[j]));
             odd = fmaf(0.f, R.v[j], odd);
         }
-        const bool any_bad = __any(cok && odd != 0.f);
+        bool any_bad = __any(cok && odd != 0.f);
         int first = kC;                                            // this column's first row that is not finite
-        if (any_bad) {
+        auto find_first = [&](const Oct<float>& x) {
 #pragma unroll
             for (int j = 7; j >= 0; --j)
-                if (not_finite(R.v[j])) first = 8 * grp + j;
+                if (not_finite(x.v[j])) first = min(first, 8 * grp + j);
             first = min(first, __shfl_xor(first, 16));
             first = min(first, __shfl_xor(first, 32));
+        };
+        if (any_bad) {
+            find_first(R);
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 if (8 * grp + j >= first) R.v[j] = 0.f;
@@ -400,11 +407,17 @@ MP_KERNEL __launch_bounds__(256, (Arith<E>::P == 1 ? NK <= 4 : NK <= 2) ? 2 : 1)
         mfma_planes_n<2, 3, 3>(T, rp, u);
         Oct<float> U, Ut;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) U.v[j] = u[j >> 2][j & 3];
-        if (any_bad)
+        for (int j = 0; j < 8; ++j) {
+            U.v[j] = u[j >> 2][j & 3];
+            odd = fmaf(0.f, U.v[j], odd);
+        }
+        if (__any(cok && odd != 0.f)) {                            // (beta is in T)
+            any_bad = true;
+            find_first(U);
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 if (8 * grp + j >= first) U.v[j] = 0.f;
+        }
         // S' = e^{G_C} S0 + K^T (e^{G_C - G} U), four tiles a step, and P U beside it
         u32x4 Pm[2][PO], ft[2][4][P];
         auto turn = [&](int m) {
@@ -447,7 +460,7 @@ MP_KERNEL __launch_bounds__(256, (Arith<E>::P == 1 ? NK <= 4 : NK <= 2) ? 2 : 1)
         mfma_planes_n<2, PO, PO>(Pm, u2, w);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            float ov = fmaf(seg[j], kq[2 + (j >> 2)][j & 3], w[j >> 2][j & 3]);
+            float ov = fmaf(a.scale * eg[j], kq[2 + (j >> 2)][j & 3], w[j >> 2][j & 3]);
             if (any_bad && 8 * grp + j >= first) ov = nan;
             store_f((E*)(vplace + j * L::kRowV), ov);
         }
