@@ -279,13 +279,13 @@ enum { MP_F32 = 0, MP_BF16 = 1 };
  *   lengths_dev  [B] int32 or NULL (all T); values are clamped to 0..T.  Inputs behind a sequence's end are not read.
  *   o_dev        [B,T,Hv,dv] (dtype), contiguous; frames behind a sequence's end are zeros (as pad_packed_sequence has them)
  *   state_in_dev [B,Hv,dk,dv] fp32 or NULL (zeros);  state_out_dev the same or NULL; both may be the same buffer
- *   ws_dev       mp_delta_rule_workspace(B, T, Hv) bytes, 16-byte aligned: the caller's until the call's work is done
+ *   ws_dev       mp_delta_rule_workspace(B, T, Hv, dk, dv) bytes, 16-byte aligned: the caller's until the call's work is done
  * dk is at most 256.  A value that is not finite reaches the outputs of its own and later frames only. */
 int mp_delta_rule(mp_handle* h, int dtype, const void* q_dev, const void* k_dev, const void* v_dev, const float* g_dev,
                   const float* beta_dev, const int64_t strides[15], const int32_t* lengths_dev, int B, int T, int Hk, int Hv,
                   int dk, int dv, float scale, void* o_dev, const float* state_in_dev, float* state_out_dev, void* ws_dev,
                   size_t ws_bytes, void* stream);
-size_t mp_delta_rule_workspace(int B, int T, int Hv);
+size_t mp_delta_rule_workspace(int B, int T, int Hv, int dk, int dv);
 
 /* One frame of S streams: the same step on states that stay in place.  q_dev, k_dev [S,Hk,dk], v_dev [S,Hv,dv], g_dev, beta_dev
  * [S,Hv]; strides: 10 values, (stream, head) of q, k, v, g, beta; o_dev [S,Hv,dv] contiguous; state_dev [n_slots,Hv,dk,dv] fp32.

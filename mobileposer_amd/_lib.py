@@ -86,7 +86,7 @@ SIGNATURES = {
     "mp_stream_get_state": (_i, [_vp, _i, _vp, _fp, C.POINTER(C.c_double), _fp, C.POINTER(_i)]),
     "mp_stream_set_state": (_i, [_vp, _i, _vp, _fp, C.POINTER(C.c_double), _fp, C.POINTER(_i)]),
     "mp_delta_rule": (_i, [_vp, _i] + [_vp] * 7 + [_i] * 6 + [C.c_float] + [_vp] * 4 + [_sz, _vp]),
-    "mp_delta_rule_workspace": (_sz, [_i, _i, _i]),
+    "mp_delta_rule_workspace": (_sz, [_i, _i, _i, _i, _i]),
     "mp_delta_rule_online": (_i, [_vp, _i] + [_vp] * 7 + [_i] * 6 + [C.c_float] + [_vp] * 3),
     "mp_linear_adapted": (_i, [_vp, _i] + [_vp] * 8 + [_i] * 7 + [_vp, _vp, _sz, _vp]),
     "mp_linear_adapted_workspace": (_sz, [_i, _i, _i]),

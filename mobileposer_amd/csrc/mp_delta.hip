@@ -27,7 +27,6 @@ constexpr int kFrag = 1024;                       // one 16 x 32 operand: 64 lan
 constexpr int kWsEg = 0, kWsTail = 4 * kC, kWsT = 8 * kC, kWsP = kWsT + 6 * kFrag;
 constexpr int ws_unit(int po) { return kWsP + 2 * po * kFrag; }
 
-size_t delta_ws_floats(int B, int T, int Hv) { return (size_t)B * Hv * ((T + kC - 1) / kC) * (ws_unit(3) / 4); }
 
 // Which frame and which component of k a lane's registers stand for.  The accumulator layout of a 16 x 16 tile (lane: column
 // lane % 16, rows 4 (lane / 16) + r) becomes the B operand of a K = 32 instruction (lane: column lane % 16, k slots
@@ -40,6 +39,12 @@ static __device__ __forceinline__ int length_of(const int* lengths, int b, int T
     if (!lengths) return T;
     const int n = lengths[b];
     return n < 0 ? 0 : n > T ? T : n;
+}
+static __device__ __forceinline__ f32x4 mfma4(float4 a, float4 b, f32x4 c) {
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.x, b.x, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.y, b.y, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.z, b.z, c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(a.w, b.w, c, 0, 0, 0);
 }
 static __device__ __forceinline__ float clamp_g(float g) { return g < -1e4f ? -1e4f : g; }      // (NaN stays NaN)
 static __device__ __forceinline__ bool not_finite(float x) { return !(fabsf(x) <= 3.402823466e38f); }
@@ -260,10 +265,21 @@ struct Rows {                                     // what a thread stages of a c
         }
     }
 };
+// Left to itself the compiler puts every LDS read in front of its use, and a lone wave waits for each.  (fp32: the operands of a
+// step ahead are 96 registers more than a wave has beside another)
+#define FENCE() do { if (P == 1) __builtin_amdgcn_sched_barrier(0); } while (0)
 static __device__ __forceinline__ u32x4 operand(const char* p, int lane) { return *(const u32x4*)(p + lane * 16); }
 
-template <class E, int NK, int MODE>
-MP_KERNEL __launch_bounds__(256, (Arith<E>::P == 1 ? NK <= 4 : NK <= 2) ? 2 : 1) void mp_delta_scan(DeltaArgs a, int ncol) {
+// Few sequences and heads: the chunks are cut into segments that run side by side.  A segment maps the state it starts from linearly,
+// S -> M S + N; N [dk][dv] is its run from zero, column j of M [dk][dk] its run from the j-th unit vector with V = 0: the same
+// kernel without its outputs (OUT = false), dv + dk columns.  mp_delta_join carries the states through the segments, then all
+// segments run from their own start (OUT = true).  Three times the work, in 2 / segments of the steps.
+struct DeltaPlan {
+    int nseg, len;                                // segments and chunks per segment; nseg = 1: the chunks in one go
+    float *N, *M;                                 // [B][Hv][nseg - 1][dk][dv] (mp_delta_join turns N of s into the start of s + 1), [..][dk][dk]
+};
+template <class E, int NK, int MODE, bool OUT>
+MP_KERNEL __launch_bounds__(256, (Arith<E>::P == 1 ? NK <= 4 : NK <= 2) ? 2 : 1) void mp_delta_scan(DeltaArgs a, DeltaPlan plan, int ncol, int ncolm) {
     using L = ScanLds<E, NK>;
     constexpr int P = L::P, PO = L::PO;
     extern __shared__ __align__(16) char scan_lds[];
@@ -271,41 +287,56 @@ MP_KERNEL __launch_bounds__(256, (Arith<E>::P == 1 ? NK <= 4 : NK <= 2) ? 2 : 1)
     const char* const ws = lds + L::kWs;
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, grp = lane >> 4;
     // the workgroups that read the same K and Q on one XCD (workgroups are dealt to the 8 of them in turn)
-    const int rep = a.Hv / a.Hk, inner = rep * ncol, rest = blockIdx.x >> 3, unit = rest / inner * 8 + (blockIdx.x & 7);
-    if (unit >= a.B * a.Hk) return;
-    const int hk = unit % a.Hk, b = unit / a.Hk, hv = hk * rep + rest % inner / ncol;
-    const int c0 = 64 * (rest % ncol), cv = c0 + 16 * (tid >> 6) + col;
-    const bool cok = cv < a.dv;
-    const int len = length_of(a.lengths, b, a.T);
-    const char* q = (const char*)((const E*)a.q + b * a.sq[0] + hk * a.sq[2]);
-    const char* k = (const char*)((const E*)a.k + b * a.sk[0] + hk * a.sk[2]);
-    const char* v = (const char*)((const E*)a.v + b * a.sv[0] + hv * a.sv[2]);
+    const int rep = a.Hv / a.Hk, nc_all = ncol + ncolm, inner = rep * nc_all, nseg = OUT ? plan.nseg : plan.nseg - 1;
+    const int rest = blockIdx.x >> 3, unit = rest / inner * 8 + (blockIdx.x & 7);
+    if (unit >= a.B * a.Hk * nseg) return;
+    const int seg = unit / (a.B * a.Hk), hk = unit % a.Hk, b = unit / a.Hk % a.B, hv = hk * rep + rest % inner / nc_all;
+    const bool unitcol = !OUT && rest % nc_all >= ncol;            // columns of M
+    const int c0 = 64 * (unitcol ? rest % nc_all - ncol : rest % nc_all), cv = c0 + 16 * (tid >> 6) + col;
+    const int width = unitcol ? a.dk : a.dv;
+    const bool cok = cv < width;
+    const int len_all = length_of(a.lengths, b, a.T);
+    // this segment's frames, as a sequence that begins at its first
+    const int s0 = seg * plan.len * kC, len = min(len_all, seg + 1 == plan.nseg ? a.T : s0 + plan.len * kC) - s0;
+    if (!OUT && (len_all <= s0 + plan.len * kC || (unitcol && seg == 0))) return;      // (no segment follows; the first one's start is known)
+    const char* q = (const char*)((const E*)a.q + b * a.sq[0] + hk * a.sq[2] + s0 * a.sq[1]);
+    const char* k = (const char*)((const E*)a.k + b * a.sk[0] + hk * a.sk[2] + s0 * a.sk[1]);
+    const char* v = (const char*)((const E*)a.v + b * a.sv[0] + hv * a.sv[2] + s0 * a.sv[1]);
     const long kstep = kC * a.sk[1] * sizeof(E), qstep = kC * a.sq[1] * sizeof(E), vstep = kC * a.sv[1] * sizeof(E);
-    const char* wsg = (const char*)a.ws + (size_t)(b * a.Hv + hv) * a.nchunk * ws_unit(PO);
-    const size_t so = (size_t)a.Hv * a.dv, sbase = (size_t)(b * a.Hv + hv) * a.dk * a.dv + (cok ? cv : a.dv - 1);
+    const char* wsg = (const char*)a.ws + ((size_t)(b * a.Hv + hv) * a.nchunk + seg * plan.len) * ws_unit(PO);
+    const size_t so = (size_t)a.Hv * a.dv, head = (size_t)(b * a.Hv + hv), cc = cok ? cv : width - 1;
+    const float* s_in = seg == 0 ? a.s_in : OUT ? plan.N + (head * (plan.nseg - 1) + seg - 1) * a.dk * a.dv : nullptr;
+    if (seg == 0 && s_in) s_in += head * a.dk * a.dv;
+    const int tmax = a.T - s0;                                     // frames of the tensor from here on
     // outputs leave as eight columns of a frame per thread, from the place of V
     const int ocol = c0 + 8 * (tid & 7), ofull = a.dv - ocol;
-    E* o = (E*)a.o + ((size_t)b * a.T * a.Hv + hv) * a.dv + (size_t)(tid >> 3) * so + ocol;
+    E* o = (E*)a.o + (((size_t)b * a.T + s0) * a.Hv + hv) * a.dv + (size_t)(tid >> 3) * so + ocol;
     char* const oplace = lds + L::kV + (tid >> 3) * L::kRowV + 8 * (tid & 7) * sizeof(E);
     char* const vplace = lds + L::kV + 8 * grp * L::kRowV + (16 * (tid >> 6) + col) * sizeof(E);
     const int turned = (4 * grp + (col >> 2)) * 16 + (col & 3) * 320;      // this lane's piece of a turning read of K's operands
     f32x4 S[2 * NK];
 #pragma unroll
     for (int n = 0; n < 2 * NK; ++n) S[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    if (a.s_in)
+    if (unitcol) {
+#pragma unroll
+        for (int n = 0; n < 2 * NK; ++n)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) S[n][r] = 32 * (n >> 1) + row_index(n & 1, 4 * grp + r) == cv ? 1.f : 0.f;
+    } else if (s_in) {
 #pragma unroll
         for (int n = 0; n < 2 * NK; ++n)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int d = 32 * (n >> 1) + row_index(n & 1, 4 * grp + r);
-                const float x = a.s_in[sbase + (size_t)min(d, a.dk - 1) * a.dv];
+                const float x = s_in[cc + (size_t)min(d, a.dk - 1) * a.dv];
                 S[n][r] = d < a.dk ? x : 0.f;
             }
+    }
     const float nan = __builtin_nanf("");
-    const int nc = (len + kC - 1) / kC;
+    const int nc = len <= 0 ? 0 : (len + kC - 1) / kC;
     Rows<E, NK, MODE> rows;
     if (nc > 0) {
-        rows.place(a, min(kC, a.T) - 1, c0);
+        rows.place(a, min(kC, tmax) - 1, c0);
         rows.load(a, k, q, v, wsg, c0);
         rows.store(a, lds, 0, len, c0);
     }
@@ -314,11 +345,12 @@ MP_KERNEL __launch_bounds__(256, (Arith<E>::P == 1 ? NK <= 4 : NK <= 2) ? 2 : 1)
         const int t0 = c * kC;
         if (c + 1 < nc) {                                          // (the last chunk asks for itself again: no branch around the loads)
             k += kstep; q += qstep; v += vstep; wsg += ws_unit(PO);
-            if (t0 + 2 * kC > a.T) rows.place(a, a.T - 1 - t0 - kC, c0);   // (rows behind the tensor's end)
+            if (t0 + 2 * kC > tmax) rows.place(a, tmax - 1 - t0 - kC, c0);   // (rows behind the tensor's end)
         }
         rows.load(a, k, q, v, wsg, c0);
         __builtin_amdgcn_sched_barrier(0);                         // (the loads are issued here, not where their values are used)
         // (requested in front of the products that they wait for)
+        FENCE();
         float eg[8], tail[8];
         __builtin_memcpy(eg, __builtin_assume_aligned(ws + kWsEg + 32 * grp, 16), 32);
         u32x4 T[2][3];
@@ -339,51 +371,63 @@ MP_KERNEL __launch_bounds__(256, (Arith<E>::P == 1 ? NK <= 4 : NK <= 2) ? 2 : 1)
         // this one is multiplied
         f32x4 kq[4] = {};                                          // K S0: 0, 1, Q S0: 2, 3
         u32x4 f[2][4][P], sp[2][3];
-        auto step = [&](int m) {
-            Oct<float> os;
+        auto request = [&](int m) {
 #pragma unroll
             for (int I = 0; I < 2; ++I)
 #pragma unroll
                 for (int p = 0; p < P; ++p) {
                     f[m & 1][I][p] = *(const u32x4*)(lds + p * L::kPlaneK + (2 * m + I) * kFragK + lane * 16 + grp * 64);
-                    f[m & 1][2 + I][p] = operand(lds + L::kQ + p * L::kPlaneQ + (2 * m + I) * kFrag, lane);
+                    if (OUT) f[m & 1][2 + I][p] = operand(lds + L::kQ + p * L::kPlaneQ + (2 * m + I) * kFrag, lane);
                 }
+        };
+        auto split = [&](int m) {
+            Oct<float> os;
 #pragma unroll
             for (int j = 0; j < 8; ++j) os.v[j] = S[2 * m + (j >> 2)][j & 3];
             os.planes(sp[m & 1]);
         };
-        step(0);
+        request(0);
+        split(0);
 #pragma unroll
         for (int m = 0; m < NK; ++m) {
-            if (m + 1 < NK) step(m + 1);
-            if (P == 1) {                                          // Q S0 with the state's first two terms: its rounding is bf16's
-                u32x4 fk[2][P] = {{f[m & 1][0][0]}, {f[m & 1][1][0]}};
+            FENCE();
+            if (m + 1 < NK) request(m + 1);
+            FENCE();
+            if (!OUT) {
+                u32x4 fk[2][P];
+                f32x4 k2[2] = {kq[0], kq[1]};
+#pragma unroll
+                for (int p = 0; p < P; ++p) { fk[0][p] = f[m & 1][0][p]; fk[1][p] = f[m & 1][1][p]; }
+                mfma_planes_n<2, P, 3>(fk, sp[m & 1], k2);
+                kq[0] = k2[0];
+                kq[1] = k2[1];
+            } else if (P == 1) {                                   // Q S0 with the state's first two terms: its rounding is bf16's
+                u32x4 fk[2][P] = {{f[m & 1][0][0]}, {f[m & 1][1][0]}}, third[1] = {sp[m & 1][2]}, two[2] = {sp[m & 1][0], sp[m & 1][1]};
                 f32x4 lowest[2] = {kq[0], kq[1]};
-                u32x4 third[1] = {sp[m & 1][2]};
                 mfma_planes_n<2, P, 1>(fk, third, lowest);
                 kq[0] = lowest[0];
                 kq[1] = lowest[1];
-                u32x4 two[2] = {sp[m & 1][0], sp[m & 1][1]};
                 mfma_planes_n<4, P, 2>(f[m & 1], two, kq);
             } else {
                 mfma_planes_n<4, P, 3>(f[m & 1], sp[m & 1], kq);
             }
             if (m + 1 < NK) {
+                split(m + 1);
 #pragma unroll
-                for (int i = 0; i < (P == 1 ? 10 : 24); ++i) {
-                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);               // an LDS read,
+                for (int i = 0; i < (OUT ? P == 1 ? 10 : 24 : P == 1 ? 6 : 12); ++i) {
                     __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);                 // a matrix instruction,
                     __builtin_amdgcn_sched_group_barrier(0x2, P == 1 ? 5 : 2, 0);    // vector instructions that fit behind it
                 }
             }
         }
+        FENCE();
         __builtin_memcpy(tail, __builtin_assume_aligned(ws + kWsTail + 32 * grp, 16), 32);
         const float whole = *(const float*)(ws + kWsEg + 4 * (kC - 1));
         Oct<float> R;
         float odd = 0.f;                                           // stays 0 while everything is finite
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            R.v[j] = fmaf(-eg[j], kq[j >> 2][j & 3], load_f(&vv[j]));
+            R.v[j] = fmaf(-eg[j], kq[j >> 2][j & 3], unitcol ? 0.f : load_f(&vv[j]));
             odd = fmaf(0.f, R.v[j], odd);
         }
         bool any_bad = __any(cok && odd != 0.f);
@@ -403,6 +447,25 @@ MP_KERNEL __launch_bounds__(256, (Arith<E>::P == 1 ? NK <= 4 : NK <= 2) ? 2 : 1)
         }
         u32x4 rp[3];
         R.planes(rp);
+        u32x4 Pm[2][PO], ft[2][4][P];
+        auto turn = [&](int m) {
+#pragma unroll
+            for (int n = 0; n < 4 && 4 * m + n < 2 * NK; ++n)
+#pragma unroll
+                for (int p = 0; p < P; ++p) {
+                    const char* at = lds + p * L::kPlaneK + ((4 * m + n) & ~1) * kFragK + turned + 8 * (n & 1);
+                    const uint2 lo = read_turned(at), hi = read_turned(at + kFragK);
+                    ft[m & 1][n][p] = (u32x4){lo.x, lo.y, hi.x, hi.y};
+                }
+        };
+        FENCE();
+        turn(0);
+#pragma unroll
+        for (int I = 0; I < 2; ++I)
+#pragma unroll
+            for (int p = 0; p < PO; ++p)
+                if (OUT) Pm[I][p] = operand(ws + kWsP + (I * PO + p) * kFrag, lane);
+        FENCE();
         f32x4 u[2] = {}, w[2] = {};
         mfma_planes_n<2, 3, 3>(T, rp, u);
         Oct<float> U, Ut;
@@ -419,32 +482,20 @@ MP_KERNEL __launch_bounds__(256, (Arith<E>::P == 1 ? NK <= 4 : NK <= 2) ? 2 : 1)
                 if (8 * grp + j >= first) U.v[j] = 0.f;
         }
         // S' = e^{G_C} S0 + K^T (e^{G_C - G} U), four tiles a step, and P U beside it
-        u32x4 Pm[2][PO], ft[2][4][P];
-        auto turn = [&](int m) {
-#pragma unroll
-            for (int n = 0; n < 4 && 4 * m + n < 2 * NK; ++n)
-#pragma unroll
-                for (int p = 0; p < P; ++p) {
-                    const char* at = lds + p * L::kPlaneK + ((4 * m + n) & ~1) * kFragK + turned + 8 * (n & 1);
-                    const uint2 lo = read_turned(at), hi = read_turned(at + kFragK);
-                    ft[m & 1][n][p] = (u32x4){lo.x, lo.y, hi.x, hi.y};
-                }
-        };
-        turn(0);
-#pragma unroll
-        for (int I = 0; I < 2; ++I)
-#pragma unroll
-            for (int p = 0; p < PO; ++p) Pm[I][p] = operand(ws + kWsP + (I * PO + p) * kFrag, lane);
 #pragma unroll
         for (int j = 0; j < 8; ++j) Ut.v[j] = tail[j] * U.v[j];
         u32x4 up[3], ut[3], u2[PO];
         Ut.planes(ut);
-        U.planes(up);
+        if (OUT) {
+            U.planes(up);
 #pragma unroll
-        for (int p = 0; p < PO; ++p) u2[p] = up[p];
+            for (int p = 0; p < PO; ++p) u2[p] = up[p];
+        }
 #pragma unroll
         for (int m = 0; m < (NK + 1) / 2; ++m) {
+            FENCE();
             if (4 * m + 4 < 2 * NK) turn(m + 1);
+            FENCE();
             if (4 * m + 4 <= 2 * NK) {
                 f32x4 s4[4];
 #pragma unroll
@@ -457,9 +508,9 @@ MP_KERNEL __launch_bounds__(256, (Arith<E>::P == 1 ? NK <= 4 : NK <= 2) ? 2 : 1)
                 for (int n = 0; n < 2; ++n) S[4 * m + n] = mfma_planes(ft[m & 1][n], ut, S[4 * m + n] * whole);
             }
         }
-        mfma_planes_n<2, PO, PO>(Pm, u2, w);
+        if (OUT) mfma_planes_n<2, PO, PO>(Pm, u2, w);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; OUT && j < 8; ++j) {
             float ov = fmaf(a.scale * eg[j], kq[2 + (j >> 2)][j & 3], w[j >> 2][j & 3]);
             if (any_bad && 8 * grp + j >= first) ov = nan;
             store_f((E*)(vplace + j * L::kRowV), ov);
@@ -471,10 +522,10 @@ MP_KERNEL __launch_bounds__(256, (Arith<E>::P == 1 ? NK <= 4 : NK <= 2) ? 2 : 1)
                 for (int r = 0; r < 4; ++r) S[n][r] = nan;
         __syncthreads();
         Oct<E> out;
-        __builtin_memcpy(&out.v, __builtin_assume_aligned(oplace, 16), sizeof(out.v));
+        if (OUT) __builtin_memcpy(&out.v, __builtin_assume_aligned(oplace, 16), sizeof(out.v));
         if (c + 1 < nc) rows.store(a, lds, t0 + kC, len, c0);
         __syncthreads();
-        if (t0 + (tid >> 3) < len) {
+        if (OUT && t0 + (tid >> 3) < len) {
             E* at = o + (size_t)t0 * so;
             if (ofull >= 8) __builtin_memcpy(at, &out.v, sizeof(out.v));
             else {
@@ -486,29 +537,140 @@ MP_KERNEL __launch_bounds__(256, (Arith<E>::P == 1 ? NK <= 4 : NK <= 2) ? 2 : 1)
             }
         }
     }
-    for (int t = len + (tid >> 3); t < a.T; t += 32) {
-        E* at = o + (size_t)(t - (tid >> 3)) * so;
-        for (int i = 0; i < min(8, ofull); ++i) at[i] = 0;
+    float* s_out = nullptr;
+    size_t pitch = a.dv;
+    if (OUT) {
+        const int end = seg + 1 == plan.nseg ? tmax : min(tmax, plan.len * kC);
+        for (int t = max(len, 0) + (tid >> 3); t < end; t += 32) {
+            E* at = o + (size_t)(t - (tid >> 3)) * so;
+            for (int i = 0; i < min(8, ofull); ++i) at[i] = 0;
+        }
+        // the segment with the sequence's last frame
+        if (a.s_out && (len > 0 || seg == 0) && (seg + 1 == plan.nseg || len_all <= s0 + plan.len * kC)) s_out = a.s_out + head * a.dk * a.dv;
+    } else {
+        pitch = width;
+        s_out = unitcol ? plan.M + (head * (plan.nseg - 1) + seg) * a.dk * a.dk : plan.N + (head * (plan.nseg - 1) + seg) * a.dk * a.dv;
     }
-    if (a.s_out && cok)
+    if (s_out && cok)
 #pragma unroll
         for (int n = 0; n < 2 * NK; ++n)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int d = 32 * (n >> 1) + row_index(n & 1, 4 * grp + r);
-                if (d < a.dk) a.s_out[sbase + (size_t)d * a.dv] = S[n][r];
+                if (d < a.dk) s_out[cv + d * pitch] = S[n][r];
             }
 }
 
-template <class E, int NK, int MODE>
-static bool scan_for(const DeltaArgs& a, hipStream_t s) {
+// The start of every segment: S_{s+1} = M_s S_s + N_s, in place of N_s.  A workgroup per (sequence, value head, 16 columns), a wave
+// per 16 rows (two for dk > 128), on the fp32 matrix instructions; S_s goes round through LDS, M of the next segment is on its way
+// while this one is multiplied.  KT = dk / 16 rounded up.
+template <int KT>
+MP_KERNEL __launch_bounds__(512) void mp_delta_join(DeltaArgs a, DeltaPlan plan, int ncol) {
+    constexpr int NT = (KT + 7) / 8;
+    constexpr bool kAhead = KT <= 8;              // (both would not fit the registers)
+    __shared__ float St[16 * KT][17];
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, grp = lane >> 4, wave = tid >> 6;
+    const int ct = blockIdx.x % ncol, head = blockIdx.x / ncol, b = head / a.Hv;
+    const int cv = 16 * ct + col, cc = min(cv, a.dv - 1);
+    // segments behind which another one begins; the first one's N is its end state
+    const int n = min(plan.nseg - 1, (length_of(a.lengths, b, a.T) + plan.len * kC - 1) / (plan.len * kC) - 1);
+    float* N = plan.N + (size_t)head * (plan.nseg - 1) * a.dk * a.dv;
+    const float* M = plan.M + (size_t)head * (plan.nseg - 1) * a.dk * a.dk;
+    if (n < 2) return;
+    for (int d = tid >> 4; d < 16 * KT; d += 32) St[d][tid & 15] = d < a.dk ? N[(size_t)d * a.dv + min(16 * ct + (tid & 15), a.dv - 1)] : 0.f;
+    float4 m[NT][KT], mn[kAhead ? NT : 1][kAhead ? KT : 1];
+    f32x4 acc[NT], an[NT];
+    auto fetch = [&](int s, auto& mn) {
+        const float* Ms = M + (size_t)s * a.dk * a.dk;
+        const float* Ns = N + (size_t)s * a.dk * a.dv;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int row = min(16 * (wave + 8 * t) + col, a.dk - 1);
+#pragma unroll
+            for (int k = 0; k < KT; ++k) {
+                const int d = 16 * k + 4 * grp;
+                const float* p = Ms + (size_t)row * a.dk;
+                mn[t][k] = {p[min(d, a.dk - 1)], p[min(d + 1, a.dk - 1)], p[min(d + 2, a.dk - 1)], p[min(d + 3, a.dk - 1)]};
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) an[t][r] = Ns[(size_t)min(16 * (wave + 8 * t) + 4 * grp + r, a.dk - 1) * a.dv + cc];
+        }
+    };
+    if constexpr (kAhead) fetch(1, mn);
+    for (int s = 1; s < n; ++s) {
+        if constexpr (!kAhead) fetch(s, m);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[t] = an[t];
+        if constexpr (kAhead) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int k = 0; k < KT; ++k) m[t][k] = mn[t][k];
+            fetch(min(s + 1, n - 1), mn);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < KT; ++k) {
+            const int d = 16 * k + 4 * grp;
+            const float4 x = {St[d][col], St[d + 1][col], St[d + 2][col], St[d + 3][col]};      // (zeros behind dk)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) acc[t] = mfma4(m[t][k], x, acc[t]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int d = 16 * (wave + 8 * t) + 4 * grp + r;
+                if (d < a.dk) {
+                    St[d][col] = acc[t][r];
+                    if (cv < a.dv) N[((size_t)s * a.dk + d) * a.dv + cv] = acc[t][r];
+                }
+            }
+    }
+}
+
+// Segments: as many as fill the chip twice over in the first pass (a workgroup per CU leaves half of each SIMD's issue slots), at
+// least four chunks each; from four on they win (3 x the work in 2 / segments of the steps).
+static DeltaPlan plan_of(int B, int T, int Hv, int dk, int dv) {
+    DeltaPlan p = {1, (T + kC - 1) / kC, nullptr, nullptr};
+    const long per = (long)B * Hv * ((dv + 63) / 64 + (dk + 63) / 64);
+    const int nchunk = p.len, want = (int)min((long)nchunk / 4, 512 / per);
+    if (want >= 4) {
+        p.len = (nchunk + want - 1) / want;
+        p.nseg = (nchunk + p.len - 1) / p.len;
+    }
+    return p;
+}
+static size_t prep_floats(int B, int T, int Hv) { return (size_t)B * Hv * ((T + kC - 1) / kC) * (ws_unit(3) / 4); }
+size_t delta_ws_floats(int B, int T, int Hv, int dk, int dv) {
+    return prep_floats(B, T, Hv) + (size_t)B * Hv * (plan_of(B, T, Hv, dk, dv).nseg - 1) * dk * (dk + dv);
+}
+
+template <class E, int NK, int MODE, bool OUT>
+static bool scan_pass(const DeltaArgs& a, const DeltaPlan& p, hipStream_t s) {
     constexpr int bytes = ScanLds<E, NK>::kBytes;
     static_assert(bytes <= 160 * 1024, "LDS of a CU");
     // (an attribute of the function on the current device: set at every launch, a call may come from any device's handle)
-    if (bytes > 64 * 1024 && hipFuncSetAttribute((const void*)mp_delta_scan<E, NK, MODE>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return false;
-    const int ncol = (a.dv + 63) / 64, units = a.B * a.Hk;
-    hipLaunchKernelGGL((mp_delta_scan<E, NK, MODE>), dim3((unsigned)((units + 7) / 8 * 8 * (a.Hv / a.Hk) * ncol)), dim3(256), bytes, s, a, ncol);
+    if (bytes > 64 * 1024 && hipFuncSetAttribute((const void*)mp_delta_scan<E, NK, MODE, OUT>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return false;
+    const int ncol = (a.dv + 63) / 64, ncolm = OUT ? 0 : (a.dk + 63) / 64, units = a.B * a.Hk * (OUT ? p.nseg : p.nseg - 1);
+    hipLaunchKernelGGL((mp_delta_scan<E, NK, MODE, OUT>), dim3((unsigned)((units + 7) / 8 * 8 * (a.Hv / a.Hk) * (ncol + ncolm))), dim3(256), bytes, s, a, p, ncol, ncolm);
     return true;
+}
+template <class E, int NK, int MODE>
+static bool scan_for(const DeltaArgs& a, hipStream_t s) {
+    DeltaPlan p = plan_of(a.B, a.T, a.Hv, a.dk, a.dv);
+    if (p.nseg > 1) {
+        p.N = a.ws + prep_floats(a.B, a.T, a.Hv);
+        p.M = p.N + (size_t)a.B * a.Hv * (p.nseg - 1) * a.dk * a.dv;
+        if (!scan_pass<E, NK, MODE, false>(a, p, s)) return false;
+        const int ncol = (a.dv + 15) / 16;
+        const dim3 grid((unsigned)(a.B * a.Hv * ncol));
+        if (a.dk <= 64) hipLaunchKernelGGL(mp_delta_join<4>, grid, dim3(512), 0, s, a, p, ncol);
+        else if (a.dk <= 128) hipLaunchKernelGGL(mp_delta_join<8>, grid, dim3(512), 0, s, a, p, ncol);
+        else hipLaunchKernelGGL(mp_delta_join<16>, grid, dim3(512), 0, s, a, p, ncol);
+    }
+    return scan_pass<E, NK, MODE, true>(a, p, s);
 }
 template <class E, int PO, int MODE>
 static bool launch_mode(const DeltaArgs& a, hipStream_t s) {

@@ -43,7 +43,7 @@ struct DeltaOnlineArgs {
     void* o;                                     // [S][Hv][dv]
     float* state;                                // [n_slots][Hv][dk][dv], updated in place
 };
-size_t delta_ws_floats(int B, int T, int Hv);
+size_t delta_ws_floats(int B, int T, int Hv, int dk, int dv);
 bool launch_delta(const DeltaArgs& a, int dtype, hipStream_t s);
 bool launch_delta_online(const DeltaOnlineArgs& a, int dtype, hipStream_t s);
 

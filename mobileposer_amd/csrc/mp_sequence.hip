@@ -18,8 +18,8 @@ bool heads_ok(int Hk, int Hv, int dk, int dv) { return Hk >= 1 && Hv >= 1 && Hv 
 
 extern "C" {
 
-size_t mp_delta_rule_workspace(int B, int T, int Hv) {
-    return B < 1 || T < 1 || Hv < 1 ? 0 : mpseq::delta_ws_floats(B, T, Hv) * sizeof(float);
+size_t mp_delta_rule_workspace(int B, int T, int Hv, int dk, int dv) {
+    return B < 1 || T < 1 || Hv < 1 || dk < 1 || dv < 1 ? 0 : mpseq::delta_ws_floats(B, T, Hv, dk, dv) * sizeof(float);
 }
 
 int mp_delta_rule(mp_handle* h, int dtype, const void* q_dev, const void* k_dev, const void* v_dev, const float* g_dev,
@@ -33,7 +33,7 @@ int mp_delta_rule(mp_handle* h, int dtype, const void* q_dev, const void* k_dev,
     if (B == 0) return MP_OK;
     if (T > 0 && (!q_dev || !k_dev || !v_dev || !g_dev || !beta_dev || !strides || !o_dev))
         return fail(h, MP_ERR_INVALID, "mp_delta_rule: NULL buffer");
-    const size_t need = mp_delta_rule_workspace(B, T, Hv);
+    const size_t need = mp_delta_rule_workspace(B, T, Hv, dk, dv);
     if (need && (!ws_dev || ws_bytes < need || (uintptr_t)ws_dev % 16))
         return fail(h, MP_ERR_INVALID, "mp_delta_rule: workspace of %zu bytes, %zu needed (16-byte aligned)", ws_bytes, need);
     const int64_t nchunk = ((int64_t)T + 31) / 32;

@@ -100,7 +100,7 @@ class SequenceOps:
         dev = q.device
         o = torch.empty(B, T, Hv, dv, device=dev, dtype=q.dtype)
         out = torch.empty(B, Hv, dk, dv, device=dev, dtype=torch.float32)
-        need = self._lib.mp_delta_rule_workspace(B, T, Hv)
+        need = self._lib.mp_delta_rule_workspace(B, T, Hv, dk, dv)
         ws = torch.empty(need, device=dev, dtype=torch.uint8)
         st = (C.c_int64 * 15)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *g.stride(), *beta.stride())
         self._check(self._lib.mp_delta_rule(

@@ -106,6 +106,39 @@ def test_delta_rule(ops, shape, dtype):
             assert not npy(o[b, lens[b]:].float()).any()
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("shape", [(1, 512, 1, 1, 64, 64), (2, 1000, 1, 2, 64, 40), (1, 1400, 1, 1, 128, 130), (1, 530, 1, 1, 200, 20), (3, 777, 1, 1, 7, 5), (1, 3000, 1, 1, 72, 33)], ids=str)
+def test_delta_rule_long_sequences_on_few_heads(ops, shape, dtype):
+    """Long enough, and few enough, to be run as segments side by side; ragged: a sequence that ends inside a segment, at a border
+    between two, in the first one, and an empty one."""
+    import torch
+    B, T, Hk, Hv, dk, dv = shape
+    q, k, v, g, beta, s0 = delta_inputs(14, B, T, Hk, Hv, dk, dv, getattr(torch, dtype))
+    for lens in ([T] * B, [T - 300] + [T - 33, 0][:B - 1], [128] + [T - 1, 1][:B - 1]):
+        for state in (None, s0):
+            o, s = ops.delta_rule(q, k, v, g, beta, lens, state)
+            wo, ws, top = delta_ref(q, k, v, g, beta, lens, state, dk ** -0.5)
+            assert_delta(o, s, wo, ws, delta_tol(T, dk, max(top, float(v.float().abs().max()))), dtype == "bfloat16")
+
+
+@pytest.mark.parametrize("where", ["k", "v", "g", "state"])
+def test_delta_rule_non_finite_values_in_segments(ops, where):
+    import torch
+    T, dk, dv, t0 = 900, 32, 20, 333
+    q, k, v, g, beta, s0 = delta_inputs(15, 1, T, 1, 1, dk, dv, torch.float32)
+    clean = ops.delta_rule(q, k, v, g, beta, None, s0)
+    {"k": k[0, t0, 0], "v": v[0, t0, 0], "g": g[0, t0], "state": s0[0, 0, 3]}[where][0 if where == "g" else 7] = float("nan")
+    o, s = ops.delta_rule(q, k, v, g, beta, None, s0)
+    hit = torch.zeros(1, T, 1, dv, dtype=torch.bool, device="cuda")
+    if where in ("v", "state"):
+        hit[:, t0 if where == "v" else 0:, :, 7] = True
+    else:
+        hit[:, t0:] = True
+    assert torch.equal(torch.isnan(o), hit)
+    assert torch.equal(torch.isnan(s), hit[0, -1, 0].expand(1, 1, dk, dv))
+    assert torch.equal(o[~hit], clean[0][~hit])
+
+
 def test_delta_rule_lengths_strides_and_garbage_behind_the_end(ops):
     import torch
     B, T, Hk, Hv, dk, dv = 4, 80, 2, 4, 72, 40

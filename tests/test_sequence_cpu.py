@@ -63,7 +63,7 @@ def test_entries_without_a_handle_and_workspace_sizes():
     assert lib.mp_delta_rule(None, 0, *[None] * 7, 1, 1, 1, 1, 1, 1, 1.0, *[None] * 4, 0, None) == _lib.MP_ERR_INVALID
     assert lib.mp_delta_rule_online(None, 0, *[None] * 7, 1, 1, 1, 1, 1, 1, 1.0, *[None] * 3) == _lib.MP_ERR_INVALID
     assert lib.mp_linear_adapted(None, 0, *[None] * 8, 1, 1, 1, 1, 1, 1, 0, None, None, 0, None) == _lib.MP_ERR_INVALID
-    for f in (lib.mp_delta_rule_workspace, lib.mp_linear_adapted_workspace):
+    for f in (lambda B, T, Hv: lib.mp_delta_rule_workspace(B, T, Hv, 64, 64), lib.mp_linear_adapted_workspace):
         assert f(0, 1, 1) == f(1, 0, 1) == f(1, 1, 0) == 0
         assert 0 < f(1, 1, 1) <= f(2, 1, 1) <= f(2, 33, 1) <= f(2, 33, 3)
         assert f(4096, 65536, 64) > 2 ** 32                # sizes pass 32 bits
