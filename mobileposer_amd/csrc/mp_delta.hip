@@ -563,14 +563,15 @@ MP_KERNEL __launch_bounds__(256, (Arith<E>::P == 1 ? NK <= 4 : NK <= 2) ? 2 : 1)
 
 // The start of every segment: S_{s+1} = M_s S_s + N_s, in place of N_s.  A workgroup per (sequence, value head, 16 columns), a wave
 // per 16 rows (two for dk > 128), on the fp32 matrix instructions; S_s goes round through LDS, M of the next segment is on its way
-// while this one is multiplied.  KT = dk / 16 rounded up.
-template <int KT>
+// while this one is multiplied.  KT = dk / 16 rounded up; VEC: dk is a multiple of 4 (rows of M in 16-byte pieces).
+template <int KT, bool VEC>
 MP_KERNEL __launch_bounds__(512) void mp_delta_join(DeltaArgs a, DeltaPlan plan, int ncol) {
     constexpr int NT = (KT + 7) / 8;
     constexpr bool kAhead = KT <= 8;              // (both would not fit the registers)
     __shared__ float St[16 * KT][17];
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, grp = lane >> 4, wave = tid >> 6;
-    const int ct = blockIdx.x % ncol, head = blockIdx.x / ncol, b = head / a.Hv;
+    const int head = blockIdx.x % (a.B * a.Hv), ct = blockIdx.x / (a.B * a.Hv), b = head / a.Hv;      // (a head's workgroups, which read the same M, on one XCD
+                                                                                                    //  where the heads are a multiple of 8)
     const int cv = 16 * ct + col, cc = min(cv, a.dv - 1);
     // segments behind which another one begins; the first one's N is its end state
     const int n = min(plan.nseg - 1, (length_of(a.lengths, b, a.T) + plan.len * kC - 1) / (plan.len * kC) - 1);
@@ -590,7 +591,8 @@ MP_KERNEL __launch_bounds__(512) void mp_delta_join(DeltaArgs a, DeltaPlan plan,
             for (int k = 0; k < KT; ++k) {
                 const int d = 16 * k + 4 * grp;
                 const float* p = Ms + (size_t)row * a.dk;
-                mn[t][k] = {p[min(d, a.dk - 1)], p[min(d + 1, a.dk - 1)], p[min(d + 2, a.dk - 1)], p[min(d + 3, a.dk - 1)]};
+                if (VEC) mn[t][k] = *(const float4*)(p + (d < a.dk ? d : 0));      // (what is read behind dk meets zeros)
+                else mn[t][k] = {p[min(d, a.dk - 1)], p[min(d + 1, a.dk - 1)], p[min(d + 2, a.dk - 1)], p[min(d + 3, a.dk - 1)]};
             }
 #pragma unroll
             for (int r = 0; r < 4; ++r) an[t][r] = Ns[(size_t)min(16 * (wave + 8 * t) + 4 * grp + r, a.dk - 1) * a.dv + cc];
@@ -635,7 +637,7 @@ MP_KERNEL __launch_bounds__(512) void mp_delta_join(DeltaArgs a, DeltaPlan plan,
 static DeltaPlan plan_of(int B, int T, int Hv, int dk, int dv) {
     DeltaPlan p = {1, (T + kC - 1) / kC, nullptr, nullptr};
     const long per = (long)B * Hv * ((dv + 63) / 64 + (dk + 63) / 64);
-    const int nchunk = p.len, want = (int)min((long)nchunk / 4, 512 / per);
+    const int nchunk = p.len, want = (int)min((long)nchunk / 4, 1024 / per);
     if (want >= 4) {
         p.len = (nchunk + want - 1) / want;
         p.nseg = (nchunk + p.len - 1) / p.len;
@@ -644,7 +646,7 @@ static DeltaPlan plan_of(int B, int T, int Hv, int dk, int dv) {
 }
 static size_t prep_floats(int B, int T, int Hv) { return (size_t)B * Hv * ((T + kC - 1) / kC) * (ws_unit(3) / 4); }
 size_t delta_ws_floats(int B, int T, int Hv, int dk, int dv) {
-    return prep_floats(B, T, Hv) + (size_t)B * Hv * (plan_of(B, T, Hv, dk, dv).nseg - 1) * dk * (dk + dv);
+    return prep_floats(B, T, Hv) + (size_t)B * Hv * (plan_of(B, T, Hv, dk, dv).nseg - 1) * dk * (dk + dv) + 4;
 }
 
 template <class E, int NK, int MODE, bool OUT>
@@ -662,13 +664,19 @@ static bool scan_for(const DeltaArgs& a, hipStream_t s) {
     DeltaPlan p = plan_of(a.B, a.T, a.Hv, a.dk, a.dv);
     if (p.nseg > 1) {
         p.N = a.ws + prep_floats(a.B, a.T, a.Hv);
-        p.M = p.N + (size_t)a.B * a.Hv * (p.nseg - 1) * a.dk * a.dv;
+        p.M = p.N + ((size_t)a.B * a.Hv * (p.nseg - 1) * a.dk * a.dv + 3) / 4 * 4;
         if (!scan_pass<E, NK, MODE, false>(a, p, s)) return false;
         const int ncol = (a.dv + 15) / 16;
         const dim3 grid((unsigned)(a.B * a.Hv * ncol));
-        if (a.dk <= 64) hipLaunchKernelGGL(mp_delta_join<4>, grid, dim3(512), 0, s, a, p, ncol);
-        else if (a.dk <= 128) hipLaunchKernelGGL(mp_delta_join<8>, grid, dim3(512), 0, s, a, p, ncol);
-        else hipLaunchKernelGGL(mp_delta_join<16>, grid, dim3(512), 0, s, a, p, ncol);
+        if (a.dk % 4) {
+            if (a.dk <= 64) hipLaunchKernelGGL((mp_delta_join<4, false>), grid, dim3(512), 0, s, a, p, ncol);
+            else if (a.dk <= 128) hipLaunchKernelGGL((mp_delta_join<8, false>), grid, dim3(512), 0, s, a, p, ncol);
+            else hipLaunchKernelGGL((mp_delta_join<16, false>), grid, dim3(512), 0, s, a, p, ncol);
+        } else {
+            if (a.dk <= 64) hipLaunchKernelGGL((mp_delta_join<4, true>), grid, dim3(512), 0, s, a, p, ncol);
+            else if (a.dk <= 128) hipLaunchKernelGGL((mp_delta_join<8, true>), grid, dim3(512), 0, s, a, p, ncol);
+            else hipLaunchKernelGGL((mp_delta_join<16, true>), grid, dim3(512), 0, s, a, p, ncol);
+        }
     }
     return scan_pass<E, NK, MODE, true>(a, p, s);
 }

@@ -1,7 +1,7 @@
 // Device helpers of the sequence operators: operands of the bf16 matrix instructions from bf16 or fp32 data.
 //
-// An fp32 value as three bf16 terms -- hi the nearest, mid the next eight bits, lo the rest -- keeps all 24 bits, and a product of
-// two such values is six products of terms: the three left out are below 2^-24 of it.  With fp32 accumulation that is the accuracy of
+// An fp32 value as three bf16 terms -- each the nearest to what the ones before it leave -- keeps all 24 bits, and a product of two
+// such values is six products of terms: the three left out are below 2^-26 of it.  With fp32 accumulation that is the accuracy of
 // an fp32 sum at 16 / 6 times the rate of the fp32 matrix instructions; beside a bf16 operand, which is its own only term, it is
 // three products.  (An infinite value gives NaN: inf - inf in the split.)
 #pragma once
@@ -53,20 +53,17 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 static __device__ __forceinline__ unsigned nearest_bf16(float a, float b) {
     return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2){a, b}, bf16x2));
 }
-// the same, and what is left of them (exact).  Halves are rounded away from zero by integer arithmetic and cut: three instructions
-// of full rate a value where v_cvt_pk_bf16_f32 has a quarter of it
+// the same, and what is left of them: x - bf16(x) is exact, and one v_dot2_f32_bf16 of the packed pair with (-1, 0) or (0, -1) does it
+// without unpacking.  (The selectors come from registers: as a constant, 0xbf800000 is taken for the inline operand -1.0, whose
+// halves are not what is meant.)
 static __device__ __forceinline__ unsigned take_bf16(float& a, float& b) {
-    const unsigned x = __float_as_uint(a) + 0x8000u, y = __float_as_uint(b) + 0x8000u;
-    a -= __uint_as_float(x & 0xffff0000u);
-    b -= __uint_as_float(y & 0xffff0000u);
-    return __builtin_amdgcn_perm(y, x, 0x07060302u);
-}
-// the upper eight bits of what is left, cut, and the rest of it (exact)
-static __device__ __forceinline__ unsigned cut_bf16(float& a, float& b) {
-    const unsigned x = __float_as_uint(a), y = __float_as_uint(b);
-    a -= __uint_as_float(x & 0xffff0000u);
-    b -= __uint_as_float(y & 0xffff0000u);
-    return __builtin_amdgcn_perm(y, x, 0x07060302u);
+    unsigned first = 0x0000bf80u, second = 0xbf800000u;
+    asm("" : "+s"(first));
+    asm("" : "+s"(second));
+    const bf16x2 w = __builtin_convertvector((f32x2){a, b}, bf16x2);
+    a = __builtin_amdgcn_fdot2_f32_bf16(w, __builtin_bit_cast(bf16x2, first), a, false);
+    b = __builtin_amdgcn_fdot2_f32_bf16(w, __builtin_bit_cast(bf16x2, second), b, false);
+    return __builtin_bit_cast(unsigned, w);
 }
 template <> struct Oct<float> {
     float v[8];
@@ -98,8 +95,8 @@ template <> struct Oct<float> {
         for (int i = 0; i < 4; ++i) {
             float a = v[2 * i], b = v[2 * i + 1];
             o[0][i] = take_bf16(a, b);
-            o[1][i] = cut_bf16(a, b);
-            o[2][i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+            o[1][i] = take_bf16(a, b);
+            o[2][i] = nearest_bf16(a, b);
         }
     }
 };
