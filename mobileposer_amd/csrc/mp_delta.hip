@@ -65,57 +65,73 @@ static __device__ __forceinline__ void fix_oct(Oct<E>& o, int d, int dk, bool on
     if (!on || d >= dk) o.zero();
 }
 
-// One wave per (sequence, key head, chunk): K K^T and Q K^T once, then the value heads that share the key head, two at a time --
-// a lane of either half solves a column of (I + A) T = I by forward substitution (stable where keys repeat and A is far from
-// small; products of powers of A are not).
-template <class E, int PO, int MODE>
+// One wave per (sequence, key head, chunk): K K^T and Q K^T once, then the value heads that share the key head, two at a time.
+// (I + A)^{-1} by forward substitution on the two 16 x 16 diagonal blocks -- a lane of four groups of 16 solves a column of one
+// block of one head; stable where keys repeat and A is far from small, products of powers of A are not -- and
+// T21 = -T22 A21 T11 on the fp32 matrix instructions.  KB: steps of 32 components whose loads are in flight together.
+template <class E, int PO, int MODE, int KB>
 MP_KERNEL __launch_bounds__(64) void mp_delta_prep(DeltaArgs a) {
     constexpr int P = Arith<E>::P, LS = kC + 4;
-    __shared__ __align__(16) float A[2][kC][LS], W[kC][LS];
+    __shared__ __align__(16) float At[2][kC][LS], Tm[2][kC][LS], betas[2][kC];      // A transposed: [column][row]
+    __shared__ __align__(16) double Gs[2][kC];
+    float (*W)[LS] = Tm[0];                       // P on its way into operand order, before T is there
     const int unit = blockIdx.x, c = unit % a.nchunk, hk = unit / a.nchunk % a.Hk, b = unit / a.nchunk / a.Hk;
     const int lane = threadIdx.x, col = lane & 15, grp = lane >> 4, half = lane >> 5, i = lane & 31, t0 = c * kC;
     const int len = length_of(a.lengths, b, a.T);
     if (t0 >= len) return;
-    const E* q = (const E*)a.q + b * a.sq[0] + hk * a.sq[2];
-    const E* k = (const E*)a.k + b * a.sk[0] + hk * a.sk[2];
-    f32x4 kk[3] = {}, qk[3] = {};                 // tiles (0,0), (1,0), (1,1) of frames 16 I + row, 16 J + column
-    const int tl[2] = {min(t0 + col, len - 1), min(t0 + 16 + col, len - 1)};
-    for (int d0 = 0; d0 < a.dk; d0 += 32) {
-        u32x4 fk[2][P], fq[2][P];
-        Oct<E> ok[2], oq[2];
-        const int d = d0 + 8 * grp;
-#pragma unroll
-        for (int I = 0; I < 2; ++I) {
-            load_oct<E, MODE>(ok[I], k + tl[I] * a.sk[1], d, a.dk);
-            load_oct<E, MODE>(oq[I], q + tl[I] * a.sq[1], d, a.dk);
-        }
-#pragma unroll
-        for (int I = 0; I < 2; ++I) {
-            fix_oct<E, MODE>(ok[I], d, a.dk, t0 + 16 * I + col < len);
-            fix_oct<E, MODE>(oq[I], d, a.dk, t0 + 16 * I + col < len);
-            ok[I].planes(fk[I]);
-            oq[I].planes(fq[I]);
-        }
-#pragma unroll
-        for (int n = 0; n < 3; ++n) {
-            kk[n] = mfma_planes(fk[n > 0], fk[n > 1], kk[n]);
-            qk[n] = mfma_planes(fq[n > 0], fk[n > 1], qk[n]);
-        }
-    }
     const int rep = a.Hv / a.Hk, t = t0 + i;
     const bool on = t < len;
+    const E* q = (const E*)a.q + b * a.sq[0] + hk * a.sq[2];
+    const E* k = (const E*)a.k + b * a.sk[0] + hk * a.sk[2];
+    auto gate = [&](const float* p, const long (&s)[3], int e0) {
+        return p[b * s[0] + min(t, len - 1) * s[1] + (hk * rep + min(e0 + half, rep - 1)) * s[2]];
+    };
+    float gnext = gate(a.g, a.sg, 0), bnext = gate(a.beta, a.sb, 0);
+    f32x4 kk[3] = {}, qk[3] = {};                 // tiles (0,0), (1,0), (1,1) of frames 16 I + row, 16 J + column
+    const int tl[2] = {min(t0 + col, len - 1), min(t0 + 16 + col, len - 1)};
+    for (int d0 = 0; d0 < a.dk; d0 += 32 * KB) {
+        Oct<E> ok[KB][2], oq[KB][2];
+#pragma unroll
+        for (int m = 0; m < KB; ++m)
+#pragma unroll
+            for (int I = 0; I < 2; ++I) {
+                load_oct<E, MODE>(ok[m][I], k + tl[I] * a.sk[1], d0 + 32 * m + 8 * grp, a.dk);
+                load_oct<E, MODE>(oq[m][I], q + tl[I] * a.sq[1], d0 + 32 * m + 8 * grp, a.dk);
+            }
+#pragma unroll
+        for (int m = 0; m < KB; ++m) {
+            u32x4 fk[2][P], fq[2][P];
+            const int d = d0 + 32 * m + 8 * grp;
+#pragma unroll
+            for (int I = 0; I < 2; ++I) {
+                fix_oct<E, MODE>(ok[m][I], d, a.dk, t0 + 16 * I + col < len);
+                fix_oct<E, MODE>(oq[m][I], d, a.dk, t0 + 16 * I + col < len);
+                ok[m][I].planes(fk[I]);
+                oq[m][I].planes(fq[I]);
+            }
+#pragma unroll
+            for (int n = 0; n < 3; ++n) {
+                kk[n] = mfma_planes(fk[n > 0], fk[n > 1], kk[n]);
+                qk[n] = mfma_planes(fq[n > 0], fk[n > 1], qk[n]);
+            }
+        }
+    }
     for (int e0 = 0; e0 < rep; e0 += 2) {
-        const int two = min(2, rep - e0), hh = hk * rep + e0 + min(half, two - 1);
-        const float beta = on ? a.beta[b * a.sb[0] + t * a.sb[1] + hh * a.sb[2]] : 0.f;
-        double G = on ? (double)clamp_g(a.g[b * a.sg[0] + t * a.sg[1] + hh * a.sg[2]]) : 0.0;
+        const int two = min(2, rep - e0);
+        const float beta = on ? bnext : 0.f;
+        double G = on ? (double)clamp_g(gnext) : 0.0;
+        if (e0 + 2 < rep) { gnext = gate(a.g, a.sg, e0 + 2); bnext = gate(a.beta, a.sb, e0 + 2); }
 #pragma unroll
         for (int s = 1; s < kC; s <<= 1) {
             const double up = __shfl_up(G, s, 32);
             if (i >= s) G += up;
         }
         const double last = __shfl(G, kC - 1, 32);
+        __syncthreads();
+        Gs[half][i] = G;
+        betas[half][i] = beta;
         if (half < two) {
-            char* ws = (char*)a.ws + ((size_t)(b * a.Hv + hh) * a.nchunk + c) * ws_unit(PO);
+            char* ws = (char*)a.ws + ((size_t)(b * a.Hv + hk * rep + e0 + half) * a.nchunk + c) * ws_unit(PO);
             ((float*)(ws + kWsEg))[i] = expf((float)G);
             ((float*)(ws + kWsTail))[i] = expf((float)(last - G));
         }
@@ -124,16 +140,19 @@ MP_KERNEL __launch_bounds__(64) void mp_delta_prep(DeltaArgs a) {
             __syncthreads();
 #pragma unroll
             for (int tile = 0; tile < 3; ++tile) {
-                const double Gj = __shfl(G, 32 * e + 16 * (tile > 1) + col);
+                const int I = tile > 0, cj = 16 * (tile > 1) + col;
+                const double Gj = Gs[e][cj];
+                float av[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int ri = 16 * (tile > 0) + 4 * grp + r, cj = 16 * (tile > 1) + col;
-                    const float D = expf((float)(__shfl(G, 32 * e + ri) - Gj));
-                    const float bi = __shfl(beta, 32 * e + ri);
-                    A[e][cj][ri] = cj < ri ? bi * D * kk[tile][r] : 0.f;
+                    const int ri = 16 * I + 4 * grp + r;
+                    const float D = expf((float)(Gs[e][ri] - Gj));
+                    av[r] = cj < ri ? betas[e][ri] * D * kk[tile][r] : 0.f;
                     W[ri][cj] = cj <= ri ? a.scale * D * qk[tile][r] : 0.f;
                 }
+                *(float4*)&At[e][cj][16 * I + 4 * grp] = {av[0], av[1], av[2], av[3]};
             }
+#pragma unroll
             for (int r = 0; r < 4; ++r) W[4 * grp + r][16 + col] = 0.f;
             __syncthreads();
 #pragma unroll
@@ -146,36 +165,56 @@ MP_KERNEL __launch_bounds__(64) void mp_delta_prep(DeltaArgs a) {
                 for (int n = 0; n < PO; ++n) *(u32x4*)(ws + kWsP + (I * PO + n) * kFrag + lane * 16) = p[n];
             }
         }
-        const int mine = min(half, two - 1);
-        float x[kC];
+        __syncthreads();
+        // the diagonal blocks
+        const int e = min(half, two - 1), blk = grp & 1;
+        float x[16];
 #pragma unroll
-        for (int n = 0; n < kC; ++n) x[n] = n == i ? 1.f : 0.f;
-        float4 now[kC / 4], next[kC / 4];         // column n of A, rows n + 1 .. : on its way while column n - 1 is used
+        for (int n = 0; n < 16; ++n) x[n] = n == col ? 1.f : 0.f;
 #pragma unroll
-        for (int m = 0; m < kC / 4; ++m) next[m] = *(const float4*)&A[mine][0][4 * m];
+        for (int n = 0; n < 15; ++n) {
+            float an[16];
 #pragma unroll
-        for (int n = 0; n < kC - 1; ++n) {
-
+            for (int m = (n + 1) / 4; m < 4; ++m) __builtin_memcpy(&an[4 * m], __builtin_assume_aligned(&At[e][16 * blk + n][16 * blk + 4 * m], 16), 16);
+            if (n < col) x[n] = 0.f;              // (not 0 * NaN where an earlier frame's row is not finite)
 #pragma unroll
-            for (int m = n / 4; m < kC / 4; ++m) now[m] = next[m];
-#pragma unroll
-            for (int m = (n + 1) / 4; m < kC / 4; ++m) next[m] = *(const float4*)&A[mine][n + 1][4 * m];
-            if (n < i) x[n] = 0.f;                // (not 0 * NaN where an earlier frame's row is not finite)
-#pragma unroll
-            for (int j = n + 1; j < kC; ++j) x[j] = fmaf(-((const float*)now)[j], x[n], x[j]);
+            for (int j = n + 1; j < 16; ++j) x[j] = fmaf(-an[j], x[n], x[j]);
         }
-        if (kC - 1 < i) x[kC - 1] = 0.f;
-        __syncthreads();
+        if (15 < col) x[15] = 0.f;
 #pragma unroll
-        for (int n = 0; n < kC; ++n) A[half][n][i] = n < i ? 0.f : x[n] * beta;        // (with one head left, the other half's copy is not read)
+        for (int n = 0; n < 16; ++n) {
+            Tm[half][16 * blk + n][16 * blk + col] = x[n];        // (with one head left, the other half's copy is not read)
+            if (blk == 0) Tm[half][n][16 + col] = 0.f;
+        }
         __syncthreads();
-        for (int e = 0; e < two; ++e) {
-            char* ws = (char*)a.ws + ((size_t)(b * a.Hv + hk * rep + e0 + e) * a.nchunk + c) * ws_unit(PO);
+        for (int h = 0; h < two; ++h) {
+            f32x4 X = {0.f, 0.f, 0.f, 0.f}, T21 = {0.f, 0.f, 0.f, 0.f};
+            float4 a21, t11, t22;
+            const int l = 4 * grp;
+            a21 = {At[h][l][16 + col], At[h][l + 1][16 + col], At[h][l + 2][16 + col], At[h][l + 3][16 + col]};
+            t11 = {Tm[h][l][col], Tm[h][l + 1][col], Tm[h][l + 2][col], Tm[h][l + 3][col]};
+            t22 = *(const float4*)&Tm[h][16 + col][16 + l];
+            X = mfma4(a21, t11, X);
+            float4 y;                                             // (a later frame's row that is not finite is kept from the zeros of T22)
+            y.x = not_finite(X[0]) ? 0.f : X[0];
+            y.y = not_finite(X[1]) ? 0.f : X[1];
+            y.z = not_finite(X[2]) ? 0.f : X[2];
+            y.w = not_finite(X[3]) ? 0.f : X[3];
+            T21 = mfma4(t22, y, T21);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) Tm[h][16 + l + r][col] = -T21[r];
+        }
+        __syncthreads();
+        for (int h = 0; h < two; ++h) {
+            char* ws = (char*)a.ws + ((size_t)(b * a.Hv + hk * rep + e0 + h) * a.nchunk + c) * ws_unit(PO);
 #pragma unroll
             for (int I = 0; I < 2; ++I) {
                 Oct<float> o;
                 u32x4 p[3];
-                o.load(&A[e][row_index(I, col)][8 * grp]);
+                const int row = row_index(I, col);
+                o.load(&Tm[h][row][8 * grp]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) o.v[j] = 8 * grp + j > row ? 0.f : o.v[j] * betas[h][8 * grp + j];
                 o.planes(p);
 #pragma unroll
                 for (int n = 0; n < 3; ++n) *(u32x4*)(ws + kWsT + (I * 3 + n) * kFrag + lane * 16) = p[n];
@@ -682,7 +721,11 @@ static bool scan_for(const DeltaArgs& a, hipStream_t s) {
 }
 template <class E, int PO, int MODE>
 static bool launch_mode(const DeltaArgs& a, hipStream_t s) {
-    if (a.nchunk) hipLaunchKernelGGL((mp_delta_prep<E, PO, MODE>), dim3((unsigned)(a.B * a.Hk * a.nchunk)), dim3(64), 0, s, a);
+    if (a.nchunk) {
+        const dim3 grid((unsigned)(a.B * a.Hk * a.nchunk));
+        if (Arith<E>::P == 1 && a.dk > 64) hipLaunchKernelGGL((mp_delta_prep<E, PO, MODE, 4>), grid, dim3(64), 0, s, a);
+        else hipLaunchKernelGGL((mp_delta_prep<E, PO, MODE, 2>), grid, dim3(64), 0, s, a);
+    }
     if (MODE == 2) return scan_for<E, 1, MODE>(a, s);
     constexpr int M = MODE == 2 ? 1 : MODE;
     const int nk = (a.dk + 31) / 32;
