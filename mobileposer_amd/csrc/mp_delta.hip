@@ -65,32 +65,36 @@ static __device__ __forceinline__ void fix_oct(Oct<E>& o, int d, int dk, bool on
     if (!on || d >= dk) o.zero();
 }
 
-// One wave per (sequence, key head, chunk): K K^T and Q K^T once, then the value heads that share the key head, two at a time.
-// (I + A)^{-1} by forward substitution on the two 16 x 16 diagonal blocks -- a lane of four groups of 16 solves a column of one
-// block of one head; stable where keys repeat and A is far from small, products of powers of A are not -- and
-// T21 = -T22 A21 T11 on the fp32 matrix instructions.  KB: steps of 32 components whose loads are in flight together.
+// e^x of a difference of 64-bit prefix sums: the product with log2(e) in 64 bits, one rounding, the hardware's 2^x (1 ulp)
+static __device__ __forceinline__ float decay(double x) { return __builtin_amdgcn_exp2f((float)(x * 1.4426950408889634)); }
+// x of the lane `n` below within 16 lanes (0 where there is none); CTRL 0x142: of the last lane of the 16 before, in every second 16
+template <int CTRL>
+static __device__ __forceinline__ double lane_below(double x) {
+    const long long v = __builtin_bit_cast(long long, x);
+    constexpr int rows = CTRL == 0x142 ? 0xa : 0xf;
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)v, CTRL, rows, 0xf, true), hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, rows, 0xf, true);
+    return __builtin_bit_cast(double, (long long)(unsigned)lo | (long long)hi << 32);
+}
+
+// One wave per (sequence, key head, chunk): K K^T and Q K^T once, then the value heads that share the key head.
+// (I + A)^{-1} by forward substitution on the two 16 x 16 diagonal blocks -- a lane of two groups of 16 solves a column; stable
+// where keys repeat and A is far from small, products of powers of A are not -- and T21 = -T22 A21 T11 on the fp32 matrix
+// instructions.  KB: steps of 32 components whose loads are in flight together.
 template <class E, int PO, int MODE, int KB>
 MP_KERNEL __launch_bounds__(64) void mp_delta_prep(DeltaArgs a) {
     constexpr int P = Arith<E>::P, LS = kC + 4;
-    __shared__ __align__(16) float At[2][kC][LS], Tm[2][kC][LS], betas[2][kC];      // A transposed: [column][row]
-    __shared__ __align__(16) double Gs[2][kC];
-    float (*W)[LS] = Tm[0];                       // P on its way into operand order, before T is there
+    __shared__ __align__(16) float At[kC][LS], Tm[kC][LS], betas[kC];      // A transposed: [column][row]
+    __shared__ __align__(16) double Gs[kC];
+    float (*W)[LS] = Tm;                          // P on its way into operand order, before T is there
     const int unit = blockIdx.x, c = unit % a.nchunk, hk = unit / a.nchunk % a.Hk, b = unit / a.nchunk / a.Hk;
-    const int lane = threadIdx.x, col = lane & 15, grp = lane >> 4, half = lane >> 5, i = lane & 31, t0 = c * kC;
-    const int len = length_of(a.lengths, b, a.T);
-    if (t0 >= len) return;
+    const int lane = threadIdx.x, col = lane & 15, grp = lane >> 4, i = lane & 31, t0 = c * kC;
     const int rep = a.Hv / a.Hk, t = t0 + i;
-    const bool on = t < len;
     const E* q = (const E*)a.q + b * a.sq[0] + hk * a.sq[2];
     const E* k = (const E*)a.k + b * a.sk[0] + hk * a.sk[2];
-    auto gate = [&](const float* p, const long (&s)[3], int e0) {
-        return p[b * s[0] + min(t, len - 1) * s[1] + (hk * rep + min(e0 + half, rep - 1)) * s[2]];
-    };
-    float gnext = gate(a.g, a.sg, 0), bnext = gate(a.beta, a.sb, 0);
-    f32x4 kk[3] = {}, qk[3] = {};                 // tiles (0,0), (1,0), (1,1) of frames 16 I + row, 16 J + column
-    const int tl[2] = {min(t0 + col, len - 1), min(t0 + 16 + col, len - 1)};
-    for (int d0 = 0; d0 < a.dk; d0 += 32 * KB) {
-        Oct<E> ok[KB][2], oq[KB][2];
+    // (everything is requested at once: rows behind the sequence's end are read as far as the tensor goes, and dropped)
+    const int tl[2] = {min(t0 + col, a.T - 1), min(t0 + 16 + col, a.T - 1)};
+    Oct<E> ok[KB][2], oq[KB][2];
+    auto request = [&](int d0) {
 #pragma unroll
         for (int m = 0; m < KB; ++m)
 #pragma unroll
@@ -98,6 +102,16 @@ MP_KERNEL __launch_bounds__(64) void mp_delta_prep(DeltaArgs a) {
                 load_oct<E, MODE>(ok[m][I], k + tl[I] * a.sk[1], d0 + 32 * m + 8 * grp, a.dk);
                 load_oct<E, MODE>(oq[m][I], q + tl[I] * a.sq[1], d0 + 32 * m + 8 * grp, a.dk);
             }
+    };
+    request(0);
+    auto gate = [&](const float* p, const long (&s)[3], int e) { return p[b * s[0] + min(t, a.T - 1) * s[1] + (hk * rep + e) * s[2]]; };
+    float gnext = gate(a.g, a.sg, 0), bnext = gate(a.beta, a.sb, 0);
+    const int len = length_of(a.lengths, b, a.T);
+    if (t0 >= len) return;
+    const bool on = t < len;
+    f32x4 kk[3] = {}, qk[3] = {};                 // tiles (0,0), (1,0), (1,1) of frames 16 I + row, 16 J + column
+    for (int d0 = 0; d0 < a.dk; d0 += 32 * KB) {
+        if (d0) request(d0);
 #pragma unroll
         for (int m = 0; m < KB; ++m) {
             u32x4 fk[2][P], fq[2][P];
@@ -116,58 +130,62 @@ MP_KERNEL __launch_bounds__(64) void mp_delta_prep(DeltaArgs a) {
             }
         }
     }
-    for (int e0 = 0; e0 < rep; e0 += 2) {
-        const int two = min(2, rep - e0);
+    char* ws = (char*)a.ws + ((size_t)(b * a.Hv + hk * rep) * a.nchunk + c) * ws_unit(PO);
+    for (int e = 0; e < rep; ++e, ws += (size_t)a.nchunk * ws_unit(PO)) {
         const float beta = on ? bnext : 0.f;
-        double G = on ? (double)clamp_g(gnext) : 0.0;
-        if (e0 + 2 < rep) { gnext = gate(a.g, a.sg, e0 + 2); bnext = gate(a.beta, a.sb, e0 + 2); }
-#pragma unroll
-        for (int s = 1; s < kC; s <<= 1) {
-            const double up = __shfl_up(G, s, 32);
-            if (i >= s) G += up;
-        }
-        const double last = __shfl(G, kC - 1, 32);
+        double G = on ? (double)clamp_g(gnext) : 0.0;             // lanes 32.. as lanes 0..31
+        if (e + 1 < rep) { gnext = gate(a.g, a.sg, e + 1); bnext = gate(a.beta, a.sb, e + 1); }
+        G += lane_below<0x111>(G);
+        G += lane_below<0x112>(G);
+        G += lane_below<0x114>(G);
+        G += lane_below<0x118>(G);
+        G += lane_below<0x142>(G);
+        const long long top = __builtin_bit_cast(long long, G);
+        const double last = __builtin_bit_cast(double, (long long)(unsigned)__builtin_amdgcn_readlane((int)top, 31) |
+                                                       (long long)__builtin_amdgcn_readlane((int)(top >> 32), 31) << 32);
         __syncthreads();
-        Gs[half][i] = G;
-        betas[half][i] = beta;
-        if (half < two) {
-            char* ws = (char*)a.ws + ((size_t)(b * a.Hv + hk * rep + e0 + half) * a.nchunk + c) * ws_unit(PO);
-            ((float*)(ws + kWsEg))[i] = expf((float)G);
-            ((float*)(ws + kWsTail))[i] = expf((float)(last - G));
-        }
-        for (int e = 0; e < two; ++e) {
-            char* ws = (char*)a.ws + ((size_t)(b * a.Hv + hk * rep + e0 + e) * a.nchunk + c) * ws_unit(PO);
-            __syncthreads();
-#pragma unroll
-            for (int tile = 0; tile < 3; ++tile) {
-                const int I = tile > 0, cj = 16 * (tile > 1) + col;
-                const double Gj = Gs[e][cj];
-                float av[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int ri = 16 * I + 4 * grp + r;
-                    const float D = expf((float)(Gs[e][ri] - Gj));
-                    av[r] = cj < ri ? betas[e][ri] * D * kk[tile][r] : 0.f;
-                    W[ri][cj] = cj <= ri ? a.scale * D * qk[tile][r] : 0.f;
-                }
-                *(float4*)&At[e][cj][16 * I + 4 * grp] = {av[0], av[1], av[2], av[3]};
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) W[4 * grp + r][16 + col] = 0.f;
-            __syncthreads();
-#pragma unroll
-            for (int I = 0; I < 2; ++I) {
-                Oct<float> o;
-                u32x4 p[3];
-                o.load(&W[row_index(I, col)][8 * grp]);
-                o.planes(p);
-#pragma unroll
-                for (int n = 0; n < PO; ++n) *(u32x4*)(ws + kWsP + (I * PO + n) * kFrag + lane * 16) = p[n];
-            }
+        if (lane < kC) {
+            Gs[i] = G;
+            betas[i] = beta;
+            ((float*)(ws + kWsEg))[i] = decay(G);
+            ((float*)(ws + kWsTail))[i] = decay(last - G);
         }
         __syncthreads();
-        // the diagonal blocks
-        const int e = min(half, two - 1), blk = grp & 1;
+        double Gr[2][4];
+        float br[2][4];
+#pragma unroll
+        for (int I = 0; I < 2; ++I) {
+            __builtin_memcpy(Gr[I], __builtin_assume_aligned(&Gs[16 * I + 4 * grp], 16), 32);
+            __builtin_memcpy(br[I], __builtin_assume_aligned(&betas[16 * I + 4 * grp], 16), 16);
+        }
+        const double Gc[2] = {Gs[col], Gs[16 + col]};
+#pragma unroll
+        for (int tile = 0; tile < 3; ++tile) {
+            const int I = tile > 0, J = tile > 1, cj = 16 * J + col;
+            float av[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int ri = 16 * I + 4 * grp + r;
+                const float D = decay(Gr[I][r] - Gc[J]);
+                av[r] = cj < ri ? br[I][r] * D * kk[tile][r] : 0.f;
+                W[ri][cj] = cj <= ri ? a.scale * D * qk[tile][r] : 0.f;
+            }
+            *(float4*)&At[cj][16 * I + 4 * grp] = {av[0], av[1], av[2], av[3]};
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) W[4 * grp + r][16 + col] = 0.f;
+        __syncthreads();
+#pragma unroll
+        for (int I = 0; I < 2; ++I) {
+            Oct<float> o;
+            u32x4 p[3];
+            o.load(&W[row_index(I, col)][8 * grp]);
+            o.planes(p);
+#pragma unroll
+            for (int n = 0; n < PO; ++n) *(u32x4*)(ws + kWsP + (I * PO + n) * kFrag + lane * 16) = p[n];
+        }
+        // the diagonal blocks (groups 2 and 3 as 0 and 1)
+        const int blk = grp & 1;
         float x[16];
 #pragma unroll
         for (int n = 0; n < 16; ++n) x[n] = n == col ? 1.f : 0.f;
@@ -175,25 +193,25 @@ MP_KERNEL __launch_bounds__(64) void mp_delta_prep(DeltaArgs a) {
         for (int n = 0; n < 15; ++n) {
             float an[16];
 #pragma unroll
-            for (int m = (n + 1) / 4; m < 4; ++m) __builtin_memcpy(&an[4 * m], __builtin_assume_aligned(&At[e][16 * blk + n][16 * blk + 4 * m], 16), 16);
+            for (int m = (n + 1) / 4; m < 4; ++m) __builtin_memcpy(&an[4 * m], __builtin_assume_aligned(&At[16 * blk + n][16 * blk + 4 * m], 16), 16);
             if (n < col) x[n] = 0.f;              // (not 0 * NaN where an earlier frame's row is not finite)
 #pragma unroll
             for (int j = n + 1; j < 16; ++j) x[j] = fmaf(-an[j], x[n], x[j]);
         }
         if (15 < col) x[15] = 0.f;
+        __syncthreads();
 #pragma unroll
         for (int n = 0; n < 16; ++n) {
-            Tm[half][16 * blk + n][16 * blk + col] = x[n];        // (with one head left, the other half's copy is not read)
-            if (blk == 0) Tm[half][n][16 + col] = 0.f;
+            Tm[16 * blk + n][16 * blk + col] = x[n];
+            if (blk == 0) Tm[n][16 + col] = 0.f;
         }
         __syncthreads();
-        for (int h = 0; h < two; ++h) {
+        {
             f32x4 X = {0.f, 0.f, 0.f, 0.f}, T21 = {0.f, 0.f, 0.f, 0.f};
-            float4 a21, t11, t22;
             const int l = 4 * grp;
-            a21 = {At[h][l][16 + col], At[h][l + 1][16 + col], At[h][l + 2][16 + col], At[h][l + 3][16 + col]};
-            t11 = {Tm[h][l][col], Tm[h][l + 1][col], Tm[h][l + 2][col], Tm[h][l + 3][col]};
-            t22 = *(const float4*)&Tm[h][16 + col][16 + l];
+            const float4 a21 = {At[l][16 + col], At[l + 1][16 + col], At[l + 2][16 + col], At[l + 3][16 + col]};
+            const float4 t11 = {Tm[l][col], Tm[l + 1][col], Tm[l + 2][col], Tm[l + 3][col]};
+            const float4 t22 = *(const float4*)&Tm[16 + col][16 + l];
             X = mfma4(a21, t11, X);
             float4 y;                                             // (a later frame's row that is not finite is kept from the zeros of T22)
             y.x = not_finite(X[0]) ? 0.f : X[0];
@@ -202,23 +220,22 @@ MP_KERNEL __launch_bounds__(64) void mp_delta_prep(DeltaArgs a) {
             y.w = not_finite(X[3]) ? 0.f : X[3];
             T21 = mfma4(t22, y, T21);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) Tm[h][16 + l + r][col] = -T21[r];
+            for (int r = 0; r < 4; ++r) Tm[16 + l + r][col] = -T21[r];
         }
         __syncthreads();
-        for (int h = 0; h < two; ++h) {
-            char* ws = (char*)a.ws + ((size_t)(b * a.Hv + hk * rep + e0 + h) * a.nchunk + c) * ws_unit(PO);
+        float bc[8];
+        __builtin_memcpy(bc, __builtin_assume_aligned(&betas[8 * grp], 16), 32);
 #pragma unroll
-            for (int I = 0; I < 2; ++I) {
-                Oct<float> o;
-                u32x4 p[3];
-                const int row = row_index(I, col);
-                o.load(&Tm[h][row][8 * grp]);
+        for (int I = 0; I < 2; ++I) {
+            Oct<float> o;
+            u32x4 p[3];
+            const int row = row_index(I, col);
+            o.load(&Tm[row][8 * grp]);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) o.v[j] = 8 * grp + j > row ? 0.f : o.v[j] * betas[h][8 * grp + j];
-                o.planes(p);
+            for (int j = 0; j < 8; ++j) o.v[j] = 8 * grp + j > row ? 0.f : o.v[j] * bc[j];
+            o.planes(p);
 #pragma unroll
-                for (int n = 0; n < 3; ++n) *(u32x4*)(ws + kWsT + (I * 3 + n) * kFrag + lane * 16) = p[n];
-            }
+            for (int n = 0; n < 3; ++n) *(u32x4*)(ws + kWsT + (I * 3 + n) * kFrag + lane * 16) = p[n];
         }
     }
 }
