@@ -51,7 +51,7 @@ static __device__ __forceinline__ bool not_finite(float x) { return !(fabsf(x) <
 
 // Components d .. d + 7 of a row of q or k, without a branch around the load (a branch would make the loads wait for each other):
 // the address is moved inside the row, fix() puts zeros where the row or the sequence has ended.  MODE 0: dk is a multiple of 8;
-// 1: it is not, but at least 8 -- the last eight components are loaded and shifted down; 2: dk < 8, component by component.
+// 1: it is not, but at least 8 -- the last eight components are loaded and shifted down; 2: dk < 8 or dv < 8, value by value.
 template <class E, int MODE>
 static __device__ __forceinline__ void load_oct(Oct<E>& o, const E* row, int d, int dk) {
     if (MODE == 0) o.load(row + (d < dk ? d : 0));
@@ -271,14 +271,14 @@ struct Rows {                                     // what a thread stages of a c
             oq[n] = (unsigned)(t * (int)a.sq[1] + at) * sizeof(E);
         }
         const int col = c0 + 8 * (threadIdx.x & 7);
-        ov = (unsigned)(min((int)threadIdx.x >> 3, last_row) * (int)a.sv[1] + (a.dv < 8 ? 0 : min(col, a.dv - 8))) * sizeof(E);
+        ov = (unsigned)(min((int)threadIdx.x >> 3, last_row) * (int)a.sv[1] + (MODE == 2 ? 0 : min(col, a.dv - 8))) * sizeof(E);
     }
     __device__ __forceinline__ void load(const DeltaArgs& a, const char* kb, const char* qb, const char* vb, const char* wp, int c0) {
         const int tid = threadIdx.x, wave = tid >> 6;
 #pragma unroll
         for (int n = 0; n < NW; ++n) ws[n] = *(const u32x4*)(wp + (unsigned)min(4096 * n + 16 * tid, kUnit - 16));
-        if (a.dv >= 8) v.load((const E*)(vb + ov));
-        else v.load_clamped((const E*)(vb + ov), c0 + 8 * (tid & 7), a.dv);
+        if (MODE == 2) v.load_clamped((const E*)(vb + ov), c0 + 8 * (tid & 7), a.dv);
+        else v.load((const E*)(vb + ov));
 #pragma unroll
         for (int n = 0; n < NF; ++n) {
             if (MODE == 2) {
@@ -298,7 +298,7 @@ struct Rows {                                     // what a thread stages of a c
         for (int n = 0; n < NW; ++n)
             if (4096 * n + 16 * tid < kUnit) *(u32x4*)(lds + L::kWs + 4096 * n + 16 * tid) = ws[n];
         const int col = c0 + 8 * (tid & 7);
-        if (a.dv % 8 && a.dv >= 8) v.shift(col - min(col, a.dv - 8));
+        if (MODE != 2 && a.dv % 8) v.shift(col - min(col, a.dv - 8));
         if (t0 + (tid >> 3) >= len) v.zero();
         __builtin_memcpy(__builtin_assume_aligned(lds + L::kV + (tid >> 3) * L::kRowV + 8 * (tid & 7) * sizeof(E), 16), &v.v, sizeof(v.v));
 #pragma unroll
@@ -579,7 +579,9 @@ MP_KERNEL __launch_bounds__(256, (Arith<E>::P == 1 ? NK <= 4 : NK <= 2) ? 2 : 1)
         __syncthreads();
         Oct<E> out;
         if (OUT) __builtin_memcpy(&out.v, __builtin_assume_aligned(oplace, 16), sizeof(out.v));
-        if (c + 1 < nc) rows.store(a, lds, t0 + kC, len, c0);
+        // (the last chunk as well, its own rows again: loads that may stay unused would have to be waited for at the loop's top, behind
+        //  the stores of the outputs)
+        rows.store(a, lds, t0 + kC, len, c0);
         __syncthreads();
         if (OUT && t0 + (tid >> 3) < len) {
             E* at = o + (size_t)t0 * so;
@@ -693,7 +695,7 @@ MP_KERNEL __launch_bounds__(512) void mp_delta_join(DeltaArgs a, DeltaPlan plan,
 static DeltaPlan plan_of(int B, int T, int Hv, int dk, int dv) {
     DeltaPlan p = {1, (T + kC - 1) / kC, nullptr, nullptr};
     const long per = (long)B * Hv * ((dv + 63) / 64 + (dk + 63) / 64);
-    const int nchunk = p.len, want = (int)min((long)nchunk / 4, 1024 / per);
+    const int nchunk = p.len, want = (int)min((long)nchunk / 4, 512 / per);
     if (want >= 4) {
         p.len = (nchunk + want - 1) / want;
         p.nseg = (nchunk + p.len - 1) / p.len;
@@ -743,7 +745,7 @@ static bool launch_mode(const DeltaArgs& a, hipStream_t s) {
         if (Arith<E>::P == 1 && a.dk > 64) hipLaunchKernelGGL((mp_delta_prep<E, PO, MODE, 4>), grid, dim3(64), 0, s, a);
         else hipLaunchKernelGGL((mp_delta_prep<E, PO, MODE, 2>), grid, dim3(64), 0, s, a);
     }
-    if (MODE == 2) return scan_for<E, 1, MODE>(a, s);
+    if (MODE == 2) return scan_for<E, 8, MODE>(a, s);
     constexpr int M = MODE == 2 ? 1 : MODE;
     const int nk = (a.dk + 31) / 32;
     return nk == 1 ? scan_for<E, 1, M>(a, s) : nk == 2 ? scan_for<E, 2, M>(a, s) : nk == 3 ? scan_for<E, 3, M>(a, s) : nk == 4 ? scan_for<E, 4, M>(a, s)
@@ -751,7 +753,7 @@ static bool launch_mode(const DeltaArgs& a, hipStream_t s) {
 }
 template <class E, int PO>
 static bool launch_for(const DeltaArgs& a, hipStream_t s) {
-    const bool ok = a.dk % 8 == 0 ? launch_mode<E, PO, 0>(a, s) : a.dk >= 8 ? launch_mode<E, PO, 1>(a, s) : launch_mode<E, PO, 2>(a, s);
+    const bool ok = a.dk < 8 || a.dv < 8 ? launch_mode<E, PO, 2>(a, s) : a.dk % 8 ? launch_mode<E, PO, 1>(a, s) : launch_mode<E, PO, 0>(a, s);
     return hipGetLastError() == hipSuccess && ok;
 }
 bool launch_delta(const DeltaArgs& a, int dtype, hipStream_t s) {
