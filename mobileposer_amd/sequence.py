@@ -13,13 +13,13 @@ from . import _lib
 
 _DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 _INT_MAX = 2 ** 31 - 1
+_stream_of = torch._C._cuda_getCurrentRawStream       # the current stream's handle (torch.cuda.current_stream builds an object around it: 2 us)
 
 
 def _no_grad(*tensors):
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise RuntimeError("the sequence operators have no backward pass: call them under torch.no_grad() or detach their inputs")
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("the sequence operators have no backward pass: call them under torch.no_grad() or detach their inputs")
 
 
 def _rows(t):
@@ -28,35 +28,34 @@ def _rows(t):
 
 
 class SequenceOps:
-    """Methods of ``MobilePoserNet`` (they use its native handle and device)."""
+    """Methods of ``MobilePoserNet`` (they use its native handle and device).  A tick's call is host time first: the checks read
+    each property once."""
 
-    def _dtype(self, what, *tensors):
+    def _dtype(self, what, first, *more):
         """The common type of the tensors, as the library numbers it; all of them on this model's device."""
-        first = tensors[0].dtype
-        if first not in _DTYPES:
-            raise RuntimeError("%s takes float32 or bfloat16 tensors, got %s" % (what, first))
-        for t in tensors:
-            if t.dtype != first:
-                raise RuntimeError("%s: tensors of one type expected, got %s and %s" % (what, first, t.dtype))
-            if t.device != self.device:
-                self._same_device(what, t)
-        return _DTYPES[first]
-
-    def _same_device(self, what, t):
-        if t.device.type != "cuda" or t.device.index != self._device_index:
-            raise RuntimeError("%s: a tensor on %s, the model is on %s" % (what, t.device, self.device))
+        dtype, index = first.dtype, self._device_index
+        if dtype not in _DTYPES:
+            raise RuntimeError("%s takes float32 or bfloat16 tensors, got %s" % (what, dtype))
+        if first.get_device() != index:
+            raise RuntimeError("%s: a tensor on %s, the model is on %s" % (what, first.device, self.device))
+        for t in more:
+            if t.dtype is not dtype:
+                raise RuntimeError("%s: tensors of one type expected, got %s and %s" % (what, dtype, t.dtype))
+            if t.get_device() != index:
+                raise RuntimeError("%s: a tensor on %s, the model is on %s" % (what, t.device, self.device))
+        return _DTYPES[dtype]
 
     def _indices(self, what, value, n, lo, hi):
         """[n] int32 on the device.  A host sequence is checked against lo..hi; a device tensor is taken as it is (the kernels
         hold its values to the range: nothing waits for the device here)."""
         if torch.is_tensor(value) and value.is_cuda:
-            if tuple(value.shape) != (n,) or value.dtype not in (torch.int32, torch.int64):
+            if value.shape != (n,) or value.dtype not in (torch.int32, torch.int64):
                 raise RuntimeError("%s: expected [%d] int32, got %s %s" % (what, n, tuple(value.shape), value.dtype))
-            if value.device != self.device:
-                self._same_device(what, value)
-            if value.dtype == torch.int64:
+            if value.get_device() != self._device_index:
+                raise RuntimeError("%s: a tensor on %s, the model is on %s" % (what, value.device, self.device))
+            if value.dtype is torch.int64:
                 value = value.clamp(-1, _INT_MAX).to(torch.int32)
-            return value if value.stride(0) == 1 or n == 1 else value.contiguous()
+            return value.contiguous()
         ints = [int(i) for i in value]
         if len(ints) != n:
             raise RuntimeError("%s: %d values for %d sequences" % (what, len(ints), n))
@@ -65,14 +64,16 @@ class SequenceOps:
         return torch.tensor(ints, dtype=torch.int32, device="cuda:%d" % self._device_index)
 
     def _heads(self, what, q, k, v, g, beta, lead):
-        if q.dim() != lead + 2 or k.shape != q.shape or v.dim() != lead + 2 or v.shape[:lead] != q.shape[:lead]:
-            raise RuntimeError("%s: q, k [.., Hk, dk] and v [.., Hv, dv] expected, got %s, %s, %s" % (what, tuple(q.shape), tuple(k.shape), tuple(v.shape)))
-        Hk, dk, Hv, dv = q.shape[-2], q.shape[-1], v.shape[-2], v.shape[-1]
+        qs, vs = q.shape, v.shape
+        if len(qs) != lead + 2 or len(vs) != lead + 2 or k.shape != qs or vs[:lead] != qs[:lead]:
+            raise RuntimeError("%s: q, k [.., Hk, dk] and v [.., Hv, dv] expected, got %s, %s, %s" % (what, tuple(qs), tuple(k.shape), tuple(vs)))
+        Hk, dk, Hv, dv = qs[lead], qs[lead + 1], vs[lead], vs[lead + 1]
         if Hk < 1 or Hv < 1 or Hv % Hk or not 1 <= dk <= 256 or dv < 1:
             raise RuntimeError("%s: %d value heads over %d key heads, head sizes %d / %d (Hv a multiple of Hk, dk at most 256)" % (what, Hv, Hk, dk, dv))
-        if g.shape != v.shape[:-1] or beta.shape != v.shape[:-1]:
-            raise RuntimeError("%s: g and beta %s expected, got %s and %s" % (what, tuple(v.shape[:-1]), tuple(g.shape), tuple(beta.shape)))
-        if g.dtype != torch.float32 or beta.dtype != torch.float32:
+        gate = vs[:lead + 1]
+        if g.shape != gate or beta.shape != gate:
+            raise RuntimeError("%s: g and beta %s expected, got %s and %s" % (what, tuple(gate), tuple(g.shape), tuple(beta.shape)))
+        if g.dtype is not torch.float32 or beta.dtype is not torch.float32:
             raise RuntimeError("%s: g and beta are float32, got %s and %s" % (what, g.dtype, beta.dtype))
         return Hk, dk, Hv, dv
 
@@ -106,7 +107,7 @@ class SequenceOps:
         self._check(self._lib.mp_delta_rule(
             self._h, dtype, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), C.addressof(st),
             0 if lens is None else lens.data_ptr(), B, T, Hk, Hv, dk, dv, dk ** -0.5 if scale is None else float(scale), o.data_ptr(),
-            0 if state is None else state.data_ptr(), out.data_ptr(), ws.data_ptr(), need, torch.cuda.current_stream(dev).cuda_stream))
+            0 if state is None else state.data_ptr(), out.data_ptr(), ws.data_ptr(), need, _stream_of(self._device_index)))
         return o, out
 
     def delta_rule_online(self, q, k, v, g, beta, state, slots=None, scale=None):
@@ -134,7 +135,7 @@ class SequenceOps:
         self._check(self._lib.mp_delta_rule_online(
             self._h, dtype, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), C.addressof(st),
             0 if slots is None else slots.data_ptr(), S, n, Hk, Hv, dk, dv, dk ** -0.5 if scale is None else float(scale), o.data_ptr(),
-            state.data_ptr(), torch.cuda.current_stream(q.device).cuda_stream))
+            state.data_ptr(), _stream_of(self._device_index)))
         return o
 
     def linear_adapted(self, x, weight, bias, down, up, scale, ids, relu=False):
@@ -169,5 +170,5 @@ class SequenceOps:
         self._check(self._lib.mp_linear_adapted(
             self._h, dtype, x.data_ptr(), C.addressof(st), weight.data_ptr(), 0 if bias is None else bias.data_ptr(), down.data_ptr(),
             up.data_ptr(), 0 if scale is None else scale.data_ptr(), ids.data_ptr(), B, T, K, M, n, r, int(bool(relu)), y.data_ptr(),
-            ws.data_ptr(), need, torch.cuda.current_stream(x.device).cuda_stream))
+            ws.data_ptr(), need, _stream_of(self._device_index)))
         return y

@@ -14,7 +14,7 @@ class NotReached:
 
 class Ops(SequenceOps):
     def __init__(self):
-        self.device, self._device_index, self._lib = torch.device("cpu"), 0, NotReached()
+        self.device, self._device_index, self._lib = torch.device("cpu"), -1, NotReached()
 
     def _require_weights(self):
         pass
