@@ -1,11 +1,10 @@
 // A linear layer over the rows of many sequences with a low-rank adapter per sequence beside the shared weight:
 //   y_n = act(W x_n + b + scale_a Up_a (Down_a x_n)),   a = ids[sequence of n]   (negative: the shared layer alone).
-// Two launches: z = scale Down x for all rows (mp_adapt_down, fp32 into the workspace), then the shared product with Up z joined
-// to it in its registers before the one rounding and the one store (mp_adapt_gemm).  Up to three operands of a product decide the arithmetic:
-// bf16 inputs go to the bf16 matrix instructions as they are; fp32 inputs as three bf16 terms each (hi + mid + lo, each the nearest
-// to what is left: all 24 bits), six products per fp32 product -- the three left out are below 2^-26 of it --, fp32 accumulation:
-// the accuracy of an fp32 sum at 16 / 6 times the rate of the fp32 matrix instructions.  (An infinite fp32 input gives NaN:
-// inf - inf in the split.)
+// Wide layers take two launches: z = scale Down x for all rows (mp_adapt_down, fp32 into the workspace), then the shared product with
+// Up z joined to it in its registers before the one rounding and the one store (mp_adapt_gemm).  Where a layer's columns and
+// the adapter's components fit one tile side by side (an output layer) and the sequences are long, Down's rows ride in the shared
+// product as further columns and x is read once (mp_adapt_gemm<.., FUSED>).
+// bf16 inputs go to the bf16 matrix instructions as they are, fp32 inputs as three bf16 terms each (mp_seq_dev.h).
 #include "mp_seq_dev.h"
 
 namespace mpseq {
@@ -14,77 +13,108 @@ size_t adapt_ws_floats(int B, int T, int r) { return (size_t)B * T * r; }
 
 // ---------------------------------------------------------------- z = scale Down x
 // A workgroup takes up to 16 frames of one sequence -- one adapter, so the product runs on the matrix units even where the 16 rows
-// are one (a tick: the reads of Down bound it either way) --, K split over the four waves and joined through LDS.
-template <class E>
+// are one (a tick: the reads of Down bound it either way) --, K split over the four waves and joined through LDS; KB steps of
+// every wave are in flight together.  RT = r / 16 rounded up.
+template <class E, int RT>
 MP_KERNEL __launch_bounds__(256) void mp_adapt_down(AdaptArgs a, int per_seq) {
-    constexpr int P = Arith<E>::P;
-    __shared__ float part[4][16][17];
+    constexpr int P = Arith<E>::P, KB = RT >= 4 ? 2 : 4;
+    __shared__ float part[4][16 * RT][17];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, grp = lane >> 4;
     const int b = blockIdx.x / per_seq, t0 = blockIdx.x % per_seq * 16, id = a.ids[b];
     if (id < 0 || id >= a.n) return;                              // (the second launch reads no z of such rows)
     const int t = t0 + col < a.T ? t0 + col : a.T - 1;
     const E* x = (const E*)a.x + (size_t)b * a.sx[0] + (size_t)t * a.sx[1];
+    const E* d[RT];
+#pragma unroll
+    for (int j = 0; j < RT; ++j) d[j] = (const E*)a.down + ((size_t)id * a.r + min(16 * j + col, a.r - 1)) * a.K;
+    f32x4 acc[RT] = {};
+    int k = (wave * 4 + grp) * 8;
+    for (; k - grp * 8 + 128 * (KB - 1) + 32 <= a.K; k += 128 * KB) {
+        Oct<E> ox[KB], od[KB][RT];
+#pragma unroll
+        for (int m = 0; m < KB; ++m) {
+            ox[m].load(x + k + 128 * m);
+#pragma unroll
+            for (int j = 0; j < RT; ++j) od[m][j].load(d[j] + k + 128 * m);
+        }
+#pragma unroll
+        for (int m = 0; m < KB; ++m) {
+            u32x4 px[P], pd[RT][P];
+            ox[m].planes(px);
+#pragma unroll
+            for (int j = 0; j < RT; ++j) od[m][j].planes(pd[j]);
+            mfma_planes_n<RT, P, P>(pd, px, acc);
+        }
+    }
+    for (; k - grp * 8 < a.K; k += 128) {
+        const int left = a.K - k < 0 ? 0 : a.K - k;
+        Oct<E> ox, od;
+        u32x4 px[P], pd[RT][P];
+        ox.load_some(x + k, left);
+        ox.planes(px);
+#pragma unroll
+        for (int j = 0; j < RT; ++j) {
+            od.load_some(d[j] + k, left);
+            od.planes(pd[j]);
+        }
+        mfma_planes_n<RT, P, P>(pd, px, acc);
+    }
+#pragma unroll
+    for (int j = 0; j < RT; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) part[wave][16 * j + 4 * grp + r][col] = acc[j][r];      // [component][row]
+    __syncthreads();
     const float sc = a.scale ? a.scale[id] : 1.f;
-    for (int j0 = 0; j0 < a.r; j0 += 16) {
-        const int j = j0 + col < a.r ? j0 + col : a.r - 1;
-        const E* d = (const E*)a.down + ((size_t)id * a.r + j) * a.K;
-        f32x4 acc = {};
-        int k = (wave * 4 + grp) * 8;
-#pragma unroll 2
-        for (; k - grp * 8 + 32 <= a.K; k += 128) {
-            Oct<E> ox, od;
-            u32x4 px[P], pd[P];
-            ox.load(x + k); od.load(d + k);
-            ox.planes(px); od.planes(pd);
-            acc = mfma_planes(pd, px, acc);
-        }
-        if (k - grp * 8 < a.K) {
-            const int left = a.K - k < 0 ? 0 : a.K - k;
-            Oct<E> ox, od;
-            u32x4 px[P], pd[P];
-            ox.load_some(x + k, left); od.load_some(d + k, left);
-            ox.planes(px); od.planes(pd);
-            acc = mfma_planes(pd, px, acc);
-        }
-        for (int r = 0; r < 4; ++r) part[wave][4 * grp + r][col] = acc[r];      // [component][row]
-        __syncthreads();
-        const int row = tid >> 4, c = tid & 15;
-        if (t0 + row < a.T && j0 + c < a.r)
-            a.ws[((size_t)b * a.T + t0 + row) * a.r + j0 + c] = sc * ((part[0][c][row] + part[1][c][row]) + (part[2][c][row] + part[3][c][row]));
-        __syncthreads();
+    for (int i = tid; i < 16 * a.r; i += 256) {
+        const int row = i / a.r, c = i % a.r;
+        if (t0 + row < a.T) a.ws[((size_t)b * a.T + t0 + row) * a.r + c] = sc * ((part[0][c][row] + part[1][c][row]) + (part[2][c][row] + part[3][c][row]));
     }
 }
 
 // ---------------------------------------------------------------- the shared product, the adapters' second half joined to it
-// A workgroup's tile is (32 MR rows of x) x (32 MC columns of y); four waves, 2 x 2, each MR x MC tiles of 16 x 16 with W as the A
-// operand (so that a lane ends with four consecutive columns of one row).  Tiles of K go through registers into LDS, rows padded by
-// 16 bytes (a 16-lane read of one K group covers every bank once); the next tile's loads are in flight while this one is
-// multiplied.
-template <class E, int MR, int MC>
-MP_KERNEL __launch_bounds__(256) void mp_adapt_gemm(AdaptArgs a, int rows, int ntr, int ntc) {
-    constexpr int P = Arith<E>::P, BK = P == 1 ? 64 : 32, UR = BK / 8, RN = 32 * MR, CM = 32 * MC, LS = BK + 8;
-    constexpr int NU = (RN + CM) * UR / 256;                      // units of eight elements that a thread stages
-    static_assert((RN + CM) * UR % 256 == 0, "whole units per thread");
-    __shared__ __align__(16) bf16raw lds[P][RN + CM][LS];
+// A workgroup's tile is RN rows of x times CM columns of y; WR x WC waves, each MR x MC tiles of 16 x 16 with W as the A operand (so
+// that a lane ends with four consecutive columns of one row).  Tiles of BK along K go through registers into LDS, rows padded by 16
+// bytes (a 16-lane read of one K group covers every bank once); the next tile's loads are in flight while this one is
+// multiplied.  BK is as long as the staging registers allow: a small tile is a chain of memory latencies.  FUSED: a row
+// tile lies inside one sequence, columns Mp .. Mp + r - 1 of the tile (Mp = M rounded up to 16) are that sequence's Down.
+template <class E, int WR, int WC, int MR, int MC, int BK, bool TWO, bool FUSED>
+struct Gemm {
+    static constexpr int P = Arith<E>::P, UR = BK / 8, RN = 16 * MR * WR, CM = 16 * MC * WC, LS = BK + 8, TH = 64 * WR * WC;
+    static constexpr int NU = (RN + CM) * UR / TH;                // units of eight elements that a thread stages
+    static constexpr int kPlane = (RN + CM) * LS * 2, kOne = P * kPlane, kZ = TWO ? 2 * kOne : kOne, kRowZ = 128 + 4;
+    static constexpr int kBytes = FUSED ? (kZ > RN * kRowZ * 4 ? kZ : RN * kRowZ * 4) : kZ;      // (z takes the operands' place)
+    static_assert((RN + CM) * UR % TH == 0 && kBytes <= 160 * 1024, "whole units per thread, LDS of a CU");
+};
+template <class E, int WR, int WC, int MR, int MC, int BK, bool TWO, bool FUSED>
+MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_gemm(AdaptArgs a, int rows, int ntr, int ntc) {
+    using G = Gemm<E, WR, WC, MR, MC, BK, TWO, FUSED>;
+    constexpr int P = G::P, UR = G::UR, RN = G::RN, LS = G::LS, NU = G::NU, TH = G::TH;
+    extern __shared__ __align__(16) char gemm_lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, grp = lane >> 4;
     // workgroups are dealt to the 8 XCDs in turn: a run of tiles (columns fastest: one panel of x) to each, so that an XCD's L2
     // holds what its tiles share
     const int nt = ntr * ntc, per = (nt + 7) / 8, tile = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
     if (tile >= nt || (int)(blockIdx.x / 8) >= per) return;
-    const int n0 = tile / ntc * RN, m0 = tile % ntc * CM;
+    // rows [n0, n1) of the flattened (sequence, frame) list; FUSED: tiles of a sequence
+    const int tps = FUSED ? (a.T + RN - 1) / RN : 1, seq = FUSED ? tile / tps : 0;
+    const int n0 = FUSED ? seq * a.T + tile % tps * RN : tile / ntc * RN, n1 = FUSED ? (seq + 1) * a.T : rows;
+    const int m0 = FUSED ? 0 : tile % ntc * G::CM, Mp = (a.M + 15) / 16 * 16;
+    const int sid = FUSED ? a.ids[seq] : 0;
+    const bool adapt = FUSED && sid >= 0 && sid < a.n;
     const E* src[NU];
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
-        const int row = (tid + 256 * u) / UR, kk = (tid + 256 * u) % UR * 8;
+        const int row = (tid + TH * u) / UR, kk = (tid + TH * u) % UR * 8;
         if (row < RN) {
-            const int n = n0 + row < rows ? n0 + row : rows - 1, b = n / a.T;
+            const int n = min(n0 + row, n1 - 1), b = n / a.T;
             src[u] = (const E*)a.x + (size_t)b * a.sx[0] + (size_t)(n - b * a.T) * a.sx[1] + kk;
         } else {
-            const int m = m0 + row - RN < a.M ? m0 + row - RN : a.M - 1;
-            src[u] = (const E*)a.w + (size_t)m * a.K + kk;
+            const int m = m0 + row - RN;
+            src[u] = (const E*)a.w + (size_t)min(m, a.M - 1) * a.K + kk;
+            if (FUSED && adapt && m >= Mp) src[u] = (const E*)a.down + ((size_t)sid * a.r + min(m - Mp, a.r - 1)) * a.K + kk;
         }
     }
-    const int wr = wave & 1, wc = wave >> 1;
+    const int wr = wave % WR, wc = wave / WR;
     f32x4 acc[MC][MR] = {};
     Oct<E> oct[NU];
     auto fetch = [&](int k0) {
@@ -93,51 +123,74 @@ MP_KERNEL __launch_bounds__(256) void mp_adapt_gemm(AdaptArgs a, int rows, int n
             for (int u = 0; u < NU; ++u) oct[u].load(src[u] + k0);
         } else {
 #pragma unroll
-            for (int u = 0; u < NU; ++u) oct[u].load_guarded(src[u] + k0, a.K - k0 - (tid + 256 * u) % UR * 8);
+            for (int u = 0; u < NU; ++u) oct[u].load_some(src[u] + k0, a.K - k0 - (tid + TH * u) % UR * 8);
         }
     };
-    fetch(0);
-    for (int k0 = 0; k0 < a.K; k0 += BK) {
-        __syncthreads();
+    auto stage = [&](char* to) {
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
-            const int row = (tid + 256 * u) / UR, kk = (tid + 256 * u) % UR * 8;
+            const int row = (tid + TH * u) / UR, kk = (tid + TH * u) % UR * 8;
             u32x4 p[P];
             oct[u].planes(p);
 #pragma unroll
-            for (int i = 0; i < P; ++i) *(u32x4*)&lds[i][row][kk] = p[i];
+            for (int i = 0; i < P; ++i) *(u32x4*)(to + i * G::kPlane + (row * LS + kk) * 2) = p[i];
         }
-        __syncthreads();
-        if (k0 + BK < a.K) fetch(k0 + BK);
+    };
+    fetch(0);
+    stage(gemm_lds);
+    __syncthreads();
+    int turn = 0;
+    for (int k0 = 0; k0 < a.K; k0 += BK, turn ^= TWO) {
+        const bool more = k0 + BK < a.K;
+        if (more) fetch(k0 + BK);
+        const char* from = gemm_lds + (TWO ? turn * G::kOne : 0);
 #pragma unroll
         for (int ks = 0; ks < BK; ks += 32) {
             u32x4 fx[MR][P];
 #pragma unroll
             for (int i = 0; i < MR; ++i)
 #pragma unroll
-                for (int p = 0; p < P; ++p) fx[i][p] = *(const u32x4*)&lds[p][(wr * MR + i) * 16 + col][ks + 8 * grp];
+                for (int p = 0; p < P; ++p) fx[i][p] = *(const u32x4*)(from + p * G::kPlane + (((wr * MR + i) * 16 + col) * LS + ks + 8 * grp) * 2);
 #pragma unroll
             for (int j = 0; j < MC; ++j) {
                 u32x4 fw[P];
 #pragma unroll
-                for (int p = 0; p < P; ++p) fw[p] = *(const u32x4*)&lds[p][RN + (wc * MC + j) * 16 + col][ks + 8 * grp];
+                for (int p = 0; p < P; ++p) fw[p] = *(const u32x4*)(from + p * G::kPlane + ((RN + (wc * MC + j) * 16 + col) * LS + ks + 8 * grp) * 2);
 #pragma unroll
                 for (int i = 0; i < MR; ++i) acc[j][i] = mfma_planes(fw, fx[i], acc[j][i]);
             }
         }
+        if (!TWO) __syncthreads();
+        if (more) stage(gemm_lds + (TWO ? (turn ^ 1) * G::kOne : 0));
+        __syncthreads();
+    }
+    const int rlen = a.r;
+    float* zl = (float*)gemm_lds;                                 // FUSED: [RN][kRowZ]
+    if (FUSED && adapt) {
+        const float sc = a.scale ? a.scale[sid] : 1.f;
+#pragma unroll
+        for (int j = 0; j < MC; ++j) {
+            const int m = (wc * MC + j) * 16 - Mp + 4 * grp;
+            if (m >= 0)
+#pragma unroll
+                for (int i = 0; i < MR; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (m + r < rlen) zl[((wr * MR + i) * 16 + col) * G::kRowZ + m + r] = sc * acc[j][i][r];
+        }
+        __syncthreads();
     }
 #pragma unroll
     for (int i = 0; i < MR; ++i) {
-        const int nb = n0 + (wr * MR + i) * 16;                   // 16 rows, one per lane column
-        const int n = nb + col, nc = n < rows ? n : rows - 1;
-        const int id = a.ids[nc / a.T];
+        const int n = n0 + (wr * MR + i) * 16 + col, nc = min(n, n1 - 1);      // 16 rows, one per lane column
+        const int id = FUSED ? sid : a.ids[nc / a.T];
         const bool use = id >= 0 && id < a.n;
-        const float* z = a.ws + (size_t)nc * a.r;
+        const float* z = FUSED ? zl + ((wr * MR + i) * 16 + col) * G::kRowZ : a.ws + (size_t)nc * rlen;
         const int id0 = __builtin_amdgcn_readfirstlane(id);
-        if (__all(id == id0)) {
+        if (FUSED ? adapt : __all(id == id0)) {
             if (id0 >= 0 && id0 < a.n)                            // one adapter for the 16 rows: the matrix units again
-                for (int r0 = 0; r0 < a.r; r0 += 32) {
-                    const int k = r0 + 8 * grp, left = a.r - k < 0 ? 0 : a.r - k;
+                for (int r0 = 0; r0 < rlen; r0 += 32) {
+                    const int k = r0 + 8 * grp, left = rlen - k < 0 ? 0 : rlen - k;
                     Oct<float> oz;
                     u32x4 p3[3], pz[P == 1 ? 2 : 3];              // z keeps 16 of its bits beside bf16 operands, all 24 beside fp32 ones
                     oz.load_some(z + k, left);
@@ -149,27 +202,27 @@ MP_KERNEL __launch_bounds__(256) void mp_adapt_gemm(AdaptArgs a, int rows, int n
                         const int m = m0 + (wc * MC + j) * 16 + col;
                         Oct<E> ou;
                         u32x4 pu[P];
-                        ou.load_some((const E*)a.up + ((size_t)id0 * a.M + (m < a.M ? m : 0)) * a.r + k, left);
+                        ou.load_some((const E*)a.up + ((size_t)id0 * a.M + (m < a.M ? m : 0)) * rlen + k, left);
                         ou.planes(pu);
                         acc[j][i] = mfma_planes(pu, pz, acc[j][i]);
                     }
                 }
-        } else if (use) {                                         // a row of its own each: dot products of the lane's four columns
-            for (int q = 0; q < a.r; q += 8) {
+        } else if (!FUSED && use) {                               // a row of its own each: dot products of the lane's four columns
+            for (int q = 0; q < rlen; q += 8) {
                 Oct<float> oz;
-                oz.load_some(z + q, a.r - q);
+                oz.load_some(z + q, rlen - q);
 #pragma unroll
                 for (int j = 0; j < MC; ++j)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const int m = m0 + (wc * MC + j) * 16 + 4 * grp + r;
                         Oct<E> ou;
-                        ou.load_some((const E*)a.up + ((size_t)id * a.M + (m < a.M ? m : 0)) * a.r + q, a.r - q);
+                        ou.load_some((const E*)a.up + ((size_t)id * a.M + (m < a.M ? m : 0)) * rlen + q, rlen - q);
                         acc[j][i][r] = ou.dot(oz, acc[j][i][r]);
                     }
             }
         }
-        if (n >= rows) continue;
+        if (n >= n1) continue;
 #pragma unroll
         for (int j = 0; j < MC; ++j) {
             const int m = m0 + (wc * MC + j) * 16 + 4 * grp;
@@ -192,21 +245,36 @@ MP_KERNEL __launch_bounds__(256) void mp_adapt_gemm(AdaptArgs a, int rows, int n
     }
 }
 
-template <class E, int MR, int MC>
-static void gemm_for(const AdaptArgs& a, int rows, hipStream_t s) {
-    const int ntr = (rows + 32 * MR - 1) / (32 * MR), ntc = (a.M + 32 * MC - 1) / (32 * MC);
-    hipLaunchKernelGGL((mp_adapt_gemm<E, MR, MC>), dim3((unsigned)((ntr * ntc + 7) / 8 * 8)), dim3(256), 0, s, a, rows, ntr, ntc);
+template <class E, int WR, int WC, int MR, int MC, int BK, bool TWO, bool FUSED = false>
+static bool gemm_for(const AdaptArgs& a, int rows, hipStream_t s) {
+    using G = Gemm<E, WR, WC, MR, MC, BK, TWO, FUSED>;
+    const auto kernel = mp_adapt_gemm<E, WR, WC, MR, MC, BK, TWO, FUSED>;
+    // (an attribute of the function on the current device: set at every launch, a call may come from any device's handle)
+    if (G::kBytes > 64 * 1024 && hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, G::kBytes) != hipSuccess) return false;
+    const int ntr = FUSED ? a.B * ((a.T + G::RN - 1) / G::RN) : (rows + G::RN - 1) / G::RN, ntc = FUSED ? 1 : (a.M + G::CM - 1) / G::CM;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((ntr * ntc + 7) / 8 * 8)), dim3(G::TH), G::kBytes, s, a, rows, ntr, ntc);
+    return true;
 }
 template <class E>
 static bool launch_for(AdaptArgs a, hipStream_t s) {
-    const int rows = a.B * a.T;
+    constexpr bool half = Arith<E>::P == 1;
+    const int rows = a.B * a.T, per_seq = (a.T + 15) / 16;
     a.vec = a.M % 4 == 0 && (uintptr_t)a.y % (4 * sizeof(E)) == 0;
-    hipLaunchKernelGGL(mp_adapt_down<E>, dim3((unsigned)(a.B * ((a.T + 15) / 16))), dim3(256), 0, s, a, (a.T + 15) / 16);
+    bool ok;
+    if ((a.M + 15) / 16 * 16 + a.r <= 128 && a.T >= 64) {
+        ok = gemm_for<E, 4, 2, 2, 4, half ? 64 : 32, true, true>(a, rows, s);
+        return hipGetLastError() == hipSuccess && ok;
+    }
+    const dim3 grid((unsigned)(a.B * per_seq));
+    if (a.r <= 16) hipLaunchKernelGGL((mp_adapt_down<E, 1>), grid, dim3(256), 0, s, a, per_seq);
+    else if (a.r <= 32) hipLaunchKernelGGL((mp_adapt_down<E, 2>), grid, dim3(256), 0, s, a, per_seq);
+    else if (a.r <= 64) hipLaunchKernelGGL((mp_adapt_down<E, 4>), grid, dim3(256), 0, s, a, per_seq);
+    else hipLaunchKernelGGL((mp_adapt_down<E, 8>), grid, dim3(256), 0, s, a, per_seq);
     auto tiles = [&](int t) { return ((long)rows + t - 1) / t * ((a.M + t - 1) / t); };
-    if (tiles(128) >= 192) gemm_for<E, 4, 4>(a, rows, s);
-    else if (tiles(64) >= 192) gemm_for<E, 2, 2>(a, rows, s);
-    else gemm_for<E, 1, 1>(a, rows, s);
-    return hipGetLastError() == hipSuccess;
+    if (tiles(128) >= 192) ok = half ? gemm_for<E, 2, 2, 4, 4, half ? 64 : 32, false>(a, rows, s) : gemm_for<E, 4, 2, 2, 4, half ? 64 : 32, true>(a, rows, s);
+    else if (tiles(64) >= 192) ok = gemm_for<E, 2, 2, 2, 2, half ? 128 : 64, false>(a, rows, s);
+    else ok = gemm_for<E, 2, 2, 1, 1, half ? 256 : 128, false>(a, rows, s);
+    return hipGetLastError() == hipSuccess && ok;
 }
 bool launch_adapt(const AdaptArgs& a, int dtype, hipStream_t s) {
     return dtype == kBF16 ? launch_for<bf16raw>(a, s) : launch_for<float>(a, s);
