@@ -7,6 +7,8 @@
 // bf16 inputs go to the bf16 matrix instructions as they are, fp32 inputs as three bf16 terms each (mp_seq_dev.h).
 #include "mp_seq_dev.h"
 
+#include <utility>
+
 namespace mpseq {
 
 size_t adapt_ws_floats(int B, int T, int r) { return (size_t)B * T * r; }
@@ -117,15 +119,6 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
     const int wr = wave % WR, wc = wave / WR;
     f32x4 acc[MC][MR] = {};
     Oct<E> oct[NU];
-    auto fetch = [&](int k0) {
-        if (k0 + BK <= a.K) {
-#pragma unroll
-            for (int u = 0; u < NU; ++u) oct[u].load(src[u] + k0);
-        } else {
-#pragma unroll
-            for (int u = 0; u < NU; ++u) oct[u].load_some(src[u] + k0, a.K - k0 - (tid + TH * u) % UR * 8);
-        }
-    };
     auto stage = [&](char* to) {
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
@@ -136,14 +129,7 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
             for (int i = 0; i < P; ++i) *(u32x4*)(to + i * G::kPlane + (row * LS + kk) * 2) = p[i];
         }
     };
-    fetch(0);
-    stage(gemm_lds);
-    __syncthreads();
-    int turn = 0;
-    for (int k0 = 0; k0 < a.K; k0 += BK, turn ^= TWO) {
-        const bool more = k0 + BK < a.K;
-        if (more) fetch(k0 + BK);
-        const char* from = gemm_lds + (TWO ? turn * G::kOne : 0);
+    auto multiply = [&](const char* from) {
 #pragma unroll
         for (int ks = 0; ks < BK; ks += 32) {
             u32x4 fx[MR][P];
@@ -160,9 +146,34 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
                 for (int i = 0; i < MR; ++i) acc[j][i] = mfma_planes(fw, fx[i], acc[j][i]);
             }
         }
-        if (!TWO) __syncthreads();
-        if (more) stage(gemm_lds + (TWO ? (turn ^ 1) * G::kOne : 0));
+    };
+    // whole tiles, each asking for the next one (the last for itself again: no branch around the loads, which would make them wait
+    // for each other), then what is left of K
+    const int whole = a.K / BK;
+    auto fetch = [&](int t) {
+#pragma unroll
+        for (int u = 0; u < NU; ++u) oct[u].load(src[u] + (size_t)t * BK);
+    };
+    char* const other = gemm_lds + (TWO ? G::kOne : 0);
+    if (whole) {
+        fetch(0);
+        stage(gemm_lds);
         __syncthreads();
+    }
+    for (int t = 0; t < whole; ++t) {
+        fetch(min(t + 1, whole - 1));
+        multiply(t & 1 ? other : gemm_lds);
+        if (!TWO) __syncthreads();
+        stage(t & 1 ? gemm_lds : other);
+        __syncthreads();
+    }
+    if (whole * BK < a.K) {
+#pragma unroll
+        for (int u = 0; u < NU; ++u) oct[u].load_some(src[u] + (size_t)whole * BK, a.K - whole * BK - (tid + TH * u) % UR * 8);
+        stage(gemm_lds);                                          // (nobody reads either buffer here: a barrier ended the last round)
+        __syncthreads();
+        multiply(gemm_lds);
+        if (FUSED) __syncthreads();
     }
     const int rlen = a.r;
     float* zl = (float*)gemm_lds;                                 // FUSED: [RN][kRowZ]
@@ -180,8 +191,9 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
         }
         __syncthreads();
     }
-#pragma unroll
-    for (int i = 0; i < MR; ++i) {
+    // one 16-row tile of the wave (a function of a constant: acc stays in registers whatever the compiler thinks of unrolling this)
+    auto finish = [&](auto tile_row) {
+        constexpr int i = decltype(tile_row)::value;
         const int n = n0 + (wr * MR + i) * 16 + col, nc = min(n, n1 - 1);      // 16 rows, one per lane column
         const int id = FUSED ? sid : a.ids[nc / a.T];
         const bool use = id >= 0 && id < a.n;
@@ -222,7 +234,7 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
                     }
             }
         }
-        if (n >= n1) continue;
+        if (n >= n1) return;
 #pragma unroll
         for (int j = 0; j < MC; ++j) {
             const int m = m0 + (wc * MC + j) * 16 + 4 * grp;
@@ -242,7 +254,8 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
                     if (m + r < a.M) store_f(out + r, y[r]);
             }
         }
-    }
+    };
+    [&]<int... I>(std::integer_sequence<int, I...>) { (finish(std::integral_constant<int, I>{}), ...); }(std::make_integer_sequence<int, MR>{});
 }
 
 template <class E, int WR, int WC, int MR, int MC, int BK, bool TWO, bool FUSED = false>
@@ -271,6 +284,11 @@ static bool launch_for(AdaptArgs a, hipStream_t s) {
     else if (a.r <= 64) hipLaunchKernelGGL((mp_adapt_down<E, 4>), grid, dim3(256), 0, s, a, per_seq);
     else hipLaunchKernelGGL((mp_adapt_down<E, 8>), grid, dim3(256), 0, s, a, per_seq);
     auto tiles = [&](int t) { return ((long)rows + t - 1) / t * ((a.M + t - 1) / t); };
+    if constexpr (half)
+        if (tiles(256) >= 192) {
+            ok = gemm_for<E, 2, 4, 8, 4, 64, true>(a, rows, s);
+            return hipGetLastError() == hipSuccess && ok;
+        }
     if (tiles(128) >= 192) ok = half ? gemm_for<E, 2, 2, 4, 4, half ? 64 : 32, false>(a, rows, s) : gemm_for<E, 4, 2, 2, 4, half ? 64 : 32, true>(a, rows, s);
     else if (tiles(64) >= 192) ok = gemm_for<E, 2, 2, 2, 2, half ? 128 : 64, false>(a, rows, s);
     else ok = gemm_for<E, 2, 2, 1, 1, half ? 256 : 128, false>(a, rows, s);
