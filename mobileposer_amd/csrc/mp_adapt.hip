@@ -75,22 +75,25 @@ MP_KERNEL __launch_bounds__(256) void mp_adapt_down(AdaptArgs a, int per_seq) {
 
 // ---------------------------------------------------------------- the shared product, the adapters' second half joined to it
 // A workgroup's tile is RN rows of x times CM columns of y; WR x WC waves, each MR x MC tiles of 16 x 16 with W as the A operand (so
-// that a lane ends with four consecutive columns of one row).  Tiles of BK along K go through registers into LDS, rows padded by 16
-// bytes (a 16-lane read of one K group covers every bank once); the next tile's loads are in flight while this one is
-// multiplied.  BK is as long as the staging registers allow: a small tile is a chain of memory latencies.  FUSED: a row
+// that a lane ends with four consecutive columns of one row).  Tiles of BK along K go through registers into LDS -- consecutive lanes
+// load consecutive pieces of a row: a wave's loads are whole cache lines, which is what bounds it otherwise -- as blocks of 16
+// rows x 32 in operand order, the 16-byte pieces of a block exchanged by block_piece() so that neither side meets a bank more
+// than twice; the next tile's loads are in flight while this one is multiplied.  BK is as long as the staging registers allow: a small tile is a chain of memory latencies.  FUSED: a row
 // tile lies inside one sequence, columns Mp .. Mp + r - 1 of the tile (Mp = M rounded up to 16) are that sequence's Down.
 template <class E, int WR, int WC, int MR, int MC, int BK, bool TWO, bool FUSED>
 struct Gemm {
-    static constexpr int P = Arith<E>::P, UR = BK / 8, RN = 16 * MR * WR, CM = 16 * MC * WC, LS = BK + 8, TH = 64 * WR * WC;
-    static constexpr int NU = (RN + CM) * UR / TH;                // units of eight elements that a thread stages
-    static constexpr int kPlane = (RN + CM) * LS * 2, kOne = P * kPlane, kZ = TWO ? 2 * kOne : kOne, kRowZ = 128 + 4;
+    static constexpr int P = Arith<E>::P, KS = BK / 32, RN = 16 * MR * WR, CM = 16 * MC * WC, TH = 64 * WR * WC;
+    static constexpr int UR = BK / 8, NB = (RN + CM) / 16 * KS, NU = (RN + CM) * UR / TH;      // blocks of a tile; pieces that a thread stages
+    static constexpr int kPlane = NB * 1024, kOne = P * kPlane, kZ = TWO ? 2 * kOne : kOne, kRowZ = 128 + 4;
     static constexpr int kBytes = FUSED ? (kZ > RN * kRowZ * 4 ? kZ : RN * kRowZ * 4) : kZ;      // (z takes the operands' place)
-    static_assert((RN + CM) * UR % TH == 0 && kBytes <= 160 * 1024, "whole units per thread, LDS of a CU");
+    static_assert((RN + CM) * UR % TH == 0 && kBytes <= 160 * 1024, "whole pieces per thread, LDS of a CU");
 };
+// where the piece (row % 16, group of eight elements 0..3) of a block lies
+static __device__ __forceinline__ int block_piece(int row, int g) { return g * 16 + (row ^ (g & 1) * 2 ^ (g >> 1) * 12); }
 template <class E, int WR, int WC, int MR, int MC, int BK, bool TWO, bool FUSED>
 MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_gemm(AdaptArgs a, int rows, int ntr, int ntc) {
     using G = Gemm<E, WR, WC, MR, MC, BK, TWO, FUSED>;
-    constexpr int P = G::P, UR = G::UR, RN = G::RN, LS = G::LS, NU = G::NU, TH = G::TH;
+    constexpr int P = G::P, KS = G::KS, UR = G::UR, RN = G::RN, NU = G::NU, TH = G::TH;
     extern __shared__ __align__(16) char gemm_lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, grp = lane >> 4;
     // workgroups are dealt to the 8 XCDs in turn: a run of tiles (columns fastest: one panel of x) to each, so that an XCD's L2
@@ -119,29 +122,35 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
     const int wr = wave % WR, wc = wave / WR;
     f32x4 acc[MC][MR] = {};
     Oct<E> oct[NU];
+    int at[NU];
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+        const int row = (tid + TH * u) / UR, o = (tid + TH * u) % UR;
+        at[u] = (row / 16 * KS + o / 4) * 1024 + block_piece(row % 16, o % 4) * 16;
+    }
+    const int mine = block_piece(col, grp) * 16;
     auto stage = [&](char* to) {
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
-            const int row = (tid + TH * u) / UR, kk = (tid + TH * u) % UR * 8;
             u32x4 p[P];
             oct[u].planes(p);
 #pragma unroll
-            for (int i = 0; i < P; ++i) *(u32x4*)(to + i * G::kPlane + (row * LS + kk) * 2) = p[i];
+            for (int i = 0; i < P; ++i) *(u32x4*)(to + i * G::kPlane + at[u]) = p[i];
         }
     };
     auto multiply = [&](const char* from) {
 #pragma unroll
-        for (int ks = 0; ks < BK; ks += 32) {
+        for (int ks = 0; ks < KS; ++ks) {
             u32x4 fx[MR][P];
 #pragma unroll
             for (int i = 0; i < MR; ++i)
 #pragma unroll
-                for (int p = 0; p < P; ++p) fx[i][p] = *(const u32x4*)(from + p * G::kPlane + (((wr * MR + i) * 16 + col) * LS + ks + 8 * grp) * 2);
+                for (int p = 0; p < P; ++p) fx[i][p] = *(const u32x4*)(from + p * G::kPlane + ((wr * MR + i) * KS + ks) * 1024 + mine);
 #pragma unroll
             for (int j = 0; j < MC; ++j) {
                 u32x4 fw[P];
 #pragma unroll
-                for (int p = 0; p < P; ++p) fw[p] = *(const u32x4*)(from + p * G::kPlane + ((RN + (wc * MC + j) * 16 + col) * LS + ks + 8 * grp) * 2);
+                for (int p = 0; p < P; ++p) fw[p] = *(const u32x4*)(from + p * G::kPlane + ((RN / 16 + wc * MC + j) * KS + ks) * 1024 + mine);
 #pragma unroll
                 for (int i = 0; i < MR; ++i) acc[j][i] = mfma_planes(fw, fx[i], acc[j][i]);
             }
