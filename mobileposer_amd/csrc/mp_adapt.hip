@@ -78,8 +78,10 @@ MP_KERNEL __launch_bounds__(256) void mp_adapt_down(AdaptArgs a, int per_seq) {
 // that a lane ends with four consecutive columns of one row).  Tiles of BK along K go through registers into LDS -- consecutive lanes
 // load consecutive pieces of a row: a wave's loads are whole cache lines, which is what bounds it otherwise -- as blocks of 16
 // rows x 32 in operand order, the 16-byte pieces of a block exchanged by block_piece() so that neither side meets a bank more
-// than twice; the next tile's loads are in flight while this one is multiplied.  BK is as long as the staging registers allow: a small tile is a chain of memory latencies.  FUSED: a row
-// tile lies inside one sequence, columns Mp .. Mp + r - 1 of the tile (Mp = M rounded up to 16) are that sequence's Down.
+// than twice.  (Any order of K serves that all operands share: an fp32 piece is two runs of four, half a tile apart, so that a
+// load of 16 bytes a lane has no gaps between the lanes either.)  The next tile's loads are in flight while this one is
+// multiplied.  BK is as long as the staging registers allow: a small tile is a chain of memory latencies.  FUSED: a row tile lies
+// inside one sequence, columns Mp .. Mp + r - 1 of the tile (Mp = M rounded up to 16) are that sequence's Down.
 template <class E, int WR, int WC, int MR, int MC, int BK, bool TWO, bool FUSED>
 struct Gemm {
     static constexpr int P = Arith<E>::P, KS = BK / 32, RN = 16 * MR * WR, CM = 16 * MC * WC, TH = 64 * WR * WC;
@@ -88,12 +90,14 @@ struct Gemm {
     static constexpr int kBytes = FUSED ? (kZ > RN * kRowZ * 4 ? kZ : RN * kRowZ * 4) : kZ;      // (z takes the operands' place)
     static_assert((RN + CM) * UR % TH == 0 && kBytes <= 160 * 1024, "whole pieces per thread, LDS of a CU");
 };
+template <class F, int... I>
+static __device__ __forceinline__ void each_of(F& f, std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }
 // where the piece (row % 16, group of eight elements 0..3) of a block lies
 static __device__ __forceinline__ int block_piece(int row, int g) { return g * 16 + (row ^ (g & 1) * 2 ^ (g >> 1) * 12); }
 template <class E, int WR, int WC, int MR, int MC, int BK, bool TWO, bool FUSED>
 MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_gemm(AdaptArgs a, int rows, int ntr, int ntc) {
     using G = Gemm<E, WR, WC, MR, MC, BK, TWO, FUSED>;
-    constexpr int P = G::P, KS = G::KS, UR = G::UR, RN = G::RN, NU = G::NU, TH = G::TH;
+    constexpr int P = G::P, KS = G::KS, UR = G::UR, RN = G::RN, NU = G::NU, TH = G::TH, RUN = P == 1 ? 8 : 4;
     extern __shared__ __align__(16) char gemm_lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, grp = lane >> 4;
     // workgroups are dealt to the 8 XCDs in turn: a run of tiles (columns fastest: one panel of x) to each, so that an XCD's L2
@@ -109,7 +113,7 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
     const E* src[NU];
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
-        const int row = (tid + TH * u) / UR, kk = (tid + TH * u) % UR * 8;
+        const int row = (tid + TH * u) / UR, kk = (tid + TH * u) % UR * RUN;
         if (row < RN) {
             const int n = min(n0 + row, n1 - 1), b = n / a.T;
             src[u] = (const E*)a.x + (size_t)b * a.sx[0] + (size_t)(n - b * a.T) * a.sx[1] + kk;
@@ -161,7 +165,7 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
     const int whole = a.K / BK;
     auto fetch = [&](int t) {
 #pragma unroll
-        for (int u = 0; u < NU; ++u) oct[u].load(src[u] + (size_t)t * BK);
+        for (int u = 0; u < NU; ++u) oct[u].load_runs(src[u] + (size_t)t * BK, BK / 2);
     };
     char* const other = gemm_lds + (TWO ? G::kOne : 0);
     if (whole) {
@@ -178,7 +182,8 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
     }
     if (whole * BK < a.K) {
 #pragma unroll
-        for (int u = 0; u < NU; ++u) oct[u].load_some(src[u] + (size_t)whole * BK, a.K - whole * BK - (tid + TH * u) % UR * 8);
+        for (int u = 0; u < NU; ++u)
+            oct[u].load_some_runs(src[u] + (size_t)whole * BK, BK / 2, a.K - whole * BK - (tid + TH * u) % UR * RUN);
         stage(gemm_lds);                                          // (nobody reads either buffer here: a barrier ended the last round)
         __syncthreads();
         multiply(gemm_lds);
@@ -264,7 +269,7 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
             }
         }
     };
-    [&]<int... I>(std::integer_sequence<int, I...>) { (finish(std::integral_constant<int, I>{}), ...); }(std::make_integer_sequence<int, MR>{});
+    each_of(finish, std::make_integer_sequence<int, MR>{});
 }
 
 template <class E, int WR, int WC, int MR, int MC, int BK, bool TWO, bool FUSED = false>

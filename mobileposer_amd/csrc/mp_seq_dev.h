@@ -27,6 +27,8 @@ template <> struct Oct<bf16raw> {
         for (int i = 0; i < 8; ++i) t[i] = i < n ? p[i] : (bf16raw)0;
         __builtin_memcpy(&v, t, 16);
     }
+    __device__ __forceinline__ void load_runs(const bf16raw* p, int) { load(p); }
+    __device__ __forceinline__ void load_some_runs(const bf16raw* p, int, int n) { load_some(p, n); }
     __device__ __forceinline__ void load_clamped(const bf16raw* row, int d, int n) {
         bf16raw t[8];
         for (int i = 0; i < 8; ++i) t[i] = row[min(d + i, n - 1)];
@@ -71,6 +73,17 @@ template <> struct Oct<float> {
     __device__ __forceinline__ void load(const float* p) { __builtin_memcpy(v, p, 32); }
     __device__ __forceinline__ void load_guarded(const float* p, int n) {
         for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : 0.f;
+    }
+    // two runs of four, `gap` apart; the first n of the row from p on are there
+    __device__ __forceinline__ void load_runs(const float* p, int gap) {
+        __builtin_memcpy(v, p, 16);
+        __builtin_memcpy(v + 4, p + gap, 16);
+    }
+    __device__ __forceinline__ void load_some_runs(const float* p, int gap, int n) {
+        for (int i = 0; i < 8; ++i) {
+            const int at = (i & 3) + (i >> 2) * gap;
+            v[i] = at < n ? p[at] : 0.f;
+        }
     }
     __device__ __forceinline__ void load_clamped(const float* row, int d, int n) {
         for (int i = 0; i < 8; ++i) v[i] = row[min(d + i, n - 1)];
