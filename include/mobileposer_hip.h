@@ -136,6 +136,16 @@ int mp_rnn_forward(mp_handle* h, int module, const float* x_dev, const int32_t* 
                    int B, int T, float* y_dev, const float* state_in_dev, float* state_out_dev,
                    void* stream);
 
+/* The same block with low-rank adapters of the batch's sequences beside its linear layers (mp_linear_adapted below has the formula):
+ * down*_dev [n,r,K], up*_dev [n,M,r], scale*_dev [n] or NULL (1), fp32, for linear1 (K = the block's input, M = its hidden size)
+ * and linear2 (K = dirs x hidden size, M = the block's output); both factors NULL: that layer as it is.  ids_dev [B] int32 on the
+ * device: negative = the shared layers alone, >= n = the sequence's outputs are NaN.  ws_dev: mp_linear_adapted_workspace(B, T, the
+ * larger rank) bytes, 16-byte aligned.  LSTM modes 0 and 1 (mode 3 is refused for the H = 256 blocks). */
+int mp_rnn_forward_adapted(mp_handle* h, int module, const float* x_dev, const int32_t* lengths_host, int B, int T, float* y_dev,
+                           const float* state_in_dev, float* state_out_dev, const float* down1_dev, const float* up1_dev,
+                           const float* scale1_dev, int r1, const float* down2_dev, const float* up2_dev, const float* scale2_dev,
+                           int r2, const int32_t* ids_dev, int n_adapters, void* ws_dev, size_t ws_bytes, void* stream);
+
 /* MobilePoserNet._reduced_global_to_full (models/net.py:93-99): r6d [N,96] -> pose [N,24,3,3]. */
 int mp_reduced_global_to_full(mp_handle* h, const float* r6d_dev, int64_t N, float* pose_dev, void* stream);
 

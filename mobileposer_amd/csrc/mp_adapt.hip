@@ -119,7 +119,7 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
             src[u] = (const E*)a.x + (size_t)b * a.sx[0] + (size_t)(n - b * a.T) * a.sx[1] + kk;
         } else {
             const int m = m0 + row - RN;
-            src[u] = (const E*)a.w + (size_t)min(m, a.M - 1) * a.K + kk;
+            src[u] = (const E*)a.w + (size_t)min(m, a.M - 1) * a.ldw + kk;
             if (FUSED && adapt && m >= Mp) src[u] = (const E*)a.down + ((size_t)sid * a.r + min(m - Mp, a.r - 1)) * a.K + kk;
         }
     }
@@ -208,8 +208,9 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
     // one 16-row tile of the wave (a function of a constant: acc stays in registers whatever the compiler thinks of unrolling this)
     auto finish = [&](auto tile_row) {
         constexpr int i = decltype(tile_row)::value;
-        const int n = n0 + (wr * MR + i) * 16 + col, nc = min(n, n1 - 1);      // 16 rows, one per lane column
-        const int id = FUSED ? sid : a.ids[nc / a.T];
+        const int n = n0 + (wr * MR + i) * 16 + col, nc = min(n, n1 - 1), b = FUSED ? seq : nc / a.T;      // 16 rows, one per lane column
+        const int id = FUSED ? sid : a.ids[b];
+        E* const yrow = (E*)a.y + (size_t)b * a.sy[0] + (size_t)(nc - b * a.T) * a.sy[1];
         const bool use = id >= 0 && id < a.n;
         const float* z = FUSED ? zl + ((wr * MR + i) * 16 + col) * G::kRowZ : a.ws + (size_t)nc * rlen;
         const int id0 = __builtin_amdgcn_readfirstlane(id);
@@ -259,7 +260,7 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
                 if (id >= a.n) y[r] = __builtin_nanf("");
                 if (a.relu) y[r] = relu_(y[r]);
             }
-            E* out = (E*)a.y + (size_t)n * a.M + m;
+            E* out = yrow + m;
             if (a.vec) {                                          // M a multiple of 4: whole groups of columns, aligned
                 if (m < a.M) store4(out, y);
             } else {
@@ -286,7 +287,7 @@ template <class E>
 static bool launch_for(AdaptArgs a, hipStream_t s) {
     constexpr bool half = Arith<E>::P == 1;
     const int rows = a.B * a.T, per_seq = (a.T + 15) / 16;
-    a.vec = a.M % 4 == 0 && (uintptr_t)a.y % (4 * sizeof(E)) == 0;
+    a.vec = a.M % 4 == 0 && a.sy[0] % 4 == 0 && a.sy[1] % 4 == 0 && (uintptr_t)a.y % (4 * sizeof(E)) == 0;
     bool ok;
     if ((a.M + 15) / 16 * 16 + a.r <= 128 && a.T >= 64) {
         ok = gemm_for<E, 4, 2, 2, 4, half ? 64 : 32, true, true>(a, rows, s);

@@ -99,12 +99,9 @@ int mp_forward_offline(mp_handle* h, const float* imu_dev, const int32_t* length
     return leave(h, stream);
 }
 
-int mp_rnn_forward(mp_handle* h, int module, const float* x_dev, const int32_t* lengths_host, int B, int T,
-                   float* y_dev, const float* state_in_dev, float* state_out_dev, void* stream) {
-    if (!h) return MP_ERR_INVALID;
-    if (int rc = need_weights(h, "mp_rnn_forward")) return rc;
-    if (module < 0 || module > 3 || !x_dev || !y_dev || !lengths_host || B < 1 || T < 1)
-        return fail(h, MP_ERR_INVALID, "mp_rnn_forward: bad argument");
+// one block over a batch; `adapters` (or nullptr): of its linear layers
+static int block_forward(mp_handle* h, const char* what, int module, const float* x_dev, const int32_t* lengths_host, int B, int T,
+                         float* y_dev, const float* state_in_dev, float* state_out_dev, const BlockAdapters* adapters, void* stream) {
     ON_DEVICE(h);
     if (int rc = enter(h, stream)) return rc;
     Plan* p = nullptr;
@@ -116,7 +113,7 @@ int mp_rnn_forward(mp_handle* h, int module, const float* x_dev, const int32_t* 
     h->segs.clear(); h->ev_used = 0;
     RnnJob job{h, p, module, user_map(x_dev, T, m.n_in), none, y_dev, (long)T * m.n_out, m.n_out,
                state_in_dev ? STATE_FROM : STATE_ZERO, state_in_dev, state_in_dev ? state_in_dev + half : nullptr,
-               state_out_dev, state_out_dev ? state_out_dev + half : nullptr};
+               state_out_dev, state_out_dev ? state_out_dev + half : nullptr, adapters};
     // state_in_dev == state_out_dev: the fused kernels update the state in place, so a starved run would leave NaN where the
     // repair has to start from -- keep a copy for the restore (recovery on only)
     const bool aliased = state_in_dev && state_in_dev == state_out_dev;
@@ -133,11 +130,42 @@ int mp_rnn_forward(mp_handle* h, int module, const float* x_dev, const int32_t* 
     }
     int rc = run_rnn(job, h->s_main);
     if (rc) return rc;
-    if (int rc2 = finish_or_recover(h, p, "mp_rnn_forward", [&]() {
+    if (int rc2 = finish_or_recover(h, p, what, [&]() {
             if (aliased) HIPCHK(h, hipMemcpyAsync(state_out_dev, h->rnn_snap, state_bytes, hipMemcpyDeviceToDevice, h->s_main));
             return (int)MP_OK;
         }, [&]() { return run_rnn(job, h->s_main); })) return rc2;
     return leave(h, stream);
+}
+
+int mp_rnn_forward(mp_handle* h, int module, const float* x_dev, const int32_t* lengths_host, int B, int T,
+                   float* y_dev, const float* state_in_dev, float* state_out_dev, void* stream) {
+    if (!h) return MP_ERR_INVALID;
+    if (int rc = need_weights(h, "mp_rnn_forward")) return rc;
+    if (module < 0 || module > 3 || !x_dev || !y_dev || !lengths_host || B < 1 || T < 1)
+        return fail(h, MP_ERR_INVALID, "mp_rnn_forward: bad argument");
+    return block_forward(h, "mp_rnn_forward", module, x_dev, lengths_host, B, T, y_dev, state_in_dev, state_out_dev, nullptr, stream);
+}
+
+int mp_rnn_forward_adapted(mp_handle* h, int module, const float* x_dev, const int32_t* lengths_host, int B, int T, float* y_dev,
+                           const float* state_in_dev, float* state_out_dev, const float* down1_dev, const float* up1_dev,
+                           const float* scale1_dev, int r1, const float* down2_dev, const float* up2_dev, const float* scale2_dev,
+                           int r2, const int32_t* ids_dev, int n_adapters, void* ws_dev, size_t ws_bytes, void* stream) {
+    if (!h) return MP_ERR_INVALID;
+    if (int rc = need_weights(h, "mp_rnn_forward_adapted")) return rc;
+    if (module < 0 || module > 3 || !x_dev || !y_dev || !lengths_host || B < 1 || T < 1 || !ids_dev || n_adapters < 1)
+        return fail(h, MP_ERR_INVALID, "mp_rnn_forward_adapted: bad argument");
+    if (!down1_dev != !up1_dev || !down2_dev != !up2_dev || (down1_dev && (r1 < 1 || r1 > 128)) || (down2_dev && (r2 < 1 || r2 > 128)))
+        return fail(h, MP_ERR_INVALID, "mp_rnn_forward_adapted: a layer has both factors or none, of rank 1..128 (%d, %d)", r1, r2);
+    const int r = down1_dev && (!down2_dev || r1 > r2) ? r1 : down2_dev ? r2 : 0;
+    const size_t need = mp_linear_adapted_workspace(B, T, r);
+    if (need && (!ws_dev || ws_bytes < need || (uintptr_t)ws_dev % 16))
+        return fail(h, MP_ERR_INVALID, "mp_rnn_forward_adapted: workspace of %zu bytes, %zu needed (16-byte aligned)", ws_bytes, need);
+    if ((int64_t)B * T > (int64_t)1 << 30 || (int64_t)B * T * r > (int64_t)0x7fffffff)
+        return fail(h, MP_ERR_INVALID, "mp_rnn_forward_adapted: %d x %d frames are too many for one call", B, T);
+    if (use_x3(h, h->mod[module]))               // (its linear layers hand their rows over as pairs of halves)
+        return fail(h, MP_ERR_INVALID, "mp_rnn_forward_adapted runs on exact-fp32 operands (LSTM mode 1 or 0)");
+    const BlockAdapters ad{{down1_dev, up1_dev, scale1_dev, r1}, {down2_dev, up2_dev, scale2_dev, r2}, ids_dev, n_adapters, (float*)ws_dev};
+    return block_forward(h, "mp_rnn_forward_adapted", module, x_dev, lengths_host, B, T, y_dev, state_in_dev, state_out_dev, &ad, stream);
 }
 
 int mp_reduced_global_to_full(mp_handle* h, const float* r6d_dev, int64_t N, float* pose_dev, void* stream) {

@@ -276,6 +276,13 @@ enum StateMode { STATE_ZERO, STATE_FROM };
 //   g2: final (h,c) copy-out, linear2 into the caller's layout
 // x = [a0 | a1] rows (b,t); y rows (b,t) at y + b*yStrideB + t*yStrideT.
 // in_h/in_c, out_h/out_c: [layers*dirs][B][H] carried state (read when mode == STATE_FROM, written when out != null)
+// adapters per sequence beside a block's two linear layers (mp_rnn_forward_adapted); a layer without any has down == nullptr
+struct BlockAdapters {
+    struct Layer { const float *down, *up, *scale; int r; } lin1, lin2;
+    const int32_t* ids;          // device, [B]
+    int n;
+    float* ws;
+};
 struct RnnJob {
     mp_handle* h; Plan* p; int id;
     RowMap a0, a1;
@@ -283,6 +290,7 @@ struct RnnJob {
     StateMode mode;
     const float *in_h, *in_c;
     float *out_h, *out_c;
+    const BlockAdapters* adapters = nullptr;
 };
 
 // ---- mp_handle.hip

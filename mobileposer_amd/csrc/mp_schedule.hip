@@ -2,6 +2,7 @@
 // kernel family and slices per slab, cluster placement on XCDs, and the schedules of forward_body (which blocks run side by
 // side, what rides in whose workgroups, which seam is one launch).
 #include "mp_host.h"
+#include "mp_seq.h"
 
 namespace mph {
 
@@ -26,6 +27,17 @@ int run_gemm(mp_handle* h, hipStream_t s, RowMap a0, RowMap a1, const Packed& w,
     return MP_OK;
 }
 
+
+// the same layer with the adapters of the batch's sequences beside it (mp_adapt.hip; exact-fp32 operands, x in one piece)
+int run_gemm_adapted(mp_handle* h, hipStream_t s, RowMap x, const Packed& w, const BlockAdapters& ad, const BlockAdapters::Layer& l,
+                     float* C, long cStrideB, long cStrideT, int B, int T, int relu) {
+    SegScope seg(h, s, 0, 2, 2.0 * B * T * ((double)w.N * w.K + (double)l.r * (w.N + w.K)));
+    mpseq::AdaptArgs a;
+    a.x = x.base; a.sx[0] = x.strideB; a.sx[1] = x.strideT; a.w = w.W; a.ldw = w.Kpad; a.bias = w.bias;
+    a.down = l.down; a.up = l.up; a.scale = l.scale; a.ids = ad.ids; a.B = B; a.T = T; a.K = w.K; a.M = w.N; a.n = ad.n; a.r = l.r;
+    a.relu = relu; a.y = C; a.sy[0] = cStrideB; a.sy[1] = cStrideT; a.ws = ad.ws;
+    return mpseq::launch_adapt(a, mpseq::kF32, s) ? MP_OK : fail(h, MP_ERR_HIP, "linear layer with adapters: launch failed");
+}
 
 // linear1's output X1 normally lives in out1's memory (dead until layer 1 writes it); the two-layer wavefront
 // kernel writes out1 while layer 0 is still reading X1, so there X1 goes to the (otherwise unused) out0
@@ -79,8 +91,12 @@ int rnn_g0(const RnnJob& j, hipStream_t s) {
     const RowMap none{nullptr, 0, 0, 0};
     float* X1 = x1_buffer(h, m, w);
     // (split-bf16 mode: this GEMM also re-arms the exchange area of the layer-0 launch that follows it)
-    run_gemm(h, s, j.a0, j.a1, m.lin1, X1, H, (long)B * H, M, B, 1, use_x3(h, m), false, use_x3(h, m),
-             use_x3(h, m) ? w.hx : nullptr, dirs * ((B + 15) / 16));                               // rnn.py:22
+    if (j.adapters && j.adapters->lin1.down) {
+        if (int rc = run_gemm_adapted(h, s, j.a0, m.lin1, *j.adapters, j.adapters->lin1, X1, H, (long)B * H, B, T, 1)) return rc;
+    } else {
+        run_gemm(h, s, j.a0, j.a1, m.lin1, X1, H, (long)B * H, M, B, 1, use_x3(h, m), false, use_x3(h, m),
+                 use_x3(h, m) ? w.hx : nullptr, dirs * ((B + 15) / 16));                           // rnn.py:22
+    }
     // the per-step kernels take the input projection from a GEMM; the persistent kernel computes it itself
     if (!h->persist && !w.xproj) return fail(h, MP_ERR_INVALID, "internal: per-step workspace missing");
     if (!h->persist)
@@ -402,8 +418,13 @@ int rnn_g2(const RnnJob& j, hipStream_t s) {
                 HIPCHK(h, hipMemcpyAsync(j.out_c + (size_t)k * B * H, w.cbuf[l][d], n, hipMemcpyDeviceToDevice, s));
             }
     }
-    run_gemm(h, s, internal_map(w.out1, B, dirs * H), none, m.lin2, j.y, j.yStrideB, j.yStrideT, M, B, 0, false,
-             use_x3(h, m), use_x3(h, m));                                                          // rnn.py:32
+    if (j.adapters && j.adapters->lin2.down) {
+        if (int rc = run_gemm_adapted(h, s, internal_map(w.out1, B, dirs * H), m.lin2, *j.adapters, j.adapters->lin2, j.y, j.yStrideB,
+                                      j.yStrideT, B, T, 0)) return rc;
+    } else {
+        run_gemm(h, s, internal_map(w.out1, B, dirs * H), none, m.lin2, j.y, j.yStrideB, j.yStrideT, M, B, 0, false,
+                 use_x3(h, m), use_x3(h, m));                                                      // rnn.py:32
+    }
     HIPCHK(h, hipGetLastError());
     return MP_OK;
 }

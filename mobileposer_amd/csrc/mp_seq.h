@@ -51,12 +51,14 @@ bool launch_delta_online(const DeltaOnlineArgs& a, int dtype, hipStream_t s);
 struct AdaptArgs {
     const void* x;                               // [B][T][K], row strides below
     long sx[2];                                  // batch, time
-    const void *w, *bias;                        // [M][K], [M] or nullptr
+    const void *w, *bias;                        // [M] rows of K, ldw apart; [M] or nullptr
+    long ldw;
     const void *down, *up;                       // [n][r][K], [n][M][r]
     const float* scale;                          // [n] or nullptr (1)
     const int* ids;                              // [B]; negative: no adapter, >= n: the sequence's rows become NaN
     int B, T, K, M, n, r, relu;
-    void* y;                                     // [B][T][M] contiguous
+    void* y;                                     // [B][T][M], row strides below
+    long sy[2];                                  // batch, time
     float* ws;                                   // [B*T][r] fp32
     bool vec;                                    // (set by the launcher) groups of four columns of y can be stored at once
 };

@@ -104,9 +104,9 @@ int mp_linear_adapted(mp_handle* h, int dtype, const void* x_dev, const int64_t 
         return fail(h, MP_ERR_INVALID, "mp_linear_adapted: %d x %d rows to %d columns are too many for one call", B, T, M);
     ON_DEVICE(h);
     mpseq::AdaptArgs a;
-    a.x = x_dev; a.sx[0] = strides[0]; a.sx[1] = strides[1]; a.w = w_dev; a.bias = bias_dev; a.down = down_dev; a.up = up_dev;
+    a.x = x_dev; a.sx[0] = strides[0]; a.sx[1] = strides[1]; a.w = w_dev; a.ldw = K; a.bias = bias_dev; a.down = down_dev; a.up = up_dev;
     a.scale = scale_dev; a.ids = ids_dev; a.B = B; a.T = T; a.K = K; a.M = M; a.n = n_adapters; a.r = r; a.relu = relu != 0;
-    a.y = y_dev; a.ws = (float*)ws_dev;
+    a.y = y_dev; a.sy[0] = (long)T * M; a.sy[1] = M; a.ws = (float*)ws_dev;
     if (!mpseq::launch_adapt(a, dtype, (hipStream_t)stream)) return fail(h, MP_ERR_HIP, "mp_linear_adapted: launch failed");
     return MP_OK;
 }

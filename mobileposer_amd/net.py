@@ -696,8 +696,10 @@ class MobilePoserNet(SequenceOps):
         self._after_call()
         return table
 
-    def rnn_forward(self, module, x, input_lengths, state=None):
-        """RNN.forward of one sub-module (models/rnn.py:20-33): -> (y [B,T,n_out], (h_n, c_n))."""
+    def rnn_forward(self, module, x, input_lengths, state=None, adapters=None, ids=None):
+        """RNN.forward of one sub-module (models/rnn.py:20-33): -> (y [B,T,n_out], (h_n, c_n)).  ``adapters``: low-rank adapters beside
+        the block's linear layers, {"linear1": (down, up, scale or None), "linear2": ...} (either may be missing) as
+        ``linear_adapted`` takes them, fp32, and ``ids`` [B]: the adapter of each sequence, negative = none."""
         self._require_weights()
         mod = {"joints": 0, "pose": 1, "foot_contact": 2, "velocity": 3}[module]
         n_out, H, dirs = {0: (72, 256, 2), 1: (96, 256, 2), 2: (2, 64, 2), 3: (72, 256, 1)}[mod]
@@ -716,7 +718,16 @@ class MobilePoserNet(SequenceOps):
                 if tuple(t.shape) != want:       # (nn.LSTM raises "Expected hidden size ..." here: SURVEY Q2, a batch-size change)
                     raise RuntimeError("Expected %s of shape %s for a batch of %d sequences, got %s" % (name, want, B, tuple(t.shape)))
             st_in = torch.stack((state[0], state[1])).to(device=self.device, dtype=torch.float32).contiguous()
-        rc = self._lib.mp_rnn_forward(self._h, mod, _ptr(x), lens, B, T, _ptr(y), _ptr(st_in), _ptr(st_out), self._stream())
+        if adapters is None:
+            if ids is not None:
+                raise RuntimeError("rnn_forward: ids without adapters")
+            rc = self._lib.mp_rnn_forward(self._h, mod, _ptr(x), lens, B, T, _ptr(y), _ptr(st_in), _ptr(st_out), self._stream())
+        else:
+            layers, n, rank, ids, keep = self._block_adapters(adapters, ids, B, {"linear1": (n_in, H), "linear2": (dirs * H, n_out)})
+            need = self._lib.mp_linear_adapted_workspace(B, T, rank)
+            ws = torch.empty(need, device=self.device, dtype=torch.uint8)
+            rc = self._lib.mp_rnn_forward_adapted(self._h, mod, _ptr(x), lens, B, T, _ptr(y), _ptr(st_in), _ptr(st_out), *layers["linear1"],
+                                                  *layers["linear2"], _ptr(ids), n, _ptr(ws), need, self._stream())
         self._check(rc)
         self._after_call()
         return y, (st_out[0], st_out[1])

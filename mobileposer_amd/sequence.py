@@ -138,6 +138,29 @@ class SequenceOps:
             state.data_ptr(), _stream_of(self._device_index)))
         return o
 
+    def _block_adapters(self, adapters, ids, B, shapes):
+        """``rnn_forward``'s adapters, checked: per layer its four arguments of mp_rnn_forward_adapted; the number of adapters, the
+        larger rank, the ids on the device, and the tensors those addresses belong to."""
+        if set(adapters) - set(shapes) or not adapters:
+            raise RuntimeError("rnn_forward: adapters of linear1 and / or linear2 expected, got %s" % sorted(adapters))
+        if ids is None:
+            raise RuntimeError("rnn_forward: adapters without ids")
+        args, n, rank, keep = {name: (0, 0, 0, 0) for name in shapes}, None, 0, []
+        for name, (down, up, scale) in adapters.items():
+            K, M = shapes[name]
+            _no_grad(down, up, scale)
+            if self._dtype("rnn_forward: adapters", down, up, *(() if scale is None else (scale,))) != _lib.F32:
+                raise RuntimeError("rnn_forward: adapters are float32, got %s" % down.dtype)
+            if down.dim() != 3 or down.shape[2] != K or not 1 <= down.shape[1] <= 128 or up.shape != (down.shape[0], M, down.shape[1]) or \
+                    down.shape[0] < 1 or down.shape[0] != (n or down.shape[0]) or (scale is not None and scale.shape != down.shape[:1]):
+                raise RuntimeError("rnn_forward: %s: down [n, r, %d], up [n, %d, r] and scale [n] with r at most 128 and one n expected, got %s and %s" %
+                                   (name, K, M, tuple(down.shape), tuple(up.shape)))
+            n, rank = down.shape[0], max(rank, down.shape[1])
+            down, up, scale = down.contiguous(), up.contiguous(), None if scale is None else scale.contiguous()
+            keep += [down, up, scale]
+            args[name] = (down.data_ptr(), up.data_ptr(), 0 if scale is None else scale.data_ptr(), down.shape[1])
+        return args, n, rank, self._indices("rnn_forward: ids", ids, B, -_INT_MAX, n - 1), keep
+
     def linear_adapted(self, x, weight, bias, down, up, scale, ids, relu=False):
         """``act(x W^T + b + scale[a] (x down[a]^T) up[a]^T)`` with a = ids[sequence]: a linear layer (nn.Linear's weight [M, K] and
         bias [M] or None) with a low-rank adapter per sequence beside it.  x [B, T, K] or, one frame each, [B, K]; down [n, r, K],

@@ -486,3 +486,87 @@ def test_refusals(ops):
         with pytest.raises(RuntimeError):
             call()
             raise AssertionError("call %d was not refused" % i)
+
+
+BLOCKS = {"joints": (60, 256, 2, 72), "pose": (132, 256, 2, 96), "foot_contact": (132, 64, 2, 2), "velocity": (132, 256, 1, 72)}
+
+
+def block_adapters(module, n, r1, r2, seed):
+    """Adapters of magnitude 1/10 of the layers' own weights, on the host."""
+    import torch
+    n_in, H, dirs, n_out = BLOCKS[module]
+    gen = torch.Generator().manual_seed(seed)
+    rn = lambda *s: torch.randn(*s, generator=gen)
+    layer = lambda K, M, r: (rn(n, r, K) / math.sqrt(K), 0.1 * rn(n, M, r) / math.sqrt(r), torch.rand(n, generator=gen) + 0.5)
+    return {"linear1": layer(n_in, H, r1), "linear2": layer(dirs * H, n_out, r2)}
+
+
+def merged(weights, prefix, adapters, a):
+    """The block's weights with adapter `a` added to them (None: as they are)."""
+    sd = dict(weights)
+    if a is not None:
+        for name, (down, up, scale) in adapters.items():
+            key = prefix + name + ".weight"
+            sd[key] = (sd[key].astype(np.float64) + float(scale[a]) * (up[a].double() @ down[a].double()).numpy()).astype(np.float32)
+    return sd
+
+
+@pytest.mark.parametrize("lstm_mode", [1, 0])
+@pytest.mark.parametrize("shape", [(1, 1), (3, 17), (2, 80), (40, 5)], ids=str)
+@pytest.mark.parametrize("module", list(BLOCKS))
+def test_block_of_the_model_with_adapters(ops, module, shape, lstm_mode):
+    """rnn_forward with adapters equals, sequence by sequence, the block whose weights have the adapter added (rounding the sums of
+    the weights is 2^-24 of them: nothing beside the 1e-4 that the network outputs are held to); ragged, on a carried state."""
+    import torch
+    from mobileposer_amd import synthetic
+    from oracle import mp_oracle as O
+    weights = synthetic.make_weights(0)
+    n_in, H, dirs, n_out = BLOCKS[module]
+    B, T = shape
+    adapters = block_adapters(module, 3, 4, 8, 30)
+    dev = {k: tuple(t.cuda() for t in v) for k, v in adapters.items()}
+    gen = torch.Generator().manual_seed(31)
+    x = torch.randn(B, T, n_in, generator=gen)
+    state = [0.3 * torch.randn(2 * dirs, B, H, generator=gen) for _ in range(2)]
+    lengths = [max(1, T - 3 * (b % 4)) for b in range(B)]
+    lengths[0] = T
+    ids = [2, -1, 0, 1][:B] if B <= 4 else [b % 4 - 1 for b in range(B)]
+    ops.set_lstm_mode(lstm_mode)
+    try:
+        y, (h, c) = ops.rnn_forward(module, x.cuda(), lengths, [s.cuda() for s in state], dev, ids)
+        one, _ = ops.rnn_forward(module, x.cuda(), lengths, None, {"linear2": dev["linear2"]}, torch.tensor(ids).cuda())
+        plain, _ = ops.rnn_forward(module, x.cuda(), lengths, None)
+        none, _ = ops.rnn_forward(module, x.cuda(), lengths, None, dev, [-1] * B)
+    finally:
+        ops.set_lstm_mode(1)
+    assert float((none - plain).abs().max()) < 1e-4
+    for b in {0, 1 % B, B // 2, B - 1}:
+        a = None if ids[b] < 0 else ids[b]
+        n = lengths[b]
+        sd = merged(weights, O.PREFIX[module], adapters, a)
+        wy, (wh, wc) = O.rnn_forward(sd, O.PREFIX[module], x[b:b + 1].numpy(), [n], tuple(s[:, b:b + 1].numpy() for s in state))
+        assert np.abs(npy(y[b, :n]) - wy[0, :n]).max() < 1e-4
+        assert np.abs(npy(h[:, b]) - wh[:, 0]).max() < 1e-4 and np.abs(npy(c[:, b]) - wc[:, 0]).max() < 1e-4
+        sd = merged(weights, O.PREFIX[module], {"linear2": adapters["linear2"]}, a)
+        wy, _ = O.rnn_forward(sd, O.PREFIX[module], x[b:b + 1].numpy(), [n])
+        assert np.abs(npy(one[b, :n]) - wy[0, :n]).max() < 1e-4
+
+
+def test_block_of_the_model_with_adapters_refusals(ops):
+    import torch
+    dev = {k: tuple(t.cuda() for t in v) for k, v in block_adapters("pose", 2, 4, 8, 32).items()}
+    x = torch.zeros(2, 3, 132, device="cuda")
+    down, up, scale = dev["linear1"]
+    run = lambda adapters, ids: ops.rnn_forward("pose", x, [3, 3], None, adapters, ids)
+    for adapters, ids in [({}, [0, 1]), ({"linear3": dev["linear1"]}, [0, 1]), (dev, None), (None, [0, 1]), (dev, [0, 2]), (dev, [0]),
+                          ({"linear1": dev["linear2"]}, [0, 1]), ({"linear1": (down, up[:1], scale)}, [0, 1]), ({"linear1": (down, up, scale[:1])}, [0, 1]),
+                          ({"linear1": (down.bfloat16(), up.bfloat16(), None)}, [0, 1]), ({"linear1": (down.cpu(), up, scale)}, [0, 1]),
+                          ({"linear1": (down[:1], up[:1], None), "linear2": dev["linear2"]}, [0, 0])]:
+        with pytest.raises(RuntimeError):
+            run(adapters, ids)
+    ops.set_lstm_mode(3)
+    try:
+        with pytest.raises(RuntimeError, match="mode 1 or 0"):
+            run(dev, [0, 1])
+    finally:
+        ops.set_lstm_mode(1)

@@ -67,3 +67,24 @@ def test_entries_without_a_handle_and_workspace_sizes():
         assert f(0, 1, 1) == f(1, 0, 1) == f(1, 1, 0) == 0
         assert 0 < f(1, 1, 1) <= f(2, 1, 1) <= f(2, 33, 1) <= f(2, 33, 3)
         assert f(4096, 65536, 64) > 2 ** 32                # sizes pass 32 bits
+
+
+def block(**change):
+    z = torch.zeros
+    layers = {"linear1": (z(2, 4, 60), z(2, 256, 4), z(2)), "linear2": (z(2, 8, 512), z(2, 72, 8), None)}
+    return Ops()._block_adapters({**layers, **change}, [0, -1], 2, {"linear1": (60, 256), "linear2": (512, 72)})
+
+
+@pytest.mark.parametrize("change", [
+    {"linear0": None}, {"linear1": (torch.zeros(2, 4, 61), torch.zeros(2, 256, 4), None)}, {"linear1": (torch.zeros(2, 4, 60), torch.zeros(2, 255, 4), None)},
+    {"linear1": (torch.zeros(3, 4, 60), torch.zeros(3, 256, 4), None)}, {"linear2": (torch.zeros(2, 129, 512), torch.zeros(2, 72, 129), None)},
+    {"linear2": (torch.zeros(2, 8, 512), torch.zeros(2, 72, 8), torch.zeros(3))}, {"linear2": (torch.zeros(2, 8, 512).double(), torch.zeros(2, 72, 8).double(), None)},
+    {"linear2": (torch.zeros(2, 8, 512).bfloat16(), torch.zeros(2, 72, 8).bfloat16(), None)}, {"linear2": (torch.zeros(2, 8, 512, requires_grad=True), torch.zeros(2, 72, 8), None)},
+], ids=lambda c: next(iter(c)))
+def test_block_adapters_refuses(change):
+    with pytest.raises(RuntimeError):
+        block(**change)
+    with pytest.raises(RuntimeError):
+        Ops()._block_adapters({}, [0, 1], 2, {"linear1": (60, 256), "linear2": (512, 72)})
+    lib = _lib.load()
+    assert lib.mp_rnn_forward_adapted(None, 0, None, None, 1, 1, *[None] * 6, 1, *[None] * 3, 1, None, 1, None, 0, None) == _lib.MP_ERR_INVALID
