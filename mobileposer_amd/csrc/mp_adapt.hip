@@ -82,7 +82,7 @@ MP_KERNEL __launch_bounds__(256) void mp_adapt_down(AdaptArgs a, int per_seq) {
 // load of 16 bytes a lane has no gaps between the lanes either.)  The next tile's loads are in flight while this one is
 // multiplied.  BK is as long as the staging registers allow: a small tile is a chain of memory latencies.  FUSED: a row tile lies
 // inside one sequence, columns Mp .. Mp + r - 1 of the tile (Mp = M rounded up to 16) are that sequence's Down.
-template <class E, int WR, int WC, int MR, int MC, int BK, bool TWO, bool FUSED>
+template <class E, int WR, int WC, int MR, int MC, int BK, bool TWO, bool FUSED, bool DIRECT>
 struct Gemm {
     static constexpr int P = Arith<E>::P, KS = BK / 32, RN = 16 * MR * WR, CM = 16 * MC * WC, TH = 64 * WR * WC;
     static constexpr int UR = BK / 8, NB = (RN + CM) / 16 * KS, NU = (RN + CM) * UR / TH;      // blocks of a tile; pieces that a thread stages
@@ -94,9 +94,9 @@ template <class F, int... I>
 static __device__ __forceinline__ void each_of(F& f, std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }
 // where the piece (row % 16, group of eight elements 0..3) of a block lies
 static __device__ __forceinline__ int block_piece(int row, int g) { return g * 16 + (row ^ (g & 1) * 2 ^ (g >> 1) * 12); }
-template <class E, int WR, int WC, int MR, int MC, int BK, bool TWO, bool FUSED>
+template <class E, int WR, int WC, int MR, int MC, int BK, bool TWO, bool FUSED, bool DIRECT>
 MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_gemm(AdaptArgs a, int rows, int ntr, int ntc) {
-    using G = Gemm<E, WR, WC, MR, MC, BK, TWO, FUSED>;
+    using G = Gemm<E, WR, WC, MR, MC, BK, TWO, FUSED, DIRECT>;
     constexpr int P = G::P, KS = G::KS, UR = G::UR, RN = G::RN, NU = G::NU, TH = G::TH, RUN = P == 1 ? 8 : 4;
     extern __shared__ __align__(16) char gemm_lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, grp = lane >> 4;
@@ -111,9 +111,11 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
     const int sid = FUSED ? a.ids[seq] : 0;
     const bool adapt = FUSED && sid >= 0 && sid < a.n;
     const E* src[NU];
+    const int w64 = __builtin_amdgcn_readfirstlane(wave) * NU;
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
-        const int row = (tid + TH * u) / UR, kk = (tid + TH * u) % UR * RUN;
+        const int row = DIRECT ? (w64 + u) * 8 + lane / 8 : (tid + TH * u) / UR;
+        const int kk = DIRECT ? (lane % 8 ^ (row >> 1 & 7)) * 8 : (tid + TH * u) % UR * RUN;
         if (row < RN) {
             const int n = min(n0 + row, n1 - 1), b = n / a.T;
             src[u] = (const E*)a.x + (size_t)b * a.sx[0] + (size_t)(n - b * a.T) * a.sx[1] + kk;
@@ -132,7 +134,10 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
         const int row = (tid + TH * u) / UR, o = (tid + TH * u) % UR;
         at[u] = (row / 16 * KS + o / 4) * 1024 + block_piece(row % 16, o % 4) * 16;
     }
-    const int mine = block_piece(col, grp) * 16;
+    const int mine = DIRECT ? col * 128 : block_piece(col, grp) * 16;
+    auto piece = [&](const char* from, int p, int tile, int ks) {
+        return *(const u32x4*)(DIRECT ? from + tile * 2048 + mine + (ks * 4 + grp ^ col >> 1) * 16 : from + p * G::kPlane + (tile * KS + ks) * 1024 + mine);
+    };
     auto stage = [&](char* to) {
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
@@ -149,12 +154,12 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
 #pragma unroll
             for (int i = 0; i < MR; ++i)
 #pragma unroll
-                for (int p = 0; p < P; ++p) fx[i][p] = *(const u32x4*)(from + p * G::kPlane + ((wr * MR + i) * KS + ks) * 1024 + mine);
+                for (int p = 0; p < P; ++p) fx[i][p] = piece(from, p, wr * MR + i, ks);
 #pragma unroll
             for (int j = 0; j < MC; ++j) {
                 u32x4 fw[P];
 #pragma unroll
-                for (int p = 0; p < P; ++p) fw[p] = *(const u32x4*)(from + p * G::kPlane + ((RN / 16 + wc * MC + j) * KS + ks) * 1024 + mine);
+                for (int p = 0; p < P; ++p) fw[p] = piece(from, p, RN / 16 + wc * MC + j, ks);
 #pragma unroll
                 for (int i = 0; i < MR; ++i) acc[j][i] = mfma_planes(fw, fx[i], acc[j][i]);
             }
@@ -168,6 +173,21 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
         for (int u = 0; u < NU; ++u) oct[u].load_runs(src[u] + (size_t)t * BK, BK / 2);
     };
     char* const other = gemm_lds + (TWO ? G::kOne : 0);
+    if constexpr (DIRECT) {
+        auto ask = [&](int t, char* to) {
+#pragma unroll
+            for (int u = 0; u < NU; ++u)
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src[u] + (size_t)t * BK),
+                                                 (__attribute__((address_space(3))) void*)(to + (w64 + u) * 1024), 16, 0, 0);
+        };
+        ask(0, gemm_lds);
+        __syncthreads();
+        for (int t = 0; t < whole; ++t) {
+            ask(min(t + 1, whole - 1), t & 1 ? gemm_lds : other);
+            multiply(t & 1 ? other : gemm_lds);
+            __syncthreads();
+        }
+    } else {
     if (whole) {
         fetch(0);
         stage(gemm_lds);
@@ -188,6 +208,7 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
         __syncthreads();
         multiply(gemm_lds);
         if (FUSED) __syncthreads();
+    }
     }
     const int rlen = a.r;
     float* zl = (float*)gemm_lds;                                 // FUSED: [RN][kRowZ]
@@ -210,7 +231,6 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
         constexpr int i = decltype(tile_row)::value;
         const int n = n0 + (wr * MR + i) * 16 + col, nc = min(n, n1 - 1), b = FUSED ? seq : nc / a.T;      // 16 rows, one per lane column
         const int id = FUSED ? sid : a.ids[b];
-        E* const yrow = (E*)a.y + (size_t)b * a.sy[0] + (size_t)(nc - b * a.T) * a.sy[1];
         const bool use = id >= 0 && id < a.n;
         const float* z = FUSED ? zl + ((wr * MR + i) * 16 + col) * G::kRowZ : a.ws + (size_t)nc * rlen;
         const int id0 = __builtin_amdgcn_readfirstlane(id);
@@ -250,6 +270,7 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
             }
         }
         if (n >= n1) return;
+        E* const yrow = (E*)a.y + (size_t)b * a.sy[0] + (size_t)(nc - b * a.T) * a.sy[1];
 #pragma unroll
         for (int j = 0; j < MC; ++j) {
             const int m = m0 + (wc * MC + j) * 16 + 4 * grp;
@@ -273,10 +294,10 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
     each_of(finish, std::make_integer_sequence<int, MR>{});
 }
 
-template <class E, int WR, int WC, int MR, int MC, int BK, bool TWO, bool FUSED = false>
+template <class E, int WR, int WC, int MR, int MC, int BK, bool TWO, bool FUSED = false, bool DIRECT = false>
 static bool gemm_for(const AdaptArgs& a, int rows, hipStream_t s) {
-    using G = Gemm<E, WR, WC, MR, MC, BK, TWO, FUSED>;
-    const auto kernel = mp_adapt_gemm<E, WR, WC, MR, MC, BK, TWO, FUSED>;
+    using G = Gemm<E, WR, WC, MR, MC, BK, TWO, FUSED, DIRECT>;
+    const auto kernel = mp_adapt_gemm<E, WR, WC, MR, MC, BK, TWO, FUSED, DIRECT>;
     // (an attribute of the function on the current device: set at every launch, a call may come from any device's handle)
     if (G::kBytes > 64 * 1024 && hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, G::kBytes) != hipSuccess) return false;
     const int ntr = FUSED ? a.B * ((a.T + G::RN - 1) / G::RN) : (rows + G::RN - 1) / G::RN, ntc = FUSED ? 1 : (a.M + G::CM - 1) / G::CM;
@@ -301,7 +322,8 @@ static bool launch_for(AdaptArgs a, hipStream_t s) {
     auto tiles = [&](int t) { return ((long)rows + t - 1) / t * ((a.M + t - 1) / t); };
     if constexpr (half)
         if (tiles(256) >= 192) {
-            ok = gemm_for<E, 2, 4, 8, 4, 64, true>(a, rows, s);
+            const bool lines = a.K % 64 == 0 && a.ldw % 8 == 0 && a.sx[0] % 8 == 0 && a.sx[1] % 8 == 0 && ((uintptr_t)a.x | (uintptr_t)a.w) % 16 == 0;
+            ok = lines ? gemm_for<E, 2, 4, 8, 4, 64, true, false, true>(a, rows, s) : gemm_for<E, 2, 4, 8, 4, 64, true>(a, rows, s);
             return hipGetLastError() == hipSuccess && ok;
         }
     if (tiles(128) >= 192) ok = half ? gemm_for<E, 2, 2, 4, 4, half ? 64 : 32, false>(a, rows, s) : gemm_for<E, 4, 2, 2, 4, half ? 64 : 32, true>(a, rows, s);

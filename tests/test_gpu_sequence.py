@@ -332,6 +332,21 @@ def test_linear_adapted(ops, shape, dtype):
         assert torch.equal(ops.linear_adapted(x[:, 0], w, None, down, up, None, ids), y[:, 0])
 
 
+@pytest.mark.parametrize("shape", [(3, 2043, 128, 2050, 2, 20), (5, 1250, 192, 2048, 3, 32), (6200, 1, 64, 2048, 4, 8), (2, 3100, 72, 2048, 2, 4), (1, 6200, 64, 2100, 1, 33)], ids=str)
+def test_linear_adapted_many_rows_to_many_columns(ops, shape):
+    """The large tiles: rows that are whole cache lines go to LDS directly, others through registers; both ends ragged; a view whose
+    rows start in the middle of a line."""
+    import torch
+    B, T, K, M, n, r = shape
+    x, w, b, down, up, scale, ids = linear_inputs(13, B, T, K, M, n, r, torch.bfloat16)
+    want = linear_ref(x, w, b, down, up, scale, ids, True)
+    assert_linear(ops.linear_adapted(x, w, b, down, up, scale, ids, relu=True), *want, K, r, True)
+    wide = torch.full((B, T, K + 24), float("nan"), device="cuda", dtype=torch.bfloat16)
+    for at in (8, 4, 1):
+        wide[..., at:at + K] = x
+        assert_linear(ops.linear_adapted(wide[..., at:at + K], w, b, down, up, scale, ids, relu=True), *want, K, r, True)
+
+
 def test_linear_adapted_strides_ids_and_non_finite_values(ops):
     import torch
     B, T, K, M, n, r = 4, 37, 48, 80, 3, 8
