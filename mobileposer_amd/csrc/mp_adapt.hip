@@ -148,6 +148,29 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
         }
     };
     auto multiply = [&](const char* from) {
+        if constexpr (DIRECT) {
+            u32x4 fw[KS][MC][1], fx[KS][MR][1];
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+                for (int j = 0; j < MC; ++j) fw[ks][j][0] = piece(from, 0, RN / 16 + wc * MC + j, ks);
+#pragma unroll
+                for (int i = 0; i < MR; ++i) fx[ks][i][0] = piece(from, 0, wr * MR + i, ks);
+            }
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int i = 0; i < MR; ++i)
+#pragma unroll
+                    for (int j = 0; j < MC; ++j) acc[j][i] = mfma_planes(fw[ks][j], fx[ks][i], acc[j][i]);
+            __builtin_amdgcn_sched_group_barrier(0x100, MC + 2, 0);
+#pragma unroll
+            for (int g = 0; g < KS * MR; ++g) {
+                __builtin_amdgcn_sched_group_barrier(0x8, MC, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+            }
+            return;
+        }
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             u32x4 fx[MR][P];
