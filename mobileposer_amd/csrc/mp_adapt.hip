@@ -87,6 +87,7 @@ struct Gemm {
     static constexpr int P = Arith<E>::P, KS = BK / 32, RN = 16 * MR * WR, CM = 16 * MC * WC, TH = 64 * WR * WC;
     static constexpr int UR = BK / 8, NB = (RN + CM) / 16 * KS, NU = (RN + CM) * UR / TH;      // blocks of a tile; pieces that a thread stages
     static constexpr int kPlane = NB * 1024, kOne = P * kPlane, kZ = TWO ? 2 * kOne : kOne, kRowZ = 128 + 4;
+    static constexpr bool kTurn = !FUSED && 16 * MC * sizeof(E) >= 128 && RN * CM * (int)sizeof(E) <= kZ;      // outputs leave through LDS
     static constexpr int kBytes = FUSED ? (kZ > RN * kRowZ * 4 ? kZ : RN * kRowZ * 4) : kZ;      // (z takes the operands' place)
     static_assert((RN + CM) * UR % TH == 0 && kBytes <= 160 * 1024, "whole pieces per thread, LDS of a CU");
 };
@@ -230,7 +231,7 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
         stage(gemm_lds);                                          // (nobody reads either buffer here: a barrier ended the last round)
         __syncthreads();
         multiply(gemm_lds);
-        if (FUSED) __syncthreads();
+        __syncthreads();
     }
     }
     const int rlen = a.r;
@@ -249,68 +250,139 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
         }
         __syncthreads();
     }
+    // the adapters, for all rows of the wave at once where they share one
+    int id[MR];
+    bool same = true;
+#pragma unroll
+    for (int i = 0; i < MR; ++i) {
+        id[i] = FUSED ? sid : a.ids[min(n0 + (wr * MR + i) * 16 + col, n1 - 1) / a.T];
+        same = same && id[i] == __builtin_amdgcn_readfirstlane(id[0]);
+    }
+    const int id0 = __builtin_amdgcn_readfirstlane(id[0]);
+    const bool wave_same = FUSED || __all(same);
+    // z keeps 16 of its bits beside bf16 operands, all 24 beside fp32 ones
+    constexpr int PZ = P == 1 ? 2 : 3;
+    auto z_of = [&](int i) {
+        return FUSED ? zl + ((wr * MR + i) * 16 + col) * G::kRowZ : a.ws + (size_t)min(n0 + (wr * MR + i) * 16 + col, n1 - 1) * rlen;
+    };
+    auto z_planes = [&](const float* z, int k, u32x4 (&pz)[PZ]) {
+        Oct<float> oz;
+        u32x4 p3[3];
+        oz.load_some(z + k, rlen - k < 0 ? 0 : rlen - k);
+        oz.planes(p3);
+#pragma unroll
+        for (int p = 0; p < PZ; ++p) pz[p] = p3[p];
+    };
+    auto up_planes = [&](int ad, int j, int k, u32x4 (&pu)[P]) {
+        const int m = m0 + (wc * MC + j) * 16 + col;
+        Oct<E> ou;
+        ou.load_some((const E*)a.up + ((size_t)ad * a.M + (m < a.M ? m : 0)) * rlen + k, rlen - k < 0 ? 0 : rlen - k);
+        ou.planes(pu);
+    };
+    if (wave_same && id0 >= 0 && id0 < a.n)
+        for (int r0 = 0; r0 < rlen; r0 += 32) {
+            u32x4 pu[MC][P];
+#pragma unroll
+            for (int j = 0; j < MC; ++j) up_planes(id0, j, r0 + 8 * grp, pu[j]);
+            auto add = [&](auto tile_row) {
+                constexpr int i = decltype(tile_row)::value;
+                u32x4 pz[PZ];
+                z_planes(z_of(i), r0 + 8 * grp, pz);
+#pragma unroll
+                for (int j = 0; j < MC; ++j) acc[j][i] = mfma_planes(pu[j], pz, acc[j][i]);
+            };
+            each_of(add, std::make_integer_sequence<int, MR>{});
+        }
+    // the bias of the lane's columns
+    float bias[MC][4];
+#pragma unroll
+    for (int j = 0; j < MC; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int m = m0 + (wc * MC + j) * 16 + 4 * grp + r;
+            bias[j][r] = a.bias && m < a.M ? load_f((const E*)a.bias + m) : 0.f;
+        }
     // one 16-row tile of the wave (a function of a constant: acc stays in registers whatever the compiler thinks of unrolling this)
+    const bool flat = a.sy[0] == (long)a.T * a.sy[1];
+    auto row_of = [&](int n) {
+        const int b = flat ? 0 : n / a.T;
+        return (E*)a.y + (size_t)b * a.sy[0] + (size_t)(n - b * a.T) * a.sy[1];
+    };
     auto finish = [&](auto tile_row) {
         constexpr int i = decltype(tile_row)::value;
-        const int n = n0 + (wr * MR + i) * 16 + col, nc = min(n, n1 - 1), b = FUSED ? seq : nc / a.T;      // 16 rows, one per lane column
-        const int id = FUSED ? sid : a.ids[b];
-        const bool use = id >= 0 && id < a.n;
-        const float* z = FUSED ? zl + ((wr * MR + i) * 16 + col) * G::kRowZ : a.ws + (size_t)nc * rlen;
-        const int id0 = __builtin_amdgcn_readfirstlane(id);
-        if (FUSED ? adapt : __all(id == id0)) {
-            if (id0 >= 0 && id0 < a.n)                            // one adapter for the 16 rows: the matrix units again
-                for (int r0 = 0; r0 < rlen; r0 += 32) {
-                    const int k = r0 + 8 * grp, left = rlen - k < 0 ? 0 : rlen - k;
+        const int nt0 = n0 + (wr * MR + i) * 16, n = nt0 + col;    // 16 rows, one per lane column
+        if (!wave_same) {
+            const float* z = z_of(i);
+            const int tid0 = __builtin_amdgcn_readfirstlane(id[i]);
+            if (__all(id[i] == tid0)) {
+                if (tid0 >= 0 && tid0 < a.n)                      // one adapter for the 16 rows: the matrix units again
+                    for (int r0 = 0; r0 < rlen; r0 += 32) {
+                        u32x4 pz[PZ], pu[P];
+                        z_planes(z, r0 + 8 * grp, pz);
+#pragma unroll
+                        for (int j = 0; j < MC; ++j) {
+                            up_planes(tid0, j, r0 + 8 * grp, pu);
+                            acc[j][i] = mfma_planes(pu, pz, acc[j][i]);
+                        }
+                    }
+            } else if (id[i] >= 0 && id[i] < a.n) {               // a row of its own each: dot products of the lane's four columns
+                for (int q = 0; q < rlen; q += 8) {
                     Oct<float> oz;
-                    u32x4 p3[3], pz[P == 1 ? 2 : 3];              // z keeps 16 of its bits beside bf16 operands, all 24 beside fp32 ones
-                    oz.load_some(z + k, left);
-                    oz.planes(p3);
+                    oz.load_some(z + q, rlen - q);
 #pragma unroll
-                    for (int p = 0; p < (P == 1 ? 2 : 3); ++p) pz[p] = p3[p];
+                    for (int j = 0; j < MC; ++j)
 #pragma unroll
-                    for (int j = 0; j < MC; ++j) {
-                        const int m = m0 + (wc * MC + j) * 16 + col;
-                        Oct<E> ou;
-                        u32x4 pu[P];
-                        ou.load_some((const E*)a.up + ((size_t)id0 * a.M + (m < a.M ? m : 0)) * rlen + k, left);
-                        ou.planes(pu);
-                        acc[j][i] = mfma_planes(pu, pz, acc[j][i]);
-                    }
+                        for (int r = 0; r < 4; ++r) {
+                            const int m = m0 + (wc * MC + j) * 16 + 4 * grp + r;
+                            Oct<E> ou;
+                            ou.load_some((const E*)a.up + ((size_t)id[i] * a.M + (m < a.M ? m : 0)) * rlen + q, rlen - q);
+                            acc[j][i][r] = ou.dot(oz, acc[j][i][r]);
+                        }
                 }
-        } else if (!FUSED && use) {                               // a row of its own each: dot products of the lane's four columns
-            for (int q = 0; q < rlen; q += 8) {
-                Oct<float> oz;
-                oz.load_some(z + q, rlen - q);
-#pragma unroll
-                for (int j = 0; j < MC; ++j)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int m = m0 + (wc * MC + j) * 16 + 4 * grp + r;
-                        Oct<E> ou;
-                        ou.load_some((const E*)a.up + ((size_t)id * a.M + (m < a.M ? m : 0)) * rlen + q, rlen - q);
-                        acc[j][i][r] = ou.dot(oz, acc[j][i][r]);
-                    }
             }
         }
+        auto value = [&](int j, float (&y)[4]) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                y[r] = acc[j][i][r] + bias[j][r];
+                if (id[i] >= a.n) y[r] = __builtin_nanf("");
+                if (a.relu) y[r] = relu_(y[r]);
+            }
+        };
+        if (G::kTurn && a.vec == 2) {
+            // whole lines: the wave's 16 rows x 16 MC columns through its own piece of LDS (the operands' place: a barrier ended
+            // their last reads), 16 bytes a lane, the pieces of a row exchanged by its index against bank conflicts
+            constexpr int PR = MC * 16 * sizeof(E) / 16;          // 16-byte pieces of a row
+            char* const own = gemm_lds + ((wave * MR + i) * 16) * PR * 16;
+#pragma unroll
+            for (int j = 0; j < MC; ++j) {
+                float y[4];
+                value(j, y);
+                const int byte = (j * 16 + 4 * grp) * sizeof(E);
+                store4((E*)(own + (col * PR + (byte / 16 ^ col % PR)) * 16 + byte % 16), y);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+            for (int q = 0; q < PR / 4; ++q) {
+                const int row = (q * 64 + lane) / PR, piece = lane % PR, m = m0 + wc * MC * 16 + piece * 16 / (int)sizeof(E);
+                const u32x4 v = *(const u32x4*)(own + (row * PR + (piece ^ row % PR)) * 16);
+                if (nt0 + row < n1 && m < a.M) *(u32x4*)(row_of(nt0 + row) + m) = v;
+            }
+            return;
+        }
         if (n >= n1) return;
-        E* const yrow = (E*)a.y + (size_t)b * a.sy[0] + (size_t)(nc - b * a.T) * a.sy[1];
+        E* const yrow = row_of(n);
 #pragma unroll
         for (int j = 0; j < MC; ++j) {
             const int m = m0 + (wc * MC + j) * 16 + 4 * grp;
             float y[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                y[r] = acc[j][i][r] + (a.bias && m + r < a.M ? load_f((const E*)a.bias + m + r) : 0.f);
-                if (id >= a.n) y[r] = __builtin_nanf("");
-                if (a.relu) y[r] = relu_(y[r]);
-            }
-            E* out = yrow + m;
+            value(j, y);
             if (a.vec) {                                          // M a multiple of 4: whole groups of columns, aligned
-                if (m < a.M) store4(out, y);
+                if (m < a.M) store4(yrow + m, y);
             } else {
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    if (m + r < a.M) store_f(out + r, y[r]);
+                    if (m + r < a.M) store_f(yrow + m + r, y[r]);
             }
         }
     };
@@ -331,7 +403,8 @@ template <class E>
 static bool launch_for(AdaptArgs a, hipStream_t s) {
     constexpr bool half = Arith<E>::P == 1;
     const int rows = a.B * a.T, per_seq = (a.T + 15) / 16;
-    a.vec = a.M % 4 == 0 && a.sy[0] % 4 == 0 && a.sy[1] % 4 == 0 && (uintptr_t)a.y % (4 * sizeof(E)) == 0;
+    auto whole = [&](int n) { return a.M % n == 0 && a.sy[0] % n == 0 && a.sy[1] % n == 0 && (uintptr_t)a.y % (n * sizeof(E)) == 0; };
+    a.vec = whole(16 / sizeof(E)) ? 2 : whole(4) ? 1 : 0;
     bool ok;
     if ((a.M + 15) / 16 * 16 + a.r <= 128 && a.T >= 64) {
         ok = gemm_for<E, 4, 2, 2, 4, half ? 64 : 32, true, true>(a, rows, s);

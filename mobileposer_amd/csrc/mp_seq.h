@@ -60,7 +60,7 @@ struct AdaptArgs {
     void* y;                                     // [B][T][M], row strides below
     long sy[2];                                  // batch, time
     float* ws;                                   // [B*T][r] fp32
-    bool vec;                                    // (set by the launcher) groups of four columns of y can be stored at once
+    int vec;                                     // (set by the launcher) columns of y that can be stored at once: 2: 16 bytes, 1: four, 0: one
 };
 size_t adapt_ws_floats(int B, int T, int r);
 bool launch_adapt(const AdaptArgs& a, int dtype, hipStream_t s);
