@@ -190,8 +190,12 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
         }
     };
     // whole tiles, each asking for the next one (the last for itself again: no branch around the loads, which would make them wait
-    // for each other), then what is left of K
+    // for each other), then what is left of K -- small tiles, which are chains of latencies, ask for that beside the last product
     const int whole = a.K / BK;
+    // small tiles ask for their rows' adapters beside the first tile of K: a latency less at the end
+    constexpr bool kEarly = MR == 1;
+    int id[MR];
+    auto early = [&]() { id[0] = a.ids[min(n0 + wr * 16 + col, n1 - 1) / a.T]; };
     auto fetch = [&](int t) {
 #pragma unroll
         for (int u = 0; u < NU; ++u) oct[u].load_runs(src[u] + (size_t)t * BK, BK / 2);
@@ -209,6 +213,34 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
         for (int t = 0; t < whole; ++t) {
             ask(min(t + 1, whole - 1), t & 1 ? gemm_lds : other);
             multiply(t & 1 ? other : gemm_lds);
+            __syncthreads();
+        }
+    } else if constexpr (kEarly) {
+        const int left = a.K - whole * BK;
+        auto fetch_left = [&]() {
+#pragma unroll
+            for (int u = 0; u < NU; ++u) oct[u].load_some_runs(src[u] + (size_t)whole * BK, BK / 2, left - (tid + TH * u) % UR * RUN);
+        };
+        if (whole) fetch(0);
+        else fetch_left();
+        stage(gemm_lds);
+        early();
+        __syncthreads();
+        for (int t = 0; t + 1 < whole; ++t) {
+            fetch(t + 1);
+            multiply(t & 1 ? other : gemm_lds);
+            if (!TWO) __syncthreads();
+            stage(t & 1 ? gemm_lds : other);
+            __syncthreads();
+        }
+        const bool two = whole && left;                           // (a last tile behind the whole ones)
+        if (two) fetch_left();
+        multiply(whole && !(whole & 1) ? other : gemm_lds);
+        __syncthreads();
+        if (two) {
+            stage(whole & 1 ? other : gemm_lds);
+            __syncthreads();
+            multiply(whole & 1 ? other : gemm_lds);
             __syncthreads();
         }
     } else {
@@ -251,11 +283,10 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
         __syncthreads();
     }
     // the adapters, for all rows of the wave at once where they share one
-    int id[MR];
     bool same = true;
 #pragma unroll
     for (int i = 0; i < MR; ++i) {
-        id[i] = FUSED ? sid : a.ids[min(n0 + (wr * MR + i) * 16 + col, n1 - 1) / a.T];
+        if (!kEarly) id[i] = FUSED ? sid : a.ids[min(n0 + (wr * MR + i) * 16 + col, n1 - 1) / a.T];
         same = same && id[i] == __builtin_amdgcn_readfirstlane(id[0]);
     }
     const int id0 = __builtin_amdgcn_readfirstlane(id[0]);
