@@ -437,7 +437,14 @@ static bool launch_for(AdaptArgs a, hipStream_t s) {
     auto whole = [&](int n) { return a.M % n == 0 && a.sy[0] % n == 0 && a.sy[1] % n == 0 && (uintptr_t)a.y % (n * sizeof(E)) == 0; };
     a.vec = whole(16 / sizeof(E)) ? 2 : whole(4) ? 1 : 0;
     bool ok;
-    if ((a.M + 15) / 16 * 16 + a.r <= 128 && a.T >= 64) {
+    // One launch that reads x once (FUSED) or two.  Its row tiles of 128 end with their sequence, its one column of tiles walks K in a
+    // chain.  With many rows it wins (us, one against two): 256 x 125 512 -> 96 bf16 15 / 32, fp32 31 / 49; 128 x 125 fp32 29 / 35;
+    // below 12000 rows the chain is what is timed (fp32 64 x 125 27 / 26, 8 x 125 26 / 16), unless K is short enough that the second
+    // launch costs more (bf16 256 x 1 13 / 16, at K = 2048 30 / 16; fp32 K = 132 14 / 16); more row tiles than CUs have to be more than
+    // half full (fp32 256 x 64 30 / 33, 1024 x 64 109 / 86, bf16 1024 x 1 30 / 16).
+    const long ftiles = (long)a.B * ((a.T + 127) / 128);
+    const bool few = ftiles <= 256, many_rows = rows >= 12000 && (few || rows > 64 * ftiles);
+    if ((a.M + 15) / 16 * 16 + a.r <= 128 && (many_rows || (few && a.K <= (half ? 512 : 192)))) {
         ok = gemm_for<E, 4, 2, 2, 4, half ? 64 : 32, true, true>(a, rows, s);
         return hipGetLastError() == hipSuccess && ok;
     }
@@ -446,15 +453,21 @@ static bool launch_for(AdaptArgs a, hipStream_t s) {
     else if (a.r <= 32) hipLaunchKernelGGL((mp_adapt_down<E, 2>), grid, dim3(256), 0, s, a, per_seq);
     else if (a.r <= 64) hipLaunchKernelGGL((mp_adapt_down<E, 4>), grid, dim3(256), 0, s, a, per_seq);
     else hipLaunchKernelGGL((mp_adapt_down<E, 8>), grid, dim3(256), 0, s, a, per_seq);
+    // The largest tile that leaves enough of them for 256 CUs (us, K = 1024, larger / smaller tile).  256: bf16 6144 x 2048 (192 tiles)
+    // 43 / 58, 4096 x 2048 (128) 41 / 36.  128: bf16 4096 x 2048 (512) 37 / 44, 4096 x 1024 (256) 32 / 28; fp32, whose products take
+    // three times as long, 4096 x 1024 (256) 60 / 76, 2048 x 1024 (128) 57 / 47.  64: 1024 x 1024 (256) bf16 15.9 / 16.2, fp32 38 / 39,
+    // 768 x 1024 (192) 16.0 / 15.7 and 38 / 29.
     auto tiles = [&](int t) { return ((long)rows + t - 1) / t * ((a.M + t - 1) / t); };
     if constexpr (half)
         if (tiles(256) >= 192) {
+            // rows of whole cache lines go to LDS directly, others through registers (8 x 2048, 2048 -> 2048: 174 us against 192 before the
+            // steps that both share)
             const bool lines = a.K % 64 == 0 && a.ldw % 8 == 0 && a.sx[0] % 8 == 0 && a.sx[1] % 8 == 0 && ((uintptr_t)a.x | (uintptr_t)a.w) % 16 == 0;
             ok = lines ? gemm_for<E, 2, 4, 8, 4, 64, true, false, true>(a, rows, s) : gemm_for<E, 2, 4, 8, 4, 64, true>(a, rows, s);
             return hipGetLastError() == hipSuccess && ok;
         }
-    if (tiles(128) >= 192) ok = half ? gemm_for<E, 2, 2, 4, 4, half ? 64 : 32, false>(a, rows, s) : gemm_for<E, 4, 2, 2, 4, half ? 64 : 32, true>(a, rows, s);
-    else if (tiles(64) >= 192) ok = gemm_for<E, 2, 2, 2, 2, half ? 128 : 64, false>(a, rows, s);
+    if (tiles(128) >= (half ? 384 : 192)) ok = half ? gemm_for<E, 2, 2, 4, 4, half ? 64 : 32, false>(a, rows, s) : gemm_for<E, 4, 2, 2, 4, half ? 64 : 32, true>(a, rows, s);
+    else if (tiles(64) >= 256) ok = gemm_for<E, 2, 2, 2, 2, half ? 128 : 64, false>(a, rows, s);
     else ok = gemm_for<E, 2, 2, 1, 1, half ? 256 : 128, false>(a, rows, s);
     return hipGetLastError() == hipSuccess && ok;
 }

@@ -334,8 +334,9 @@ struct DeltaPlan {
     int nseg, len;                                // segments and chunks per segment; nseg = 1: the chunks in one go
     float *N, *M;                                 // [B][Hv][nseg - 1][dk][dv] (mp_delta_join turns N of s into the start of s + 1), [..][dk][dk]
 };
+template <class E, int NK> constexpr bool two_per_cu() { return Arith<E>::P == 1 ? NK <= 4 : NK <= 2; }
 template <class E, int NK, int MODE, bool OUT>
-MP_KERNEL __launch_bounds__(256, (Arith<E>::P == 1 ? NK <= 4 : NK <= 2) ? 2 : 1) void mp_delta_scan(DeltaArgs a, DeltaPlan plan, int ncol, int ncolm) {
+MP_KERNEL __launch_bounds__(256, (two_per_cu<E, NK>() ? 2 : 1)) void mp_delta_scan(DeltaArgs a, DeltaPlan plan, int ncol, int ncolm) {
     using L = ScanLds<E, NK>;
     constexpr int P = L::P, PO = L::PO;
     extern __shared__ __align__(16) char scan_lds[];
@@ -690,12 +691,15 @@ MP_KERNEL __launch_bounds__(512) void mp_delta_join(DeltaArgs a, DeltaPlan plan,
     }
 }
 
-// Segments: as many as fill the chip twice over in the first pass (a workgroup per CU leaves half of each SIMD's issue slots), at
-// least four chunks each; from four on they win (3 x the work in 2 / segments of the steps).
-static DeltaPlan plan_of(int B, int T, int Hv, int dk, int dv) {
+// Segments: as many as give the first pass two workgroups a CU, at least four chunks each; from four segments on they win (3 x the
+// work in 2 / segments of the steps): 1 x 512 frames, 4 heads of 64, bf16 35 -> 31 us (fp32 54 -> 41), 1 x 3000 161 -> 50 (262 -> 62),
+// 1 x 32768 1641 -> 144 (2726 -> 183).  Where that makes no more than eight, and two workgroups of this kernel share a CU, twice as
+// many: 2 x 4096, 32 heads of 64, bf16 147 -> 134 (fp32 236 -> 212), 4 x 4096, 16 heads of 128, bf16 320 -> 302 (fp32, one a CU, 567
+// -> 585); with more the join, whose steps are one after the other, takes what the passes gain (1 x 32768, 4 heads, 144 -> 199).
+static DeltaPlan plan_of(int B, int T, int Hv, int dk, int dv, bool two) {
     DeltaPlan p = {1, (T + kC - 1) / kC, nullptr, nullptr};
     const long per = (long)B * Hv * ((dv + 63) / 64 + (dk + 63) / 64);
-    const int nchunk = p.len, want = (int)min((long)nchunk / 4, 512 / per);
+    const int nchunk = p.len, want = (int)min((long)nchunk / 4, (two && 512 / per <= 8 ? 1024 : 512) / per);
     if (want >= 4) {
         p.len = (nchunk + want - 1) / want;
         p.nseg = (nchunk + p.len - 1) / p.len;
@@ -704,7 +708,7 @@ static DeltaPlan plan_of(int B, int T, int Hv, int dk, int dv) {
 }
 static size_t prep_floats(int B, int T, int Hv) { return (size_t)B * Hv * ((T + kC - 1) / kC) * (ws_unit(3) / 4); }
 size_t delta_ws_floats(int B, int T, int Hv, int dk, int dv) {
-    return prep_floats(B, T, Hv) + (size_t)B * Hv * (plan_of(B, T, Hv, dk, dv).nseg - 1) * dk * (dk + dv) + 4;
+    return prep_floats(B, T, Hv) + (size_t)B * Hv * (max(plan_of(B, T, Hv, dk, dv, false).nseg, plan_of(B, T, Hv, dk, dv, true).nseg) - 1) * dk * (dk + dv) + 4;
 }
 
 template <class E, int NK, int MODE, bool OUT>
@@ -719,7 +723,7 @@ static bool scan_pass(const DeltaArgs& a, const DeltaPlan& p, hipStream_t s) {
 }
 template <class E, int NK, int MODE>
 static bool scan_for(const DeltaArgs& a, hipStream_t s) {
-    DeltaPlan p = plan_of(a.B, a.T, a.Hv, a.dk, a.dv);
+    DeltaPlan p = plan_of(a.B, a.T, a.Hv, a.dk, a.dv, two_per_cu<E, NK>());
     if (p.nseg > 1) {
         p.N = a.ws + prep_floats(a.B, a.T, a.Hv);
         p.M = p.N + ((size_t)a.B * a.Hv * (p.nseg - 1) * a.dk * a.dv + 3) / 4 * 4;

@@ -107,7 +107,7 @@ def test_delta_rule(ops, shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
-@pytest.mark.parametrize("shape", [(1, 512, 1, 1, 64, 64), (2, 1000, 1, 2, 64, 40), (1, 1400, 1, 1, 128, 130), (1, 530, 1, 1, 200, 20), (3, 777, 1, 1, 7, 5), (1, 3000, 1, 1, 72, 33)], ids=str)
+@pytest.mark.parametrize("shape", [(1, 512, 1, 1, 64, 64), (2, 1000, 1, 2, 64, 40), (1, 1400, 1, 1, 128, 130), (1, 530, 1, 1, 200, 20), (2, 4500, 16, 32, 64, 40), (1, 2100, 8, 16, 100, 128), (3, 777, 1, 1, 7, 5), (1, 3000, 1, 1, 72, 33)], ids=str)
 def test_delta_rule_long_sequences_on_few_heads(ops, shape, dtype):
     """Long enough, and few enough, to be run as segments side by side; ragged: a sequence that ends inside a segment, at a border
     between two, in the first one, and an empty one."""
@@ -317,7 +317,8 @@ def assert_linear(y, want, mag, K, r, bf16):
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("shape", [(1, 1, 1, 1, 1, 1), (1, 1, 60, 256, 3, 8), (5, 1, 132, 96, 2, 4), (130, 1, 64, 65, 40, 16), (3, 40, 100, 70, 2, 5), (2, 129, 256, 300, 4, 32),
-                                   (7, 125, 72, 2, 3, 64), (2, 64, 33, 31, 1, 128), (1, 300, 512, 96, 2, 8), (9, 17, 130, 257, 5, 33)], ids=str)
+                                   (7, 125, 72, 2, 3, 64), (2, 64, 33, 31, 1, 128), (1, 300, 512, 96, 2, 8), (9, 17, 130, 257, 5, 33),
+                                   (130, 1, 600, 65, 40, 16), (300, 2, 64, 40, 5, 8), (3, 40, 600, 70, 2, 5), (280, 45, 200, 70, 3, 9), (100, 129, 96, 33, 3, 64)], ids=str)
 def test_linear_adapted(ops, shape, dtype):
     import torch
     B, T, K, M, n, r = shape
