@@ -278,7 +278,8 @@ int mp_live_form_frames(mp_handle* h, const float* quat_dev, const float* acc_de
  * layers).  Inputs of two types; fp32 accumulation and state in both.  Unlike the network entry points these run on the
  * caller's stream itself and use no memory of the handle: calls on several streams are independent, a call can be captured
  * into the caller's graph (lengths, slots and ids are device memory and read on replay), every kind of handle serves them.
- * They return without waiting.  Replaces: nothing in the reference. */
+ * They return without waiting; an output buffer overlaps an input only where that is said.  Replaces: nothing in the
+ * reference. */
 enum { MP_F32 = 0, MP_BF16 = 1 };
 
 /* Gated delta rule over B ragged sequences: per value head a state S [dk][dv] and per frame

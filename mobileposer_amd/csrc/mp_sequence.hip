@@ -100,7 +100,8 @@ int mp_linear_adapted(mp_handle* h, int dtype, const void* x_dev, const int64_t 
     const size_t need = mp_linear_adapted_workspace(B, T, r);
     if (!ws_dev || ws_bytes < need || (uintptr_t)ws_dev % 16)
         return fail(h, MP_ERR_INVALID, "mp_linear_adapted: workspace of %zu bytes, %zu needed (16-byte aligned)", ws_bytes, need);
-    if ((int64_t)B * T > (int64_t)1 << 30 || (int64_t)B * T * r > (int64_t)kMaxBlocks || ((int64_t)M + 15) / 16 > 65535)
+    if ((int64_t)B * T > (int64_t)1 << 30 || (int64_t)B * T * r > (int64_t)kMaxBlocks || ((int64_t)M + 15) / 16 > 65535 ||
+        ((int64_t)B * T + 31) / 32 * (((int64_t)M + 31) / 32) > kMaxBlocks - 8)
         return fail(h, MP_ERR_INVALID, "mp_linear_adapted: %d x %d rows to %d columns are too many for one call", B, T, M);
     ON_DEVICE(h);
     mpseq::AdaptArgs a;

@@ -568,6 +568,18 @@ def test_block_of_the_model_with_adapters(ops, module, shape, lstm_mode):
         assert np.abs(npy(one[b, :n]) - wy[0, :n]).max() < 1e-4
 
 
+def test_block_of_the_model_with_adapters_that_are_not_there(ops):
+    """An id on the device that is no adapter's: that sequence's outputs are NaN, the others' are what they are without it; the call
+    behind it is untouched."""
+    import torch
+    dev = {k: tuple(t.cuda() for t in v) for k, v in block_adapters("velocity", 2, 4, 8, 33).items()}
+    x = torch.randn(3, 20, 132, generator=torch.Generator().manual_seed(34)).cuda()
+    run = lambda ids: ops.rnn_forward("velocity", x, [20, 15, 20], None, dev, torch.tensor(ids, device="cuda", dtype=torch.int32))[0]
+    want, got, after = run([1, 0, -1]), run([1, 2, -1]), run([1, 0, -1])
+    assert torch.isnan(got[1, :15]).all() and torch.equal(got[0], want[0]) and torch.equal(got[2], want[2])
+    assert torch.equal(after, want)
+
+
 def test_block_of_the_model_with_adapters_refusals(ops):
     import torch
     dev = {k: tuple(t.cuda() for t in v) for k, v in block_adapters("pose", 2, 4, 8, 32).items()}
