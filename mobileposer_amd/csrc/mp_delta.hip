@@ -786,17 +786,19 @@ MP_KERNEL __launch_bounds__(256) void mp_delta_online(DeltaOnlineArgs a, int nti
     // a row of the state that an earlier stream of this call uses, or that is not there: never plausible numbers
     bool refuse = slot >= a.n_slots;
     float* state = a.state + ((size_t)(refuse ? 0 : slot) * a.Hv + hv) * a.dk * a.dv;
+    const E* v = (const E*)a.v + st * a.sv[0] + hv * a.sv[1];      // (requested with the state: a latency less behind the sums)
+    float vc[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) vc[i] = load_f(v + min(c0, a.dv - VEC) + i);
+    const float g = a.g[st * a.sg[0] + hv * a.sg[1]], beta = a.beta[st * a.sb[0] + hv * a.sb[1]];
     float S[NR][VEC];
+    const float* const at = state + min(c0, a.dv - VEC);
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
         const int d = n * rows + rl;
-        if (VEC == 4) {
-            float4 x = {0.f, 0.f, 0.f, 0.f};
-            if (cok && d < a.dk) x = *(const float4*)(state + (size_t)d * a.dv + c0);
-            S[n][0] = x.x; S[n][VEC > 1 ? 1 : 0] = x.y; S[n][VEC > 2 ? 2 : 0] = x.z; S[n][VEC > 3 ? 3 : 0] = x.w;
-        } else {
-            S[n][0] = cok && d < a.dk ? state[(size_t)d * a.dv + c0] : 0.f;
-        }
+        const float* x = at + (size_t)min(d, a.dk - 1) * a.dv;     // (no branch around the load: the rows behind dk are not used)
+        if (VEC == 4) __builtin_memcpy(S[n], __builtin_assume_aligned(x, 16), 16);
+        else S[n][0] = *x;
     }
     if (a.slots) {
         bool twice = false;
@@ -807,7 +809,7 @@ MP_KERNEL __launch_bounds__(256) void mp_delta_online(DeltaOnlineArgs a, int nti
     const E* q = (const E*)a.q + st * a.sq[0] + hk * a.sq[1];
     const E* k = (const E*)a.k + st * a.sk[0] + hk * a.sk[1];
     for (int d = tid; d < a.dk; d += 256) { lk[d] = load_f(k + d); lq[d] = load_f(q + d); }
-    const float eg = expf(a.g[st * a.sg[0] + hv * a.sg[1]]), beta = a.beta[st * a.sb[0] + hv * a.sb[1]];
+    const float eg = expf(g);
     __syncthreads();
     float ak[VEC], aq[VEC];
     for (int i = 0; i < VEC; ++i) ak[i] = aq[i] = 0.f;
@@ -834,7 +836,6 @@ MP_KERNEL __launch_bounds__(256) void mp_delta_online(DeltaOnlineArgs a, int nti
     __syncthreads();
     if (!cok) return;
     float u[VEC];
-    const E* v = (const E*)a.v + st * a.sv[0] + hv * a.sv[1];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
         float sk = 0.f, sq = 0.f;
@@ -842,7 +843,7 @@ MP_KERNEL __launch_bounds__(256) void mp_delta_online(DeltaOnlineArgs a, int nti
             sk += part[(w * 2 + 0) * cw + cl * VEC + i];
             sq += part[(w * 2 + 1) * cw + cl * VEC + i];
         }
-        u[i] = beta * (load_f(v + c0 + i) - eg * sk);
+        u[i] = beta * (vc[i] - eg * sk);
         if (rl == 0) store_f(o + c0 + i, refuse ? __builtin_nanf("") : a.scale * (eg * sq + kq * u[i]));
     }
     if (refuse) return;
