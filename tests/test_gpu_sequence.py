@@ -238,7 +238,7 @@ def test_delta_rule_empty(ops):
 
 # ---------------------------------------------------------------- ticks
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
-@pytest.mark.parametrize("shape", [(1, 1, 1, 1, 1), (3, 1, 2, 16, 16), (5, 2, 4, 64, 64), (4, 1, 1, 128, 128), (3, 3, 3, 96, 41), (2, 1, 2, 256, 36),
+@pytest.mark.parametrize("shape", [(1, 1, 1, 1, 1), (3, 1, 2, 16, 16), (5, 2, 4, 64, 64), (4, 1, 1, 128, 128), (3, 3, 3, 96, 41), (2, 1, 2, 256, 36), (2, 1, 1, 256, 41), (2, 1, 1, 129, 50), (3, 1, 2, 128, 63), (2, 1, 1, 128, 129),
                                    (2, 1, 1, 33, 260), (70, 2, 2, 20, 12)], ids=str)
 def test_delta_rule_online(ops, shape, dtype):
     import torch
