@@ -621,13 +621,14 @@ MP_KERNEL __launch_bounds__(256, (two_per_cu<E, NK>() ? 2 : 1)) void mp_delta_sc
 }
 
 // The start of every segment: S_{s+1} = M_s S_s + N_s, in place of N_s.  A workgroup per (sequence, value head, 16 columns), a wave
-// per 16 rows (two for dk > 128), on the fp32 matrix instructions; S_s goes round through LDS, M of the next segment is on its way
-// while this one is multiplied.  KT = dk / 16 rounded up; VEC: dk is a multiple of 4 (rows of M in 16-byte pieces).
+// per 16 rows (two for dk > 128), on the fp32 matrix instructions; S_s goes round through LDS (by columns: a lane's four rows are one
+// piece; two buffers, one barrier a step), M of the next segment is on its way while this one is multiplied.  KT = dk / 16 rounded
+// up; VEC: dk is a multiple of 4 (rows of M in 16-byte pieces).
 template <int KT, bool VEC>
-MP_KERNEL __launch_bounds__(512) void mp_delta_join(DeltaArgs a, DeltaPlan plan, int ncol) {
-    constexpr int NT = (KT + 7) / 8;
+MP_KERNEL __launch_bounds__(KT <= 4 ? 256 : 512) void mp_delta_join(DeltaArgs a, DeltaPlan plan, int ncol) {
+    constexpr int NT = (KT + 7) / 8, TH = KT <= 4 ? 256 : 512;
     constexpr bool kAhead = KT <= 8;              // (both would not fit the registers)
-    __shared__ float St[16 * KT][17];
+    __shared__ __align__(16) float St[2][16][16 * KT + 4];        // [column][row]
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, grp = lane >> 4, wave = tid >> 6;
     const int head = blockIdx.x % (a.B * a.Hv), ct = blockIdx.x / (a.B * a.Hv), b = head / a.Hv;      // (a head's workgroups, which read the same M, on one XCD
                                                                                                     //  where the heads are a multiple of 8)
@@ -637,7 +638,10 @@ MP_KERNEL __launch_bounds__(512) void mp_delta_join(DeltaArgs a, DeltaPlan plan,
     float* N = plan.N + (size_t)head * (plan.nseg - 1) * a.dk * a.dv;
     const float* M = plan.M + (size_t)head * (plan.nseg - 1) * a.dk * a.dk;
     if (n < 2) return;
-    for (int d = tid >> 4; d < 16 * KT; d += 32) St[d][tid & 15] = d < a.dk ? N[(size_t)d * a.dv + min(16 * ct + (tid & 15), a.dv - 1)] : 0.f;
+    for (int d = tid >> 4; d < 16 * KT; d += TH / 16) {
+        St[0][tid & 15][d] = d < a.dk ? N[(size_t)d * a.dv + min(16 * ct + (tid & 15), a.dv - 1)] : 0.f;
+        St[1][tid & 15][d] = 0.f;
+    }
     float4 m[NT][KT], mn[kAhead ? NT : 1][kAhead ? KT : 1];
     f32x4 acc[NT], an[NT];
     auto fetch = [&](int s, auto& mn) {
@@ -670,24 +674,32 @@ MP_KERNEL __launch_bounds__(512) void mp_delta_join(DeltaArgs a, DeltaPlan plan,
             fetch(min(s + 1, n - 1), mn);
         }
         __syncthreads();
+        const float (*const from)[16 * KT + 4] = St[(s - 1) & 1];
+        float (*const to)[16 * KT + 4] = St[s & 1];
+        f32x4 odd[NT] = {};                                       // (a second chain of sums: a product does not wait for the one before it)
 #pragma unroll
         for (int k = 0; k < KT; ++k) {
-            const int d = 16 * k + 4 * grp;
-            const float4 x = {St[d][col], St[d + 1][col], St[d + 2][col], St[d + 3][col]};      // (zeros behind dk)
+            const float4 x = *(const float4*)&from[col][16 * k + 4 * grp];      // (zeros behind dk)
 #pragma unroll
-            for (int t = 0; t < NT; ++t) acc[t] = mfma4(m[t][k], x, acc[t]);
+            for (int t = 0; t < NT; ++t) {
+                if (k & 1) odd[t] = mfma4(m[t][k], x, odd[t]);
+                else acc[t] = mfma4(m[t][k], x, acc[t]);
+            }
         }
-        __syncthreads();
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int t = 0; t < NT; ++t) {
+            acc[t] += odd[t];
+            const int d0 = 16 * (wave + 8 * t) + 4 * grp;
+            if (d0 + 4 <= a.dk) *(float4*)&to[col][d0] = {acc[t][0], acc[t][1], acc[t][2], acc[t][3]};
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int d = 16 * (wave + 8 * t) + 4 * grp + r;
+                const int d = d0 + r;
                 if (d < a.dk) {
-                    St[d][col] = acc[t][r];
+                    if (d0 + 4 > a.dk) to[col][d] = acc[t][r];
                     if (cv < a.dv) N[((size_t)s * a.dk + d) * a.dv + cv] = acc[t][r];
                 }
             }
+        }
     }
 }
 
@@ -731,11 +743,11 @@ static bool scan_for(const DeltaArgs& a, hipStream_t s) {
         const int ncol = (a.dv + 15) / 16;
         const dim3 grid((unsigned)(a.B * a.Hv * ncol));
         if (a.dk % 4) {
-            if (a.dk <= 64) hipLaunchKernelGGL((mp_delta_join<4, false>), grid, dim3(512), 0, s, a, p, ncol);
+            if (a.dk <= 64) hipLaunchKernelGGL((mp_delta_join<4, false>), grid, dim3(256), 0, s, a, p, ncol);
             else if (a.dk <= 128) hipLaunchKernelGGL((mp_delta_join<8, false>), grid, dim3(512), 0, s, a, p, ncol);
             else hipLaunchKernelGGL((mp_delta_join<16, false>), grid, dim3(512), 0, s, a, p, ncol);
         } else {
-            if (a.dk <= 64) hipLaunchKernelGGL((mp_delta_join<4, true>), grid, dim3(512), 0, s, a, p, ncol);
+            if (a.dk <= 64) hipLaunchKernelGGL((mp_delta_join<4, true>), grid, dim3(256), 0, s, a, p, ncol);
             else if (a.dk <= 128) hipLaunchKernelGGL((mp_delta_join<8, true>), grid, dim3(512), 0, s, a, p, ncol);
             else hipLaunchKernelGGL((mp_delta_join<16, true>), grid, dim3(512), 0, s, a, p, ncol);
         }
