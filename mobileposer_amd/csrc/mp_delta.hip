@@ -622,7 +622,8 @@ MP_KERNEL __launch_bounds__(256, (two_per_cu<E, NK>() ? 2 : 1)) void mp_delta_sc
 
 // The start of every segment: S_{s+1} = M_s S_s + N_s, in place of N_s.  A workgroup per (sequence, value head, 16 columns), a wave
 // per 16 rows (two for dk > 128), on the fp32 matrix instructions; S_s goes round through LDS (by columns: a lane's four rows are one
-// piece; two buffers, one barrier a step), M of the next segment is on its way while this one is multiplied.  KT = dk / 16 rounded
+// piece; two buffers, one barrier a step), M of the next two segments is on its
+// way while one is multiplied.  KT = dk / 16 rounded
 // up; VEC: dk is a multiple of 4 (rows of M in 16-byte pieces).
 template <int KT, bool VEC>
 MP_KERNEL __launch_bounds__(KT <= 4 ? 256 : 512) void mp_delta_join(DeltaArgs a, DeltaPlan plan, int ncol) {
@@ -642,9 +643,9 @@ MP_KERNEL __launch_bounds__(KT <= 4 ? 256 : 512) void mp_delta_join(DeltaArgs a,
         St[0][tid & 15][d] = d < a.dk ? N[(size_t)d * a.dv + min(16 * ct + (tid & 15), a.dv - 1)] : 0.f;
         St[1][tid & 15][d] = 0.f;
     }
-    float4 m[NT][KT], mn[kAhead ? NT : 1][kAhead ? KT : 1];
-    f32x4 acc[NT], an[NT];
-    auto fetch = [&](int s, auto& mn) {
+    float4 m[kAhead ? 2 : 1][NT][KT];
+    f32x4 an[kAhead ? 2 : 1][NT];
+    auto fetch = [&](int s, float4 (&mn)[NT][KT], f32x4 (&nn)[NT]) {
         const float* Ms = M + (size_t)s * a.dk * a.dk;
         const float* Ns = N + (size_t)s * a.dk * a.dv;
 #pragma unroll
@@ -658,47 +659,52 @@ MP_KERNEL __launch_bounds__(KT <= 4 ? 256 : 512) void mp_delta_join(DeltaArgs a,
                 else mn[t][k] = {p[min(d, a.dk - 1)], p[min(d + 1, a.dk - 1)], p[min(d + 2, a.dk - 1)], p[min(d + 3, a.dk - 1)]};
             }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) an[t][r] = Ns[(size_t)min(16 * (wave + 8 * t) + 4 * grp + r, a.dk - 1) * a.dv + cc];
+            for (int r = 0; r < 4; ++r) nn[t][r] = Ns[(size_t)min(16 * (wave + 8 * t) + 4 * grp + r, a.dk - 1) * a.dv + cc];
         }
     };
-    if constexpr (kAhead) fetch(1, mn);
-    for (int s = 1; s < n; ++s) {
-        if constexpr (!kAhead) fetch(s, m);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) acc[t] = an[t];
-        if constexpr (kAhead) {
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int k = 0; k < KT; ++k) m[t][k] = mn[t][k];
-            fetch(min(s + 1, n - 1), mn);
-        }
+    auto step = [&](int s, float4 (&ms)[NT][KT], f32x4 (&acc)[NT]) {
         __syncthreads();
         const float (*const from)[16 * KT + 4] = St[(s - 1) & 1];
         float (*const to)[16 * KT + 4] = St[s & 1];
+        float4 x[KT];
+#pragma unroll
+        for (int k = 0; k < KT; ++k) x[k] = *(const float4*)&from[col][16 * k + 4 * grp];      // (zeros behind dk)
         f32x4 odd[NT] = {};                                       // (a second chain of sums: a product does not wait for the one before it)
 #pragma unroll
-        for (int k = 0; k < KT; ++k) {
-            const float4 x = *(const float4*)&from[col][16 * k + 4 * grp];      // (zeros behind dk)
+        for (int k = 0; k < KT; ++k)
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                if (k & 1) odd[t] = mfma4(m[t][k], x, odd[t]);
-                else acc[t] = mfma4(m[t][k], x, acc[t]);
+                if (k & 1) odd[t] = mfma4(ms[t][k], x[k], odd[t]);
+                else acc[t] = mfma4(ms[t][k], x[k], acc[t]);
             }
-        }
+        // (no branches: what a lane has behind the last row or column is that row's or column's value once more)
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             acc[t] += odd[t];
-            const int d0 = 16 * (wave + 8 * t) + 4 * grp;
-            if (d0 + 4 <= a.dk) *(float4*)&to[col][d0] = {acc[t][0], acc[t][1], acc[t][2], acc[t][3]};
+            const int d = 16 * (wave + 8 * t) + 4 * grp;
+            if (16 * (wave + 8 * t) < 16 * KT)
+                *(float4*)&to[col][d] = {d < a.dk ? acc[t][0] : 0.f, d + 1 < a.dk ? acc[t][1] : 0.f, d + 2 < a.dk ? acc[t][2] : 0.f, d + 3 < a.dk ? acc[t][3] : 0.f};
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int d = d0 + r;
-                if (d < a.dk) {
-                    if (d0 + 4 > a.dk) to[col][d] = acc[t][r];
-                    if (cv < a.dv) N[((size_t)s * a.dk + d) * a.dv + cv] = acc[t][r];
-                }
-            }
+            for (int r = 0; r < 4; ++r) N[((size_t)s * a.dk + min(d + r, a.dk - 1)) * a.dv + cc] = acc[t][r];
+        }
+    };
+    if constexpr (kAhead) {
+        fetch(1, m[0], an[0]);
+        __builtin_amdgcn_sched_barrier(0);                        // (in this order: the loop waits for as many as are older)
+        fetch(min(2, n - 1), m[1], an[1]);
+        __builtin_amdgcn_sched_barrier(0);
+        int s = 1;
+        for (; s + 1 < n; s += 2) {
+            step(s, m[0], an[0]);
+            fetch(min(s + 2, n - 1), m[0], an[0]);
+            step(s + 1, m[1], an[1]);
+            fetch(min(s + 3, n - 1), m[1], an[1]);
+        }
+        if (s < n) step(s, m[0], an[0]);
+    } else {
+        for (int s = 1; s < n; ++s) {
+            fetch(s, m[0], an[0]);
+            step(s, m[0], an[0]);
         }
     }
 }
