@@ -319,6 +319,12 @@ struct Rows {                                     // what a thread stages of a c
                 }
             }
         }
+        // what a branch above left unused: its registers would have to be waited for at the loop's top, behind the stores of the outputs
+#pragma unroll
+        for (int n = 0; n < NW; ++n) asm volatile("" ::"v"(ws[n]));
+        v.arrived();
+#pragma unroll
+        for (int n = 0; n < NF; ++n) { k[n].arrived(); q[n].arrived(); }
     }
 };
 // Left to itself the compiler puts every LDS read in front of its use, and a lone wave waits for each.  (fp32: the operands of a

@@ -21,6 +21,7 @@ template <class E> struct Oct;
 template <> struct Oct<bf16raw> {
     u32x4 v;
     __device__ __forceinline__ void zero() { v = (u32x4){0, 0, 0, 0}; }
+    __device__ __forceinline__ void arrived() const { asm volatile("" ::"v"(v)); }      // no load of it is in flight behind this
     __device__ __forceinline__ void load(const bf16raw* p) { __builtin_memcpy(&v, p, 16); }
     __device__ __forceinline__ void load_guarded(const bf16raw* p, int n) {
         bf16raw t[8];
@@ -70,6 +71,7 @@ static __device__ __forceinline__ unsigned take_bf16(float& a, float& b) {
 template <> struct Oct<float> {
     float v[8];
     __device__ __forceinline__ void zero() { for (int i = 0; i < 8; ++i) v[i] = 0.f; }
+    __device__ __forceinline__ void arrived() const { for (int i = 0; i < 8; ++i) asm volatile("" ::"v"(v[i])); }
     __device__ __forceinline__ void load(const float* p) { __builtin_memcpy(v, p, 32); }
     __device__ __forceinline__ void load_guarded(const float* p, int n) {
         for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : 0.f;
