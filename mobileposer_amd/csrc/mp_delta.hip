@@ -79,7 +79,8 @@ static __device__ __forceinline__ double lane_below(double x) {
 // One wave per (sequence, key head, chunk): K K^T and Q K^T once, then the value heads that share the key head.
 // (I + A)^{-1} by forward substitution on the two 16 x 16 diagonal blocks -- a lane of two groups of 16 solves a column; stable
 // where keys repeat and A is far from small, products of powers of A are not -- and T21 = -T22 A21 T11 on the fp32 matrix
-// instructions.  KB: steps of 32 components whose loads are in flight together.
+// instructions.  KB: steps of 32 components whose loads are in flight together.  Bound by memory, its own output being the larger part:
+// 8 x 2048 frames, 8 / 16 heads of 128, bf16 34 us (4.5 TB/s), 256 x 125 frames, 4 heads of 64, fp32 22 us.
 template <class E, int PO, int MODE, int KB>
 MP_KERNEL __launch_bounds__(64) void mp_delta_prep(DeltaArgs a) {
     constexpr int P = Arith<E>::P, LS = kC + 4;
@@ -244,6 +245,9 @@ MP_KERNEL __launch_bounds__(64) void mp_delta_prep(DeltaArgs a) {
 // rounded up.  The workgroup stages a chunk in LDS -- K and Q as ready operands (bf16 terms, one 16-byte read per lane and operand;
 // K^T comes from K's operands by the turning reads), the chunk's workspace, the 64 columns of V, whose place the outputs take --
 // and the next chunk is on its way through registers meanwhile, with no use of its values before this chunk's products are done.
+// Bound by the chain of a chunk -- products with S, U, products with U, the new S split into terms again -- whose steps overlap between
+// waves only: 8 x 2048 frames, 16 heads of 128, bf16 153 us, 2.4 us a chunk, the matrix units busy 18 % of it; 256 x 125, 4 heads of 64,
+// fp32 48 us.  Two waves per 16 columns (each half of dk) took as long: what they share goes through LDS once more.
 constexpr int kFragK = kFrag + 256;               // K's operands: 64 bytes between the groups of eight components, or the 16 lanes of a
                                                   // turning read would meet in a quarter of the banks
 template <class E, int NK>
@@ -628,9 +632,9 @@ MP_KERNEL __launch_bounds__(256, (two_per_cu<E, NK>() ? 2 : 1)) void mp_delta_sc
 
 // The start of every segment: S_{s+1} = M_s S_s + N_s, in place of N_s.  A workgroup per (sequence, value head, 16 columns), a wave
 // per 16 rows (two for dk > 128), on the fp32 matrix instructions; S_s goes round through LDS (by columns: a lane's four rows are one
-// piece; two buffers, one barrier a step), M of the next two segments is on its
-// way while one is multiplied.  KT = dk / 16 rounded
-// up; VEC: dk is a multiple of 4 (rows of M in 16-byte pieces).
+// piece; two buffers, one barrier a step), M of the next two segments is on its way while one is multiplied.  A step is 0.6 us at
+// dk = 64 and 2.6 at 128, where it reads 64 KB of M.  KT = dk / 16 rounded up; VEC: dk is a multiple of 4 (rows of M in 16-byte
+// pieces).
 template <int KT, bool VEC>
 MP_KERNEL __launch_bounds__(KT <= 4 ? 256 : 512) void mp_delta_join(DeltaArgs a, DeltaPlan plan, int ncol) {
     constexpr int NT = (KT + 7) / 8, TH = KT <= 4 ? 256 : 512;
@@ -791,7 +795,8 @@ bool launch_delta(const DeltaArgs& a, int dtype, hipStream_t s) {
 // ---------------------------------------------------------------- one frame per stream
 // A workgroup owns (stream, value head, tile of columns): its part of the state is read once into registers -- a thread holds
 // VEC columns of NR rows --, S^T k and S^T q are reduced together (o = e^g S^T q + (k . q) u needs no second pass), and the updated
-// state is written once.  HBM-bound: 8 dk dv bytes per stream and head.
+// state is written once.  HBM-bound: 8 dk dv bytes per stream and head (512 streams, 16 heads of 128 x 128: 217 us, 4.98 TB/s; a copy
+// reaches 5.08).
 template <class E, int VEC, int NR>
 MP_KERNEL __launch_bounds__(256) void mp_delta_online(DeltaOnlineArgs a, int ntile, int log_lanes) {
     extern __shared__ float tick_lds[];               // k [dk] | q [dk] | partial sums [4 waves][2][lanes * VEC]
