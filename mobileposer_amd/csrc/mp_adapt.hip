@@ -14,61 +14,71 @@ namespace mpseq {
 size_t adapt_ws_floats(int B, int T, int r) { return (size_t)B * T * r; }
 
 // ---------------------------------------------------------------- z = scale Down x
-// A workgroup takes up to 16 frames of one sequence -- one adapter, so the product runs on the matrix units even where the 16 rows
+// A workgroup takes up to 16 RG frames of one sequence -- one adapter, so the product runs on the matrix units even where the rows
 // are one (a tick: the reads of Down bound it either way) --, K split over the four waves and joined through LDS; KB steps of
 // every wave are in flight together.  RT = r / 16 rounded up.  Bound by the latency of one pass for a tick (512 x 1, 1024, r 16: 6 us), by
-// the reads of x and Down together for long sequences (8 x 2048, 2048, r 32: 25 us, 67 MB of x and 134 MB of Down, that from L2).
-template <class E, int RT>
+// the reads of x and Down together for long sequences (8 x 2048, 2048, r 32: 18 us, 67 MB of x and as many of Down, those from L2).
+template <class E, int RT, int RG>
 MP_KERNEL __launch_bounds__(256) void mp_adapt_down(AdaptArgs a, int per_seq) {
-    constexpr int P = Arith<E>::P, KB = RT >= 4 ? 2 : 4;
-    __shared__ float part[4][16 * RT][17];
+    constexpr int P = Arith<E>::P, KB = RT >= 4 ? 2 : 4, NR = 16 * RG;
+    __shared__ float part[4][16 * RT][NR + 1];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 15, grp = lane >> 4;
-    const int b = blockIdx.x / per_seq, t0 = blockIdx.x % per_seq * 16, id = a.ids[b];
+    const int b = blockIdx.x / per_seq, t0 = blockIdx.x % per_seq * NR, id = a.ids[b];
     if (id < 0 || id >= a.n) return;                              // (the second launch reads no z of such rows)
-    const int t = t0 + col < a.T ? t0 + col : a.T - 1;
-    const E* x = (const E*)a.x + (size_t)b * a.sx[0] + (size_t)t * a.sx[1];
+    const E* x[RG];
+#pragma unroll
+    for (int g = 0; g < RG; ++g) x[g] = (const E*)a.x + (size_t)b * a.sx[0] + (size_t)min(t0 + 16 * g + col, a.T - 1) * a.sx[1];
     const E* d[RT];
 #pragma unroll
     for (int j = 0; j < RT; ++j) d[j] = (const E*)a.down + ((size_t)id * a.r + min(16 * j + col, a.r - 1)) * a.K;
-    f32x4 acc[RT] = {};
+    f32x4 acc[RG][RT] = {};
     int k = (wave * 4 + grp) * 8;
     for (; k - grp * 8 + 128 * (KB - 1) + 32 <= a.K; k += 128 * KB) {
-        Oct<E> ox[KB], od[KB][RT];
+        Oct<E> ox[KB][RG], od[KB][RT];
 #pragma unroll
         for (int m = 0; m < KB; ++m) {
-            ox[m].load(x + k + 128 * m);
+#pragma unroll
+            for (int g = 0; g < RG; ++g) ox[m][g].load(x[g] + k + 128 * m);
 #pragma unroll
             for (int j = 0; j < RT; ++j) od[m][j].load(d[j] + k + 128 * m);
         }
 #pragma unroll
         for (int m = 0; m < KB; ++m) {
             u32x4 px[P], pd[RT][P];
-            ox[m].planes(px);
 #pragma unroll
             for (int j = 0; j < RT; ++j) od[m][j].planes(pd[j]);
-            mfma_planes_n<RT, P, P>(pd, px, acc);
+#pragma unroll
+            for (int g = 0; g < RG; ++g) {
+                ox[m][g].planes(px);
+                mfma_planes_n<RT, P, P>(pd, px, acc[g]);
+            }
         }
     }
     for (; k - grp * 8 < a.K; k += 128) {
         const int left = a.K - k < 0 ? 0 : a.K - k;
         Oct<E> ox, od;
         u32x4 px[P], pd[RT][P];
-        ox.load_some(x + k, left);
-        ox.planes(px);
 #pragma unroll
         for (int j = 0; j < RT; ++j) {
             od.load_some(d[j] + k, left);
             od.planes(pd[j]);
         }
-        mfma_planes_n<RT, P, P>(pd, px, acc);
+#pragma unroll
+        for (int g = 0; g < RG; ++g) {
+            ox.load_some(x[g] + k, left);
+            ox.planes(px);
+            mfma_planes_n<RT, P, P>(pd, px, acc[g]);
+        }
     }
 #pragma unroll
-    for (int j = 0; j < RT; ++j)
+    for (int g = 0; g < RG; ++g)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) part[wave][16 * j + 4 * grp + r][col] = acc[j][r];      // [component][row]
+        for (int j = 0; j < RT; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) part[wave][16 * j + 4 * grp + r][16 * g + col] = acc[g][j][r];      // [component][row]
     __syncthreads();
     const float sc = a.scale ? a.scale[id] : 1.f;
-    for (int i = tid; i < 16 * a.r; i += 256) {
+    for (int i = tid; i < NR * a.r; i += 256) {
         const int row = i / a.r, c = i % a.r;
         if (t0 + row < a.T) a.ws[((size_t)b * a.T + t0 + row) * a.r + c] = sc * ((part[0][c][row] + part[1][c][row]) + (part[2][c][row] + part[3][c][row]));
     }
@@ -438,7 +448,7 @@ static bool gemm_for(const AdaptArgs& a, int rows, hipStream_t s) {
 template <class E>
 static bool launch_for(AdaptArgs a, hipStream_t s) {
     constexpr bool half = Arith<E>::P == 1;
-    const int rows = a.B * a.T, per_seq = (a.T + 15) / 16;
+    const int rows = a.B * a.T;
     auto whole = [&](int n) { return a.M % n == 0 && a.sy[0] % n == 0 && a.sy[1] % n == 0 && (uintptr_t)a.y % (n * sizeof(E)) == 0; };
     a.vec = whole(16 / sizeof(E)) ? 2 : whole(4) ? 1 : 0;
     bool ok;
@@ -453,11 +463,18 @@ static bool launch_for(AdaptArgs a, hipStream_t s) {
         ok = gemm_for<E, 4, 2, 2, 4, half ? 64 : 32, true, true>(a, rows, s);
         return hipGetLastError() == hipSuccess && ok;
     }
-    const dim3 grid((unsigned)(a.B * per_seq));
-    if (a.r <= 16) hipLaunchKernelGGL((mp_adapt_down<E, 1>), grid, dim3(256), 0, s, a, per_seq);
-    else if (a.r <= 32) hipLaunchKernelGGL((mp_adapt_down<E, 2>), grid, dim3(256), 0, s, a, per_seq);
-    else if (a.r <= 64) hipLaunchKernelGGL((mp_adapt_down<E, 4>), grid, dim3(256), 0, s, a, per_seq);
-    else hipLaunchKernelGGL((mp_adapt_down<E, 8>), grid, dim3(256), 0, s, a, per_seq);
+    auto down = [&](auto groups) {
+        constexpr int RG = decltype(groups)::value;
+        const int per_seq = (a.T + 16 * RG - 1) / (16 * RG);
+        const dim3 grid((unsigned)(a.B * per_seq));
+        if (a.r <= 16) hipLaunchKernelGGL((mp_adapt_down<E, 1, RG>), grid, dim3(256), 0, s, a, per_seq);
+        else if (a.r <= 32) hipLaunchKernelGGL((mp_adapt_down<E, 2, RG>), grid, dim3(256), 0, s, a, per_seq);
+        else if (a.r <= 64) hipLaunchKernelGGL((mp_adapt_down<E, 4, 1>), dim3((unsigned)(a.B * ((a.T + 15) / 16))), dim3(256), 0, s, a, (a.T + 15) / 16);
+        else hipLaunchKernelGGL((mp_adapt_down<E, 8, 1>), dim3((unsigned)(a.B * ((a.T + 15) / 16))), dim3(256), 0, s, a, (a.T + 15) / 16);
+    };
+    // long sequences that fill the chip with groups of 32 frames read Down half as often (8 x 2048, K 2048, r 32: 18 us against 25)
+    if (a.T >= 64 && rows >= 8192) down(std::integral_constant<int, 2>{});
+    else down(std::integral_constant<int, 1>{});
     // The largest tile that leaves enough of them for 256 CUs (us, K = 1024, larger / smaller tile).  256: bf16 6144 x 2048 (192 tiles)
     // 43 / 58, 4096 x 2048 (128) 41 / 36.  128: bf16 4096 x 2048 (512) 37 / 44, 4096 x 1024 (256) 32 / 28; fp32, whose products take
     // three times as long, 4096 x 1024 (256) 60 / 76, 2048 x 1024 (128) 57 / 47.  64: 1024 x 1024 (256) bf16 15.9 / 16.2, fp32 38 / 39,

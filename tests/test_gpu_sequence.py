@@ -318,7 +318,8 @@ def assert_linear(y, want, mag, K, r, bf16):
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("shape", [(1, 1, 1, 1, 1, 1), (1, 1, 60, 256, 3, 8), (5, 1, 132, 96, 2, 4), (130, 1, 64, 65, 40, 16), (3, 40, 100, 70, 2, 5), (2, 129, 256, 300, 4, 32),
                                    (7, 125, 72, 2, 3, 64), (2, 64, 33, 31, 1, 128), (1, 300, 512, 96, 2, 8), (9, 17, 130, 257, 5, 33),
-                                   (130, 1, 600, 65, 40, 16), (300, 2, 64, 40, 5, 8), (3, 40, 600, 70, 2, 5), (280, 45, 200, 70, 3, 9), (100, 129, 96, 33, 3, 64)], ids=str)
+                                   (130, 1, 600, 65, 40, 16), (300, 2, 64, 40, 5, 8), (3, 40, 600, 70, 2, 5), (280, 45, 200, 70, 3, 9), (100, 129, 96, 33, 3, 64), (4, 2100, 70, 200, 3, 20),
+                                   (2, 4100, 33, 150, 2, 40)], ids=str)
 def test_linear_adapted(ops, shape, dtype):
     import torch
     B, T, K, M, n, r = shape
