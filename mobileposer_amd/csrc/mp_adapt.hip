@@ -96,7 +96,7 @@ MP_KERNEL __launch_bounds__(256) void mp_adapt_down(AdaptArgs a, int per_seq) {
 // whole cache lines): tiles go from memory to LDS without registers, 8 rows x 128 bytes a wave and instruction, the pieces of a row
 // exchanged by its index; the fragments are read between the products.  8 x 2048, 2048 -> 2048, r 32: 126 us, 1090 TFLOP/s (the
 // library's product: 1180), 1.35 us per step of K beside 0.85 of products alone, 18 us for loads before and stores behind;
-// 256 x 125, 512 -> 96, r 8, fp32 (FUSED): 30 us, 2.7 TB/s.
+// 256 x 125, 512 -> 96, r 8, fp32 (FUSED): 29 us, 2.8 TB/s, 1.4 us per step of K beside 0.64 of products alone (LDS and splitting the rest).
 template <class E, int WR, int WC, int MR, int MC, int BK, bool TWO, bool FUSED, bool DIRECT>
 struct Gemm {
     static constexpr int P = Arith<E>::P, KS = BK / 32, RN = 16 * MR * WR, CM = 16 * MC * WC, TH = 64 * WR * WC;
@@ -154,7 +154,7 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
     auto piece = [&](const char* from, int p, int tile, int ks) {
         return *(const u32x4*)(DIRECT ? from + tile * 2048 + mine + (ks * 4 + grp ^ col >> 1) * 16 : from + p * G::kPlane + (tile * KS + ks) * 1024 + mine);
     };
-    auto stage = [&](char* to) {
+    auto stage_from = [&](Oct<E> (&oct)[NU], char* to) {
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
             u32x4 p[P];
@@ -163,6 +163,7 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
             for (int i = 0; i < P; ++i) *(u32x4*)(to + i * G::kPlane + at[u]) = p[i];
         }
     };
+    auto stage = [&](char* to) { stage_from(oct, to); };
     auto multiply = [&](const char* from) {
         if constexpr (DIRECT) {
             u32x4 fw[KS][MC][1], fx[KS][MR][1];
@@ -211,10 +212,11 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
     constexpr bool kEarly = MR == 1;
     int id[MR];
     auto early = [&]() { id[0] = a.ids[min(n0 + wr * 16 + col, n1 - 1) / a.T]; };
-    auto fetch = [&](int t) {
+    auto fetch_to = [&](Oct<E> (&oct)[NU], int t) {
 #pragma unroll
         for (int u = 0; u < NU; ++u) oct[u].load_runs(src[u] + (size_t)t * BK, BK / 2);
     };
+    auto fetch = [&](int t) { fetch_to(oct, t); };
     char* const other = gemm_lds + (TWO ? G::kOne : 0);
     if constexpr (DIRECT) {
         auto ask = [&](int t, char* to) {
@@ -259,27 +261,53 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
             __syncthreads();
         }
     } else {
-    if (whole) {
-        fetch(0);
-        stage(gemm_lds);
-        __syncthreads();
-    }
-    for (int t = 0; t < whole; ++t) {
-        fetch(min(t + 1, whole - 1));
-        multiply(t & 1 ? other : gemm_lds);
-        if (!TWO) __syncthreads();
-        stage(t & 1 ? gemm_lds : other);
-        __syncthreads();
-    }
-    if (whole * BK < a.K) {
+        if constexpr (FUSED) {
+            // one workgroup a CU, and a tile's products are shorter than its loads' way: two tiles are on theirs
+            Oct<E> far[NU];
+            if (whole) {
+                fetch(0);
+                __builtin_amdgcn_sched_barrier(0);                // (in this order: the loop waits for as many as are older)
+                fetch_to(far, min(1, whole - 1));
+                __builtin_amdgcn_sched_barrier(0);
+                stage(gemm_lds);
+                __syncthreads();
+            }
+            int t = 0;
+            for (; t + 1 < whole; t += 2) {
+                fetch(min(t + 2, whole - 1));
+                multiply(gemm_lds);
+                stage_from(far, other);
+                __syncthreads();
+                fetch_to(far, min(t + 3, whole - 1));
+                multiply(other);
+                stage(gemm_lds);
+                __syncthreads();
+            }
+            if (t < whole) multiply(gemm_lds);
+            __syncthreads();
+        } else {
+            if (whole) {
+                fetch(0);
+                stage(gemm_lds);
+                __syncthreads();
+            }
+            for (int t = 0; t < whole; ++t) {
+                fetch(min(t + 1, whole - 1));
+                multiply(t & 1 ? other : gemm_lds);
+                if (!TWO) __syncthreads();
+                stage(t & 1 ? gemm_lds : other);
+                __syncthreads();
+            }
+        }
+        if (whole * BK < a.K) {
 #pragma unroll
-        for (int u = 0; u < NU; ++u)
-            oct[u].load_some_runs(src[u] + (size_t)whole * BK, BK / 2, a.K - whole * BK - (tid + TH * u) % UR * RUN);
-        stage(gemm_lds);                                          // (nobody reads either buffer here: a barrier ended the last round)
-        __syncthreads();
-        multiply(gemm_lds);
-        __syncthreads();
-    }
+            for (int u = 0; u < NU; ++u)
+                oct[u].load_some_runs(src[u] + (size_t)whole * BK, BK / 2, a.K - whole * BK - (tid + TH * u) % UR * RUN);
+            stage(gemm_lds);                                      // (nobody reads either buffer here: a barrier ended the last round)
+            __syncthreads();
+            multiply(gemm_lds);
+            __syncthreads();
+        }
     }
     const int rlen = a.r;
     float* zl = (float*)gemm_lds;                                 // FUSED: [RN][kRowZ]
