@@ -136,7 +136,9 @@ def arm_watchdog(seconds, rank, n_gpus):
             pass
         os._exit(3)
 
-    t = threading.Timer(seconds, bail, args=("bench.py: no result after %d s (--timeout): a rank hung or died" % seconds,))
+    # the other ranks give rank 0 five seconds to print: a rank that leaves first closes its connections, and rank 0 ends in the
+    # collective's own error, without a line
+    t = threading.Timer(seconds + (0 if rank == 0 else 5), bail, args=("bench.py: no result after %d s (--timeout): a rank hung or died" % seconds,))
     t.daemon = True
     why_term = "bench.py: terminated by the launcher (another rank failed?)"
     try:
