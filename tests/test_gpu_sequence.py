@@ -599,3 +599,43 @@ def test_block_of_the_model_with_adapters_refusals(ops):
             run(dev, [0, 1])
     finally:
         ops.set_lstm_mode(1)
+
+
+def test_foot_contact_block_with_adapters_in_the_split_mode(ops):
+    """Mode 3 concerns the H = 256 blocks only: the H = 64 block takes adapters there and gives what it gives in mode 1."""
+    import torch
+    dev = {k: tuple(t.cuda() for t in v) for k, v in block_adapters("foot_contact", 2, 4, 8, 35).items()}
+    x = torch.randn(3, 70, 132, generator=torch.Generator().manual_seed(36)).cuda()
+    run = lambda: ops.rnn_forward("foot_contact", x, [70, 41, 70], None, dev, [0, -1, 1])[0]
+    want = run()
+    ops.set_lstm_mode(3)
+    try:
+        got = run()
+    finally:
+        ops.set_lstm_mode(1)
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("shape", [(2, 3100, 128, 2050, 2, 20), (4, 300, 100, 70, 2, 5), (3, 1, 1024, 300, 3, 16)], ids=str)
+def test_linear_adapted_captured(ops, shape):
+    """Every kind of launch (large tiles straight to LDS, one launch, small tiles) in a graph: replays with other inputs and ids, the
+    eager call between them."""
+    import torch
+    x, w, b, down, up, scale, ids = linear_inputs(14, *shape, torch.bfloat16)
+    call = lambda: ops.linear_adapted(x, w, b, down, up, scale, ids, relu=True)
+    call()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = call()
+    for i in range(4):
+        x.copy_(x.roll(1, -1))
+        ids.copy_((ids + 2) % (shape[4] + 1) - 1)
+        graph.replay()
+        got = y.clone()
+        assert torch.equal(got, call())
+        torch.cuda.synchronize()
