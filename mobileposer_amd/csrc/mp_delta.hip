@@ -20,13 +20,12 @@
 namespace mpseq {
 
 constexpr int kC = 32;                            // frames per chunk
-// Workspace of one (sequence, value head, chunk), bytes: T = (I + A)^{-1} diag(beta) as three terms and P = scale tril(Q K^T) o D as two (bf16
-// outputs) or three, in the order in which a lane of v_mfma_f32_16x16x32_bf16 takes its A operand, behind e^G and e^{G_C - G} of the
-// 32 frames.
+// Workspace of one (sequence, value head, chunk), bytes: T = (I + A)^{-1} diag(beta) and P = scale tril(Q K^T) o D as three terms each, in
+// the order in which a lane of v_mfma_f32_16x16x32_bf16 takes its A operand, behind e^G and e^{G_C - G} of the 32 frames.  (Three
+// beside bf16 outputs as well: with two of P, of U beside it and of the S in Q S0 the outputs of 8 x 2048 frames were not the
+// correctly rounded ones in 0.23 % instead of 0.01 % of all places, in 173 us instead of 188.)
 constexpr int kFrag = 1024;                       // one 16 x 32 operand: 64 lanes x 8 bf16
-constexpr int kWsEg = 0, kWsTail = 4 * kC, kWsT = 8 * kC, kWsP = kWsT + 6 * kFrag;
-constexpr int ws_unit(int po) { return kWsP + 2 * po * kFrag; }
-
+constexpr int kWsEg = 0, kWsTail = 4 * kC, kWsT = 8 * kC, kWsP = kWsT + 6 * kFrag, kWsUnit = kWsP + 6 * kFrag;
 
 // Which frame and which component of k a lane's registers stand for.  The accumulator layout of a 16 x 16 tile (lane: column
 // lane % 16, rows 4 (lane / 16) + r) becomes the B operand of a K = 32 instruction (lane: column lane % 16, k slots
@@ -81,7 +80,7 @@ static __device__ __forceinline__ double lane_below(double x) {
 // where keys repeat and A is far from small, products of powers of A are not -- and T21 = -T22 A21 T11 on the fp32 matrix
 // instructions.  KB: steps of 32 components whose loads are in flight together.  Bound by memory, its own output being the larger part:
 // 8 x 2048 frames, 8 / 16 heads of 128, bf16 34 us (4.5 TB/s), 256 x 125 frames, 4 heads of 64, fp32 22 us.
-template <class E, int PO, int MODE, int KB>
+template <class E, int MODE, int KB>
 MP_KERNEL __launch_bounds__(64) void mp_delta_prep(DeltaArgs a) {
     constexpr int P = Arith<E>::P, LS = kC + 4;
     __shared__ __align__(16) float At[kC][LS], Tm[kC][LS], betas[kC];      // A transposed: [column][row]
@@ -131,8 +130,8 @@ MP_KERNEL __launch_bounds__(64) void mp_delta_prep(DeltaArgs a) {
             }
         }
     }
-    char* ws = (char*)a.ws + ((size_t)(b * a.Hv + hk * rep) * a.nchunk + c) * ws_unit(PO);
-    for (int e = 0; e < rep; ++e, ws += (size_t)a.nchunk * ws_unit(PO)) {
+    char* ws = (char*)a.ws + ((size_t)(b * a.Hv + hk * rep) * a.nchunk + c) * kWsUnit;
+    for (int e = 0; e < rep; ++e, ws += (size_t)a.nchunk * kWsUnit) {
         const float beta = on ? bnext : 0.f;
         double G = on ? (double)clamp_g(gnext) : 0.0;             // lanes 32.. as lanes 0..31
         if (e + 1 < rep) { gnext = gate(a.g, a.sg, e + 1); bnext = gate(a.beta, a.sb, e + 1); }
@@ -183,7 +182,7 @@ MP_KERNEL __launch_bounds__(64) void mp_delta_prep(DeltaArgs a) {
             o.load(&W[row_index(I, col)][8 * grp]);
             o.planes(p);
 #pragma unroll
-            for (int n = 0; n < PO; ++n) *(u32x4*)(ws + kWsP + (I * PO + n) * kFrag + lane * 16) = p[n];
+            for (int n = 0; n < 3; ++n) *(u32x4*)(ws + kWsP + (I * 3 + n) * kFrag + lane * 16) = p[n];
         }
         // the diagonal blocks (groups 2 and 3 as 0 and 1)
         const int blk = grp & 1;
@@ -252,14 +251,14 @@ constexpr int kFragK = kFrag + 256;               // K's operands: 64 bytes betw
                                                   // turning read would meet in a quarter of the banks
 template <class E, int NK>
 struct ScanLds {
-    static constexpr int P = Arith<E>::P, PO = P == 1 ? 2 : 3, kPlaneK = 2 * NK * kFragK, kPlaneQ = 2 * NK * kFrag;
-    static constexpr int kQ = P * kPlaneK, kWs = kQ + P * kPlaneQ, kV = kWs + (ws_unit(PO) + 15) / 16 * 16, kRowV = (64 + 16 / sizeof(E)) * sizeof(E);
+    static constexpr int P = Arith<E>::P, kPlaneK = 2 * NK * kFragK, kPlaneQ = 2 * NK * kFrag;
+    static constexpr int kQ = P * kPlaneK, kWs = kQ + P * kPlaneQ, kV = kWs + (kWsUnit + 15) / 16 * 16, kRowV = (64 + 16 / sizeof(E)) * sizeof(E);
     static constexpr int kBytes = kV + kC * kRowV;
 };
 template <class E, int NK, int MODE>
 struct Rows {                                     // what a thread stages of a chunk
     using L = ScanLds<E, NK>;
-    static constexpr int P = L::P, NF = (2 * NK + 3) / 4, kUnit = ws_unit(L::PO), NW = (kUnit + 4095) / 4096;
+    static constexpr int P = L::P, NF = (2 * NK + 3) / 4, kUnit = kWsUnit, NW = (kUnit + 4095) / 4096;
     Oct<E> k[NF], q[NF], v;
     u32x4 ws[NW];
     unsigned ok[NF], oq[NF], ov;                  // byte offsets from the chunk's first row
@@ -348,7 +347,7 @@ template <class E, int NK> constexpr bool two_per_cu() { return Arith<E>::P == 1
 template <class E, int NK, int MODE, bool OUT>
 MP_KERNEL __launch_bounds__(256, (two_per_cu<E, NK>() ? 2 : 1)) void mp_delta_scan(DeltaArgs a, DeltaPlan plan, int ncol, int ncolm) {
     using L = ScanLds<E, NK>;
-    constexpr int P = L::P, PO = L::PO;
+    constexpr int P = L::P;
     extern __shared__ __align__(16) char scan_lds[];
     char* const lds = scan_lds;
     const char* const ws = lds + L::kWs;
@@ -370,7 +369,7 @@ MP_KERNEL __launch_bounds__(256, (two_per_cu<E, NK>() ? 2 : 1)) void mp_delta_sc
     const char* k = (const char*)((const E*)a.k + b * a.sk[0] + hk * a.sk[2] + s0 * a.sk[1]);
     const char* v = (const char*)((const E*)a.v + b * a.sv[0] + hv * a.sv[2] + s0 * a.sv[1]);
     const long kstep = kC * a.sk[1] * sizeof(E), qstep = kC * a.sq[1] * sizeof(E), vstep = kC * a.sv[1] * sizeof(E);
-    const char* wsg = (const char*)a.ws + ((size_t)(b * a.Hv + hv) * a.nchunk + seg * plan.len) * ws_unit(PO);
+    const char* wsg = (const char*)a.ws + ((size_t)(b * a.Hv + hv) * a.nchunk + seg * plan.len) * kWsUnit;
     const size_t so = (size_t)a.Hv * a.dv, head = (size_t)(b * a.Hv + hv), cc = cok ? cv : width - 1;
     const float* s_in = seg == 0 ? a.s_in : OUT ? plan.N + (head * (plan.nseg - 1) + seg - 1) * a.dk * a.dv : nullptr;
     if (seg == 0 && s_in) s_in += head * a.dk * a.dv;
@@ -411,7 +410,7 @@ MP_KERNEL __launch_bounds__(256, (two_per_cu<E, NK>() ? 2 : 1)) void mp_delta_sc
     for (int c = 0; c < nc; ++c) {
         const int t0 = c * kC;
         if (c + 1 < nc) {                                          // (the last chunk asks for itself again: no branch around the loads)
-            k += kstep; q += qstep; v += vstep; wsg += ws_unit(PO);
+            k += kstep; q += qstep; v += vstep; wsg += kWsUnit;
             if (t0 + 2 * kC > tmax) rows.place(a, tmax - 1 - t0 - kC, c0);   // (rows behind the tensor's end)
         }
         rows.load(a, k, q, v, wsg, c0);
@@ -468,20 +467,13 @@ MP_KERNEL __launch_bounds__(256, (two_per_cu<E, NK>() ? 2 : 1)) void mp_delta_sc
                 mfma_planes_n<2, P, 3>(fk, sp[m & 1], k2);
                 kq[0] = k2[0];
                 kq[1] = k2[1];
-            } else if (P == 1) {                                   // Q S0 with the state's first two terms: its rounding is bf16's
-                u32x4 fk[2][P] = {{f[m & 1][0][0]}, {f[m & 1][1][0]}}, third[1] = {sp[m & 1][2]}, two[2] = {sp[m & 1][0], sp[m & 1][1]};
-                f32x4 lowest[2] = {kq[0], kq[1]};
-                mfma_planes_n<2, P, 1>(fk, third, lowest);
-                kq[0] = lowest[0];
-                kq[1] = lowest[1];
-                mfma_planes_n<4, P, 2>(f[m & 1], two, kq);
             } else {
                 mfma_planes_n<4, P, 3>(f[m & 1], sp[m & 1], kq);
             }
             if (m + 1 < NK) {
                 split(m + 1);
 #pragma unroll
-                for (int i = 0; i < (OUT ? P == 1 ? 10 : 24 : P == 1 ? 6 : 12); ++i) {
+                for (int i = 0; i < (OUT ? P == 1 ? 12 : 24 : P == 1 ? 6 : 12); ++i) {
                     __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);                 // a matrix instruction,
                     __builtin_amdgcn_sched_group_barrier(0x2, P == 1 ? 5 : 2, 0);    // vector instructions that fit behind it
                 }
@@ -514,7 +506,7 @@ MP_KERNEL __launch_bounds__(256, (two_per_cu<E, NK>() ? 2 : 1)) void mp_delta_sc
         }
         u32x4 rp[3];
         R.planes(rp);
-        u32x4 Pm[2][PO], ft[2][4][P];
+        u32x4 Pm[2][3], ft[2][4][P];
         auto turn = [&](int m) {
 #pragma unroll
             for (int n = 0; n < 4 && 4 * m + n < 2 * NK; ++n)
@@ -530,8 +522,8 @@ MP_KERNEL __launch_bounds__(256, (two_per_cu<E, NK>() ? 2 : 1)) void mp_delta_sc
 #pragma unroll
         for (int I = 0; I < 2; ++I)
 #pragma unroll
-            for (int p = 0; p < PO; ++p)
-                if (OUT) Pm[I][p] = operand(ws + kWsP + (I * PO + p) * kFrag, lane);
+            for (int p = 0; p < 3; ++p)
+                if (OUT) Pm[I][p] = operand(ws + kWsP + (I * 3 + p) * kFrag, lane);
         FENCE();
         f32x4 u[2] = {}, w[2] = {};
         mfma_planes_n<2, 3, 3>(T, rp, u);
@@ -551,13 +543,9 @@ MP_KERNEL __launch_bounds__(256, (two_per_cu<E, NK>() ? 2 : 1)) void mp_delta_sc
         // S' = e^{G_C} S0 + K^T (e^{G_C - G} U), four tiles a step, and P U beside it
 #pragma unroll
         for (int j = 0; j < 8; ++j) Ut.v[j] = tail[j] * U.v[j];
-        u32x4 up[3], ut[3], u2[PO];
+        u32x4 up[3], ut[3];
         Ut.planes(ut);
-        if (OUT) {
-            U.planes(up);
-#pragma unroll
-            for (int p = 0; p < PO; ++p) u2[p] = up[p];
-        }
+        if (OUT) U.planes(up);
 #pragma unroll
         for (int m = 0; m < (NK + 1) / 2; ++m) {
             FENCE();
@@ -575,7 +563,7 @@ MP_KERNEL __launch_bounds__(256, (two_per_cu<E, NK>() ? 2 : 1)) void mp_delta_sc
                 for (int n = 0; n < 2; ++n) S[4 * m + n] = mfma_planes(ft[m & 1][n], ut, S[4 * m + n] * whole);
             }
         }
-        if (OUT) mfma_planes_n<2, PO, PO>(Pm, u2, w);
+        if (OUT) mfma_planes_n<2, 3, 3>(Pm, up, w);
 #pragma unroll
         for (int j = 0; OUT && j < 8; ++j) {
             float ov = fmaf(a.scale * eg[j], kq[2 + (j >> 2)][j & 3], w[j >> 2][j & 3]);
@@ -734,7 +722,7 @@ static DeltaPlan plan_of(int B, int T, int Hv, int dk, int dv, bool two) {
     }
     return p;
 }
-static size_t prep_floats(int B, int T, int Hv) { return (size_t)B * Hv * ((T + kC - 1) / kC) * (ws_unit(3) / 4); }
+static size_t prep_floats(int B, int T, int Hv) { return (size_t)B * Hv * ((T + kC - 1) / kC) * (kWsUnit / 4); }
 size_t delta_ws_floats(int B, int T, int Hv, int dk, int dv) {
     return prep_floats(B, T, Hv) + (size_t)B * Hv * (max(plan_of(B, T, Hv, dk, dv, false).nseg, plan_of(B, T, Hv, dk, dv, true).nseg) - 1) * dk * (dk + dv) + 4;
 }
@@ -770,12 +758,13 @@ static bool scan_for(const DeltaArgs& a, hipStream_t s) {
     }
     return scan_pass<E, NK, MODE, true>(a, p, s);
 }
-template <class E, int PO, int MODE>
+template <class E, int MODE>
 static bool launch_mode(const DeltaArgs& a, hipStream_t s) {
     if (a.nchunk) {
         const dim3 grid((unsigned)(a.B * a.Hk * a.nchunk));
-        if (Arith<E>::P == 1 && a.dk > 64) hipLaunchKernelGGL((mp_delta_prep<E, PO, MODE, 4>), grid, dim3(64), 0, s, a);
-        else hipLaunchKernelGGL((mp_delta_prep<E, PO, MODE, 2>), grid, dim3(64), 0, s, a);
+        constexpr int wide = Arith<E>::P == 1 ? 4 : 2;
+        if (a.dk > 64) hipLaunchKernelGGL((mp_delta_prep<E, MODE, wide>), grid, dim3(64), 0, s, a);
+        else hipLaunchKernelGGL((mp_delta_prep<E, MODE, 2>), grid, dim3(64), 0, s, a);
     }
     if (MODE == 2) return scan_for<E, 8, MODE>(a, s);
     constexpr int M = MODE == 2 ? 1 : MODE;
@@ -783,13 +772,13 @@ static bool launch_mode(const DeltaArgs& a, hipStream_t s) {
     return nk == 1 ? scan_for<E, 1, M>(a, s) : nk == 2 ? scan_for<E, 2, M>(a, s) : nk == 3 ? scan_for<E, 3, M>(a, s) : nk == 4 ? scan_for<E, 4, M>(a, s)
          : nk <= 6 ? scan_for<E, 6, M>(a, s) : scan_for<E, 8, M>(a, s);
 }
-template <class E, int PO>
+template <class E>
 static bool launch_for(const DeltaArgs& a, hipStream_t s) {
-    const bool ok = a.dk < 8 || a.dv < 8 ? launch_mode<E, PO, 2>(a, s) : a.dk % 8 ? launch_mode<E, PO, 1>(a, s) : launch_mode<E, PO, 0>(a, s);
+    const bool ok = a.dk < 8 || a.dv < 8 ? launch_mode<E, 2>(a, s) : a.dk % 8 ? launch_mode<E, 1>(a, s) : launch_mode<E, 0>(a, s);
     return hipGetLastError() == hipSuccess && ok;
 }
 bool launch_delta(const DeltaArgs& a, int dtype, hipStream_t s) {
-    return dtype == kBF16 ? launch_for<bf16raw, 2>(a, s) : launch_for<float, 3>(a, s);
+    return dtype == kBF16 ? launch_for<bf16raw>(a, s) : launch_for<float>(a, s);
 }
 
 // ---------------------------------------------------------------- one frame per stream
