@@ -334,18 +334,15 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
     }
     const int id0 = __builtin_amdgcn_readfirstlane(id[0]);
     const bool wave_same = FUSED || __all(same);
-    // z keeps 16 of its bits beside bf16 operands, all 24 beside fp32 ones
-    constexpr int PZ = P == 1 ? 2 : 3;
+    // z is fp32 whatever the inputs are: all three terms of it
+    constexpr int PZ = 3;
     auto z_of = [&](int i) {
         return FUSED ? zl + ((wr * MR + i) * 16 + col) * G::kRowZ : a.ws + (size_t)min(n0 + (wr * MR + i) * 16 + col, n1 - 1) * rlen;
     };
     auto z_planes = [&](const float* z, int k, u32x4 (&pz)[PZ]) {
         Oct<float> oz;
-        u32x4 p3[3];
         oz.load_some(z + k, rlen - k < 0 ? 0 : rlen - k);
-        oz.planes(p3);
-#pragma unroll
-        for (int p = 0; p < PZ; ++p) pz[p] = p3[p];
+        oz.planes(pz);
     };
     auto up_planes = [&](int ad, int j, int k, u32x4 (&pu)[P]) {
         const int m = m0 + (wc * MC + j) * 16 + col;

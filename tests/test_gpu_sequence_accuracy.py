@@ -19,3 +19,12 @@ def test_delta_rule_is_as_accurate_as_fp32_sums(ops, shape, dtype):  # noqa: F81
     o, s = ops.delta_rule(q, k, v, g, beta, None, state)
     assert F.held(s.cpu(), ws, ps) <= 1
     assert F.held(o.cpu(), wo, po) <= 1
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("shape", F.LINEAR, ids=str)
+def test_linear_adapted_is_as_accurate_as_fp32_sums(ops, shape, dtype):  # noqa: F811
+    import torch
+    args = F.linear_inputs(2, *shape, getattr(torch, dtype), adapter=4.0)
+    y = ops.linear_adapted(*(t.cuda() for t in args))
+    assert F.held(y.cpu(), F.linear_exact(*args), F.linear_fp32(*args)) <= 1

@@ -20,3 +20,14 @@ def test_delta_bounds_tell_two_terms_from_three(shape, dtype):
         assert F.held(o, wo, po) > 1
     o, _ = F.delta_fp32(*args, scale, out_cut=2)
     assert F.held(o.to(dtype), wo, po) > 1
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("shape", F.LINEAR, ids=str)
+def test_linear_bounds_tell_two_terms_from_three(shape, dtype):
+    args = F.linear_inputs(2, *shape, dtype, adapter=4.0)
+    want, plain = F.linear_exact(*args), F.linear_fp32(*args)
+    assert F.held(F.linear_fp32(*args, cut=3, z_cut=3).to(dtype), want, plain) <= 1
+    assert F.held(F.linear_fp32(*args, z_cut=2).to(dtype), want, plain) > 1
+    if dtype is torch.float32:
+        assert F.held(F.linear_fp32(*args, cut=2), want, plain) > 1
