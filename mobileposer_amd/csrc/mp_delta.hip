@@ -338,10 +338,14 @@ static __device__ __forceinline__ u32x4 operand(const char* p, int lane) { retur
 // Few sequences and heads: the chunks are cut into segments that run side by side.  A segment maps the state it starts from linearly,
 // S -> M S + N; N [dk][dv] is its run from zero, column j of M [dk][dk] its run from the j-th unit vector with V = 0: the same
 // kernel without its outputs (OUT = false), dv + dk columns.  mp_delta_join carries the states through the segments, then all
-// segments run from their own start (OUT = true).  Three times the work, in 2 / segments of the steps.
+// segments run from their own start (OUT = true).  Three times the work, in 2 / segments of the steps.  state_in may be state_out,
+// and in the last pass the segment with a sequence's end writes that buffer while nothing orders it behind the first one: the first
+// pass puts the start of every sequence aside for it, by the workgroups whose part of M would be the first segment's (by those that
+// run it: 1 x 3000 frames 54.5 -> 58.5 us).
 struct DeltaPlan {
     int nseg, len;                                // segments and chunks per segment; nseg = 1: the chunks in one go
     float *N, *M;                                 // [B][Hv][nseg - 1][dk][dv] (mp_delta_join turns N of s into the start of s + 1), [..][dk][dk]
+    float* S0;                                    // [B][Hv][dk][dv]: the start of sequences that go on behind the first segment
 };
 template <class E, int NK> constexpr bool two_per_cu() { return Arith<E>::P == 1 ? NK <= 4 : NK <= 2; }
 template <class E, int NK, int MODE, bool OUT>
@@ -364,7 +368,13 @@ MP_KERNEL __launch_bounds__(256, (two_per_cu<E, NK>() ? 2 : 1)) void mp_delta_sc
     const int len_all = length_of(a.lengths, b, a.T);
     // this segment's frames, as a sequence that begins at its first
     const int s0 = seg * plan.len * kC, len = min(len_all, seg + 1 == plan.nseg ? a.T : s0 + plan.len * kC) - s0;
-    if (!OUT && (len_all <= s0 + plan.len * kC || (unitcol && seg == 0))) return;      // (no segment follows; the first one's start is known)
+    if (!OUT && len_all <= s0 + plan.len * kC) return;             // (no segment follows)
+    if (!OUT && unitcol && seg == 0) {                             // (the first one's start is known: nothing to run, but put it aside)
+        const size_t at = (size_t)(b * a.Hv + hv) * a.dk * a.dv;
+        if (a.s_in)
+            for (int i = c0 * a.dv + tid; i < min(c0 + 64, a.dk) * a.dv; i += 256) plan.S0[at + i] = a.s_in[at + i];
+        return;
+    }
     const char* q = (const char*)((const E*)a.q + b * a.sq[0] + hk * a.sq[2] + s0 * a.sq[1]);
     const char* k = (const char*)((const E*)a.k + b * a.sk[0] + hk * a.sk[2] + s0 * a.sk[1]);
     const char* v = (const char*)((const E*)a.v + b * a.sv[0] + hv * a.sv[2] + s0 * a.sv[1]);
@@ -372,7 +382,7 @@ MP_KERNEL __launch_bounds__(256, (two_per_cu<E, NK>() ? 2 : 1)) void mp_delta_sc
     const char* wsg = (const char*)a.ws + ((size_t)(b * a.Hv + hv) * a.nchunk + seg * plan.len) * kWsUnit;
     const size_t so = (size_t)a.Hv * a.dv, head = (size_t)(b * a.Hv + hv), cc = cok ? cv : width - 1;
     const float* s_in = seg == 0 ? a.s_in : OUT ? plan.N + (head * (plan.nseg - 1) + seg - 1) * a.dk * a.dv : nullptr;
-    if (seg == 0 && s_in) s_in += head * a.dk * a.dv;
+    if (seg == 0 && s_in) s_in = (OUT && len_all > plan.len * kC ? plan.S0 : s_in) + head * a.dk * a.dv;
     const int tmax = a.T - s0;                                     // frames of the tensor from here on
     // outputs leave as eight columns of a frame per thread, from the place of V
     const int ocol = c0 + 8 * (tid & 7), ofull = a.dv - ocol;
@@ -713,7 +723,7 @@ MP_KERNEL __launch_bounds__(KT <= 4 ? 256 : 512) void mp_delta_join(DeltaArgs a,
 // many: 2 x 4096, 32 heads of 64, bf16 147 -> 134 (fp32 236 -> 212), 4 x 4096, 16 heads of 128, bf16 320 -> 302 (fp32, one a CU, 567
 // -> 585); with more the join, whose steps are one after the other, takes what the passes gain (1 x 32768, 4 heads, 144 -> 199).
 static DeltaPlan plan_of(int B, int T, int Hv, int dk, int dv, bool two) {
-    DeltaPlan p = {1, (T + kC - 1) / kC, nullptr, nullptr};
+    DeltaPlan p = {1, (T + kC - 1) / kC, nullptr, nullptr, nullptr};
     const long per = (long)B * Hv * ((dv + 63) / 64 + (dk + 63) / 64);
     const int nchunk = p.len, want = (int)min((long)nchunk / 4, (two && 512 / per <= 8 ? 1024 : 512) / per);
     if (want >= 4) {
@@ -724,7 +734,8 @@ static DeltaPlan plan_of(int B, int T, int Hv, int dk, int dv, bool two) {
 }
 static size_t prep_floats(int B, int T, int Hv) { return (size_t)B * Hv * ((T + kC - 1) / kC) * (kWsUnit / 4); }
 size_t delta_ws_floats(int B, int T, int Hv, int dk, int dv) {
-    return prep_floats(B, T, Hv) + (size_t)B * Hv * (max(plan_of(B, T, Hv, dk, dv, false).nseg, plan_of(B, T, Hv, dk, dv, true).nseg) - 1) * dk * (dk + dv) + 4;
+    const size_t cuts = max(plan_of(B, T, Hv, dk, dv, false).nseg, plan_of(B, T, Hv, dk, dv, true).nseg) - 1;
+    return prep_floats(B, T, Hv) + (size_t)B * Hv * (cuts * dk * (dk + dv) + (cuts ? (size_t)dk * dv : 0)) + 4;
 }
 
 template <class E, int NK, int MODE, bool OUT>
@@ -743,6 +754,7 @@ static bool scan_for(const DeltaArgs& a, hipStream_t s) {
     if (p.nseg > 1) {
         p.N = a.ws + prep_floats(a.B, a.T, a.Hv);
         p.M = p.N + ((size_t)a.B * a.Hv * (p.nseg - 1) * a.dk * a.dv + 3) / 4 * 4;
+        p.S0 = p.M + (size_t)a.B * a.Hv * (p.nseg - 1) * a.dk * a.dk;
         if (!scan_pass<E, NK, MODE, false>(a, p, s)) return false;
         const int ncol = (a.dv + 15) / 16;
         const dim3 grid((unsigned)(a.B * a.Hv * ncol));

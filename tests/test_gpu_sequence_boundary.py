@@ -1,0 +1,46 @@
+"""Calls of the sequence operators that the header allows and the facade does not make: through the C entries, on the caller's own
+buffers."""
+import ctypes as C
+
+import pytest
+
+import sequence_forms as F
+from test_gpu_sequence import ops  # noqa: F401  (the model object as a fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+def delta_call(ops, q, k, v, g, beta, lengths, state_in, state_out, scale, shape=None, strides=None):  # noqa: F811
+    """mp_delta_rule on these buffers -> o.  shape, strides: of inputs that are flat buffers."""
+    import torch
+    B, T, Hk, Hv, dk, dv = shape or (*q.shape[:3], v.shape[2], q.shape[3], v.shape[3])
+    o = torch.full((B, T, Hv, dv), float("nan"), device="cuda", dtype=q.dtype)
+    need = ops._lib.mp_delta_rule_workspace(B, T, Hv, dk, dv)
+    ws = torch.full((need + 256,), 0xa5, device="cuda", dtype=torch.uint8)
+    st = (C.c_int64 * 15)(*(strides or [s for t in (q, k, v, g, beta) for s in t.stride()[:3]]))
+    ptr = lambda t: 0 if t is None else t.data_ptr()
+    ops._check(ops._lib.mp_delta_rule(ops._h, 1 if q.dtype is torch.bfloat16 else 0, *(ptr(t) for t in (q, k, v, g, beta)), C.addressof(st), ptr(lengths), B, T, Hk,
+                                      Hv, dk, dv, scale, ptr(o), ptr(state_in), ptr(state_out), ptr(ws), need, torch.cuda.current_stream().cuda_stream))
+    assert (ws[need:] == 0xa5).all()                  # the workspace is as large as its function says
+    return o
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("shape", [(3, 1000, 1, 2, 64, 40), (5, 700, 1, 1, 32, 65), (1, 1400, 1, 1, 128, 130), (4, 600, 1, 3, 200, 20), (3, 90, 2, 2, 64, 64), (2, 770, 1, 1, 7, 5)], ids=str)
+def test_delta_rule_state_in_its_own_buffer(ops, shape, dtype):  # noqa: F811
+    """state_in and state_out are one buffer: bit for bit what two buffers give, whole and in segments, with sequences that end one
+    frame and one chunk behind a border between two segments, at it, in the first segment, and at once."""
+    import torch
+    B, T = shape[:2]
+    q, k, v, g, beta, state = (t.cuda() for t in F.delta_inputs(5, *shape, getattr(torch, dtype)))
+    for lens in ([T] * B, [T, 129, 128, 1, 0][:B], [161, 257, T - 1, 0, 33][:B], [385, 513, 289, T, 96][:B]):
+        lens = torch.tensor([min(n, T) for n in lens], device="cuda", dtype=torch.int32)
+        out = torch.full_like(state, float("nan"))
+        want = delta_call(ops, q, k, v, g, beta, lens, state, out, 0.3, shape)
+        for _ in range(3):
+            own = state.clone()
+            got = delta_call(ops, q, k, v, g, beta, lens, own, own, 0.3, shape)
+            assert torch.equal(got, want) and torch.equal(own, out)
+        assert torch.equal(delta_call(ops, q, k, v, g, beta, lens, state, None, 0.3, shape), want)
+        zero = torch.zeros_like(state)
+        assert torch.equal(delta_call(ops, q, k, v, g, beta, lens, None, None, 0.3, shape), delta_call(ops, q, k, v, g, beta, lens, zero, zero, 0.3, shape))
