@@ -91,8 +91,10 @@ MP_KERNEL __launch_bounds__(64) void mp_delta_prep(DeltaArgs a) {
     const int rep = a.Hv / a.Hk, t = t0 + i;
     const E* q = (const E*)a.q + b * a.sq[0] + hk * a.sq[2];
     const E* k = (const E*)a.k + b * a.sk[0] + hk * a.sk[2];
-    // (everything is requested at once: rows behind the sequence's end are read as far as the tensor goes, and dropped)
-    const int tl[2] = {min(t0 + col, a.T - 1), min(t0 + 16 + col, a.T - 1)};
+    const int len = length_of(a.lengths, b, a.T);
+    if (t0 >= len) return;
+    // (everything is requested at once; rows behind the sequence's end are not there: its last one instead, and dropped)
+    const int tl[2] = {min(t0 + col, len - 1), min(t0 + 16 + col, len - 1)};
     Oct<E> ok[KB][2], oq[KB][2];
     auto request = [&](int d0) {
 #pragma unroll
@@ -104,10 +106,8 @@ MP_KERNEL __launch_bounds__(64) void mp_delta_prep(DeltaArgs a) {
             }
     };
     request(0);
-    auto gate = [&](const float* p, const long (&s)[3], int e) { return p[b * s[0] + min(t, a.T - 1) * s[1] + (hk * rep + e) * s[2]]; };
+    auto gate = [&](const float* p, const long (&s)[3], int e) { return p[b * s[0] + min(t, len - 1) * s[1] + (hk * rep + e) * s[2]]; };
     float gnext = gate(a.g, a.sg, 0), bnext = gate(a.beta, a.sb, 0);
-    const int len = length_of(a.lengths, b, a.T);
-    if (t0 >= len) return;
     const bool on = t < len;
     f32x4 kk[3] = {}, qk[3] = {};                 // tiles (0,0), (1,0), (1,1) of frames 16 I + row, 16 J + column
     for (int d0 = 0; d0 < a.dk; d0 += 32 * KB) {
@@ -412,7 +412,7 @@ MP_KERNEL __launch_bounds__(256, (two_per_cu<E, NK>() ? 2 : 1)) void mp_delta_sc
     const int nc = len <= 0 ? 0 : (len + kC - 1) / kC;
     Rows<E, NK, MODE> rows;
     if (nc > 0) {
-        rows.place(a, min(kC, tmax) - 1, c0);
+        rows.place(a, min(kC, len) - 1, c0);
         rows.load(a, k, q, v, wsg, c0);
         rows.store(a, lds, 0, len, c0);
     }
@@ -421,7 +421,7 @@ MP_KERNEL __launch_bounds__(256, (two_per_cu<E, NK>() ? 2 : 1)) void mp_delta_sc
         const int t0 = c * kC;
         if (c + 1 < nc) {                                          // (the last chunk asks for itself again: no branch around the loads)
             k += kstep; q += qstep; v += vstep; wsg += kWsUnit;
-            if (t0 + 2 * kC > tmax) rows.place(a, tmax - 1 - t0 - kC, c0);   // (rows behind the tensor's end)
+            if (t0 + 2 * kC > len) rows.place(a, len - 1 - t0 - kC, c0);     // (rows behind the sequence's end are not there)
         }
         rows.load(a, k, q, v, wsg, c0);
         __builtin_amdgcn_sched_barrier(0);                         // (the loads are issued here, not where their values are used)

@@ -44,3 +44,20 @@ def test_delta_rule_state_in_its_own_buffer(ops, shape, dtype):  # noqa: F811
         assert torch.equal(delta_call(ops, q, k, v, g, beta, lens, state, None, 0.3, shape), want)
         zero = torch.zeros_like(state)
         assert torch.equal(delta_call(ops, q, k, v, g, beta, lens, None, None, 0.3, shape), delta_call(ops, q, k, v, g, beta, lens, zero, zero, 0.3, shape))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("shape", [(3, 70, 2, 4, 64, 40), (2, 97, 1, 1, 41, 9), (2, 60, 1, 2, 7, 5), (1, 1000, 1, 2, 64, 64)], ids=str)
+def test_delta_rule_of_buffers_that_end_with_their_last_sequence(ops, shape, dtype):  # noqa: F811
+    """Frames behind a sequence's end need no memory: the inputs' buffers end with the last sequence's last frame."""
+    import torch
+    B, T, Hk, Hv, dk, dv = shape
+    q, k, v, g, beta, state = (t.cuda() for t in F.delta_inputs(6, *shape, getattr(torch, dtype)))
+    for last in (T, T - 1, 33, 32, 31, 1, 0):
+        lens = torch.tensor([T, 17][:B - 1] + [last], device="cuda", dtype=torch.int32)
+        frames = (B - 1) * T + last
+        short = [torch.cat([t.flatten(0, 1)[:frames].flatten(), t.new_zeros(1 if frames == 0 else 0)]) for t in (q, k, v, g, beta)]
+        strides = [x for t in (q, k, v, g, beta) for x in t.stride()[:3]]
+        out, want_out = torch.empty_like(state), torch.empty_like(state)
+        got = delta_call(ops, *short, lens, state, out, 0.3, shape, strides)
+        assert torch.equal(got, delta_call(ops, q, k, v, g, beta, lens, state, want_out, 0.3)) and torch.equal(out, want_out)
