@@ -213,14 +213,15 @@ MP_KERNEL __launch_bounds__(64) void mp_delta_prep(DeltaArgs a) {
             const float4 t11 = {Tm[l][col], Tm[l + 1][col], Tm[l + 2][col], Tm[l + 3][col]};
             const float4 t22 = *(const float4*)&Tm[16 + col][16 + l];
             X = mfma4(a21, t11, X);
-            float4 y;                                             // (a later frame's row that is not finite is kept from the zeros of T22)
+            float4 y;                                             // (a later frame's row that is not finite is kept from the zeros of T22,
+                                                                  //  and is NaN itself: what hides in it may come from finite inputs)
             y.x = not_finite(X[0]) ? 0.f : X[0];
             y.y = not_finite(X[1]) ? 0.f : X[1];
             y.z = not_finite(X[2]) ? 0.f : X[2];
             y.w = not_finite(X[3]) ? 0.f : X[3];
             T21 = mfma4(t22, y, T21);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) Tm[16 + l + r][col] = -T21[r];
+            for (int r = 0; r < 4; ++r) Tm[16 + l + r][col] = not_finite(X[r]) ? __builtin_nanf("") : -T21[r];
         }
         __syncthreads();
         float bc[8];
