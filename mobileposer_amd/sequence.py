@@ -3,11 +3,13 @@
 recurrent block, over mp_delta_rule / mp_delta_rule_online / mp_linear_adapted (include/mobileposer_hip.h).
 
 They take torch tensors on the model's device, fp32 or bf16, run on the current stream, and return fresh tensors without waiting.
-Inference only, as the rest of the package: a tensor that requires a gradient is refused while gradients are recorded.
+Inference only, as the rest of the package: a tensor that requires a gradient is refused while gradients are recorded, and one that
+carries a tangent (forward-mode derivatives) always.
 No counterpart in the reference."""
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -20,6 +22,8 @@ def _no_grad(*tensors):
     for t in tensors:
         if t is not None and t.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("the sequence operators have no backward pass: call them under torch.no_grad() or detach their inputs")
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("the sequence operators have no forward-mode derivative: a tensor carries a tangent")
 
 
 def _rows(t):

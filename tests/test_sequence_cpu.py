@@ -88,3 +88,34 @@ def test_block_adapters_refuses(change):
         Ops()._block_adapters({}, [0, 1], 2, {"linear1": (60, 256), "linear2": (512, 72)})
     lib = _lib.load()
     assert lib.mp_rnn_forward_adapted(None, 0, None, None, 1, 1, *[None] * 6, 1, *[None] * 3, 1, None, 1, None, 0, None) == _lib.MP_ERR_INVALID
+
+
+def linear():
+    z = torch.zeros
+    return {"x": z(2, 3, 16), "weight": z(24, 16), "bias": z(24), "down": z(2, 4, 16), "up": z(2, 24, 4), "scale": z(2), "ids": [0, 1]}
+
+
+@pytest.mark.parametrize("name", ["q", "k", "v", "g", "beta", "state"])
+def test_delta_rule_refuses_a_tangent(name):
+    from torch.autograd import forward_ad
+    args = {**delta(), "state": torch.zeros(2, 4, 16, 8)}
+    with forward_ad.dual_level():
+        args[name] = forward_ad.make_dual(args[name], torch.ones_like(args[name]))
+        with pytest.raises(RuntimeError, match="tangent"):
+            Ops().delta_rule(**args)
+        with pytest.raises(RuntimeError, match="tangent"):
+            Ops().delta_rule_online(**{n: t if n == "state" else t[:, 0] for n, t in args.items()})
+
+
+@pytest.mark.parametrize("name", ["x", "weight", "bias", "down", "up", "scale"])
+def test_linear_adapted_refuses_a_tangent(name):
+    from torch.autograd import forward_ad
+    args = linear()
+    with forward_ad.dual_level():
+        args[name] = forward_ad.make_dual(args[name], torch.ones_like(args[name]))
+        with pytest.raises(RuntimeError, match="tangent"):
+            Ops().linear_adapted(**args)
+        if name in ("down", "up", "scale"):
+            layer = {n: forward_ad.make_dual(t, t) if n == name else t for n, t in (("down", torch.zeros(2, 4, 60)), ("up", torch.zeros(2, 256, 4)), ("scale", torch.zeros(2)))}
+            with pytest.raises(RuntimeError, match="tangent"):
+                block(linear1=tuple(layer.values()))
