@@ -32,8 +32,18 @@ def _rows(t):
 
 
 class SequenceOps:
-    """Methods of ``MobilePoserNet`` (they use its native handle and device).  A tick's call is host time first: the checks read
-    each property once."""
+    """Methods of ``MobilePoserNet``, on its device.  They need none of its weights: a model that has not loaded any serves them
+    through its body model's handle.  A tick's call is host time first: the checks read each property once."""
+
+    _device_index = None         # set with the model's handle
+
+    def _find_device(self):
+        self._device_index = self.device.index if self.device.index is not None else torch.cuda.current_device()
+
+    def _failed(self, rc, h):
+        if h is self._h:
+            self._check(rc)
+        _lib.check(rc, h)
 
     def _dtype(self, what, first, *more):
         """The common type of the tensors, as the library numbers it; all of them on this model's device."""
@@ -89,7 +99,8 @@ class SequenceOps:
         fp32, ``input_lengths`` [B] (0..T; a list, or an int32 tensor on the device, whose values are clamped), ``state``
         [B, Hv, dk, dv] fp32 or None (zeros), ``scale`` (default dk ** -0.5).
         -> (o [B, T, Hv, dv], zeros behind a sequence's end; the state after each sequence's last frame, fp32)."""
-        self._require_weights()
+        if self._device_index is None:
+            self._find_device()
         _no_grad(q, k, v, g, beta, state)
         dtype = self._dtype("delta_rule", q, k, v)
         Hk, dk, Hv, dv = self._heads("delta_rule", q, k, v, g, beta, 2)
@@ -108,10 +119,13 @@ class SequenceOps:
         need = self._lib.mp_delta_rule_workspace(B, T, Hv, dk, dv)
         ws = torch.empty(need, device=dev, dtype=torch.uint8)
         st = (C.c_int64 * 15)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *g.stride(), *beta.stride())
-        self._check(self._lib.mp_delta_rule(
-            self._h, dtype, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), C.addressof(st),
+        h = self._h or self.bodymodel._handle()[1]
+        rc = self._lib.mp_delta_rule(
+            h, dtype, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), C.addressof(st),
             0 if lens is None else lens.data_ptr(), B, T, Hk, Hv, dk, dv, dk ** -0.5 if scale is None else float(scale), o.data_ptr(),
-            0 if state is None else state.data_ptr(), out.data_ptr(), ws.data_ptr(), need, _stream_of(self._device_index)))
+            0 if state is None else state.data_ptr(), out.data_ptr(), ws.data_ptr(), need, _stream_of(self._device_index))
+        if rc:
+            self._failed(rc, h)
         return o, out
 
     def delta_rule_online(self, q, k, v, g, beta, state, slots=None, scale=None):
@@ -119,7 +133,8 @@ class SequenceOps:
         [n, Hv, dk, dv] fp32 contiguous, updated; ``slots`` [S]: the state of each stream (None: stream s has state s).  A negative
         slot is a stream without a frame (zeros, no state changes); a slot that is not there, or that an earlier stream of the
         call has, gives a row of NaN and changes no state.  -> o [S, Hv, dv]."""
-        self._require_weights()
+        if self._device_index is None:
+            self._find_device()
         _no_grad(q, k, v, g, beta, state)
         dtype = self._dtype("delta_rule_online", q, k, v)
         Hk, dk, Hv, dv = self._heads("delta_rule_online", q, k, v, g, beta, 1)
@@ -136,10 +151,13 @@ class SequenceOps:
         q, k, v = _rows(q), _rows(k), _rows(v)
         o = torch.empty(S, Hv, dv, device=q.device, dtype=q.dtype)
         st = (C.c_int64 * 10)(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *g.stride(), *beta.stride())
-        self._check(self._lib.mp_delta_rule_online(
-            self._h, dtype, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), C.addressof(st),
+        h = self._h or self.bodymodel._handle()[1]
+        rc = self._lib.mp_delta_rule_online(
+            h, dtype, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), C.addressof(st),
             0 if slots is None else slots.data_ptr(), S, n, Hk, Hv, dk, dv, dk ** -0.5 if scale is None else float(scale), o.data_ptr(),
-            state.data_ptr(), _stream_of(self._device_index)))
+            state.data_ptr(), _stream_of(self._device_index))
+        if rc:
+            self._failed(rc, h)
         return o
 
     def _block_adapters(self, adapters, ids, B, shapes):
@@ -170,7 +188,8 @@ class SequenceOps:
         bias [M] or None) with a low-rank adapter per sequence beside it.  x [B, T, K] or, one frame each, [B, K]; down [n, r, K],
         up [n, M, r], r at most 128; ``scale`` [n] fp32 or None (1); ``ids`` [B]: negative = the shared layer alone (a list, or an
         int32 tensor on the device: a value >= n gives rows of NaN); ``relu``: ReLU behind it.  -> [B, T, M] or [B, M]."""
-        self._require_weights()
+        if self._device_index is None:
+            self._find_device()
         _no_grad(x, weight, bias, down, up, scale)
         dtype = self._dtype("linear_adapted", x, weight, down, up, *(() if bias is None else (bias,)))
         if x.dim() not in (2, 3) or weight.dim() != 2 or weight.shape[1] != x.shape[-1]:
@@ -194,8 +213,11 @@ class SequenceOps:
         need = self._lib.mp_linear_adapted_workspace(B, T, r)
         ws = torch.empty(need, device=x.device, dtype=torch.uint8)
         st = (C.c_int64 * 2)(x.stride(0), x.stride(1) if x.dim() == 3 else 0)
-        self._check(self._lib.mp_linear_adapted(
-            self._h, dtype, x.data_ptr(), C.addressof(st), weight.data_ptr(), 0 if bias is None else bias.data_ptr(), down.data_ptr(),
+        h = self._h or self.bodymodel._handle()[1]
+        rc = self._lib.mp_linear_adapted(
+            h, dtype, x.data_ptr(), C.addressof(st), weight.data_ptr(), 0 if bias is None else bias.data_ptr(), down.data_ptr(),
             up.data_ptr(), 0 if scale is None else scale.data_ptr(), ids.data_ptr(), B, T, K, M, n, r, int(bool(relu)), y.data_ptr(),
-            ws.data_ptr(), need, _stream_of(self._device_index)))
+            ws.data_ptr(), need, _stream_of(self._device_index))
+        if rc:
+            self._failed(rc, h)
         return y

@@ -61,3 +61,31 @@ def test_delta_rule_of_buffers_that_end_with_their_last_sequence(ops, shape, dty
         out, want_out = torch.empty_like(state), torch.empty_like(state)
         got = delta_call(ops, *short, lens, state, out, 0.3, shape, strides)
         assert torch.equal(got, delta_call(ops, q, k, v, g, beta, lens, state, want_out, 0.3)) and torch.equal(out, want_out)
+
+
+def test_operators_of_a_model_without_weights(ops):  # noqa: F811
+    """The operators take none of the model's weights: a model that has loaded none gives the same bits, before and after it loads
+    some, and errors of its calls are its own."""
+    import torch
+    from mobileposer_amd import synthetic
+    from mobileposer_amd.net import MobilePoserNet
+    q, k, v, g, beta, state = (t.cuda() for t in F.delta_inputs(8, 2, 40, 1, 2, 32, 24, torch.float32))
+    x, w, b, down, up, scale, ids = (t.cuda() for t in F.linear_inputs(9, 2, 40, 60, 72, 3, 4, torch.float32))
+    def all_of(net):
+        live = state.clone()
+        o, s = net.delta_rule(q, k, v, g, beta, None, state)
+        tick = net.delta_rule_online(q[:, 0], k[:, 0], v[:, 0], g[:, 0], beta[:, 0], live)
+        return o, s, tick, live, net.linear_adapted(x, w, b, down, up, scale, ids)
+    want = all_of(ops)
+    bare = MobilePoserNet(smpl=synthetic.synthetic_smpl(), device="cuda")
+    for i in range(3):
+        assert all(torch.equal(a, c) for a, c in zip(all_of(bare), want))
+        if i == 0:
+            with pytest.raises(RuntimeError, match="frame stride"):
+                bare.delta_rule(*(torch.as_strided(torch.empty(2 ** 24 + 32, device="cuda"), (1, 2, 1, 32), (0, 2 ** 24, 0, 1)) for _ in "qk"),
+                                torch.zeros(1, 2, 1, 8, device="cuda"), torch.zeros(1, 2, 1, device="cuda"), torch.zeros(1, 2, 1, device="cuda"))
+            with pytest.raises(RuntimeError, match="weights"):
+                bare.rnn_forward("joints", torch.zeros(1, 2, 60, device="cuda"), [2], None, {"linear1": (down, up, None)}, [0])
+        if i == 1:
+            bare.load_state_dict(synthetic.make_weights(0))
+    bare.close()
