@@ -513,7 +513,8 @@ static bool launch_for(AdaptArgs a, hipStream_t s) {
             ok = lines ? gemm_for<E, 2, 4, 8, 4, 64, true, false, true>(a, rows, s) : gemm_for<E, 2, 4, 8, 4, 64, true>(a, rows, s);
             return hipGetLastError() == hipSuccess && ok;
         }
-    if (tiles(128) >= (half ? 384 : 192)) ok = half ? gemm_for<E, 2, 2, 4, 4, half ? 64 : 32, false>(a, rows, s) : gemm_for<E, 4, 2, 2, 4, half ? 64 : 32, true>(a, rows, s);
+    constexpr int wr128 = half ? 2 : 4, mr128 = half ? 4 : 2;
+    if (tiles(128) >= (half ? 384 : 192)) ok = gemm_for<E, wr128, 2, mr128, 4, half ? 64 : 32, !half>(a, rows, s);
     else if (tiles(64) >= 256) ok = gemm_for<E, 2, 2, 2, 2, half ? 128 : 64, false>(a, rows, s);
     else ok = gemm_for<E, 2, 2, 1, 1, half ? 256 : 128, false>(a, rows, s);
     return hipGetLastError() == hipSuccess && ok;
