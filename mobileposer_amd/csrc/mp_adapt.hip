@@ -4,7 +4,11 @@
 // Up z joined to it in its registers before the one rounding and the one store (mp_adapt_gemm).  Where a layer's columns and
 // the adapter's components fit one tile side by side (an output layer) and the sequences are long, Down's rows ride in the shared
 // product as further columns and x is read once (mp_adapt_gemm<.., FUSED>).
-// bf16 inputs go to the bf16 matrix instructions as they are, fp32 inputs as three bf16 terms each (mp_seq_dev.h).
+// bf16 inputs go to the bf16 matrix instructions as they are, fp32 inputs as three bf16 terms each (mp_seq_dev.h).  Terms hold no
+// infinity, nor the last half step of bf16 below FLT_MAX (the first term would be infinite, the next ones NaN): a result that is not finite is
+// computed again from the inputs in fp32 (plain_dot, plain_tile).  That keeps infinities what they are in an fp32 product.  It costs a
+// look at every result: no time that can be measured; with one infinite sample 8 x 2048 (2048 -> 2048, bf16) 149 -> 302 us, with nothing
+// but NaN 5.7 ms.
 #include "mp_seq_dev.h"
 
 #include <utility>
@@ -12,6 +16,19 @@
 namespace mpseq {
 
 size_t adapt_ws_floats(int B, int T, int r) { return (size_t)B * T * r; }
+
+static __device__ __forceinline__ bool not_finite(float x) { return !(fabsf(x) <= 3.402823466e38f); }
+template <class E>
+static __device__ __forceinline__ const E* row_of_x(const AdaptArgs& a, int n) {
+    const int b = n / a.T;
+    return (const E*)a.x + (size_t)b * a.sx[0] + (size_t)(n - b * a.T) * a.sx[1];
+}
+template <class E>
+static __device__ __attribute__((noinline)) float plain_dot(const E* x, const E* w, int K) {
+    float s = 0.f;
+    for (int k = 0; k < K; ++k) s = fmaf(load_f(x + k), load_f(w + k), s);
+    return s;
+}
 
 // ---------------------------------------------------------------- z = scale Down x
 // A workgroup takes up to 16 RG frames of one sequence -- one adapter, so the product runs on the matrix units even where the rows
@@ -80,7 +97,11 @@ MP_KERNEL __launch_bounds__(256) void mp_adapt_down(AdaptArgs a, int per_seq) {
     const float sc = a.scale ? a.scale[id] : 1.f;
     for (int i = tid; i < NR * a.r; i += 256) {
         const int row = i / a.r, c = i % a.r;
-        if (t0 + row < a.T) a.ws[((size_t)b * a.T + t0 + row) * a.r + c] = sc * ((part[0][c][row] + part[1][c][row]) + (part[2][c][row] + part[3][c][row]));
+        if (t0 + row < a.T) {
+            float z = (part[0][c][row] + part[1][c][row]) + (part[2][c][row] + part[3][c][row]);
+            if (P > 1 && not_finite(z)) z = plain_dot(row_of_x<E>(a, b * a.T + t0 + row), (const E*)a.down + ((size_t)id * a.r + c) * a.K, a.K);
+            a.ws[((size_t)b * a.T + t0 + row) * a.r + c] = sc * z;
+        }
     }
 }
 
@@ -106,6 +127,52 @@ struct Gemm {
     static constexpr int kBytes = FUSED ? (kZ > RN * kRowZ * 4 ? kZ : RN * kRowZ * 4) : kZ;      // (z takes the operands' place)
     static_assert((RN + CM) * UR % TH == 0 && kBytes <= 160 * 1024, "whole pieces per thread, LDS of a CU");
 };
+// Outputs of rows n .. n + 15 and columns m .. m + 15 that are not finite, from the inputs on the fp32 matrix instructions (a wave; z: of
+// the lane's row n + lane % 16)
+template <class E>
+static __device__ __forceinline__ void plain_tile(const AdaptArgs& a, int n, int n1, int m, const float* z) {
+    const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4, row = min(n + col, n1 - 1), b = row / a.T, id = a.ids[b];
+    E* const y = (E*)a.y + (size_t)b * a.sy[0] + (size_t)(row - b * a.T) * a.sy[1];
+    bool odd[4], any = false;
+    for (int r = 0; r < 4; ++r) {
+        const int c = m + 4 * grp + r;
+        odd[r] = n + col < n1 && c < a.M && id < a.n && not_finite(load_f(y + min(c, a.M - 1)));
+        any = any || odd[r];
+    }
+    if (!__any(any)) return;
+    const E* x = row_of_x<E>(a, row);
+    const E* w = (const E*)a.w + (size_t)min(m + col, a.M - 1) * a.ldw;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    int k = 4 * grp;
+    for (; k - 4 * grp + 64 <= a.K; k += 64) {                    // four steps' loads in flight together
+        E fw[4][4], fx[4][4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            __builtin_memcpy(fw[u], w + k + 16 * u, 4 * sizeof(E));
+            __builtin_memcpy(fx[u], x + k + 16 * u, 4 * sizeof(E));
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(load_f(&fw[u][i]), load_f(&fx[u][i]), acc, 0, 0, 0);
+    }
+    for (; k - 4 * grp < a.K; k += 16)
+        for (int i = 0; i < 4; ++i) {
+            const bool on = k + i < a.K;
+            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(on ? load_f(w + k + i) : 0.f, on ? load_f(x + k + i) : 0.f, acc, 0, 0, 0);
+        }
+    for (int r = 0; r < 4; ++r) {
+        if (!odd[r]) continue;
+        const int c = m + 4 * grp + r;
+        float v = acc[r] + (a.bias ? load_f((const E*)a.bias + c) : 0.f);
+        if (id >= 0) {
+            float s = 0.f;
+            for (int q = 0; q < a.r; ++q) s = fmaf(load_f((const E*)a.up + ((size_t)id * a.M + c) * a.r + q), z[q], s);
+            v += s;
+        }
+        store_f(y + c, a.relu ? relu_(v) : v);
+    }
+}
 template <class F, int... I>
 static __device__ __forceinline__ void each_of(F& f, std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }
 // where the piece (row % 16, group of eight elements 0..3) of a block lies
@@ -313,6 +380,7 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
     float* zl = (float*)gemm_lds;                                 // FUSED: [RN][kRowZ]
     if (FUSED && adapt) {
         const float sc = a.scale ? a.scale[sid] : 1.f;
+        float bad = 0.f;                                          // stays 0 while everything is finite
 #pragma unroll
         for (int j = 0; j < MC; ++j) {
             const int m = (wc * MC + j) * 16 - Mp + 4 * grp;
@@ -321,9 +389,20 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
                 for (int i = 0; i < MR; ++i)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        if (m + r < rlen) zl[((wr * MR + i) * 16 + col) * G::kRowZ + m + r] = sc * acc[j][i][r];
+                        if (m + r < rlen) {
+                            zl[((wr * MR + i) * 16 + col) * G::kRowZ + m + r] = sc * acc[j][i][r];
+                            bad = fmaf(0.f, acc[j][i][r], bad);
+                        }
         }
-        __syncthreads();
+        if (P == 1) __syncthreads();
+        else if (__syncthreads_or(bad != 0.f)) {
+            for (int i = tid; i < RN * rlen; i += TH) {
+                const int row = i / rlen, c = i % rlen;
+                float* const z = zl + row * G::kRowZ + c;
+                if (n0 + row < n1 && not_finite(*z)) *z = sc * plain_dot(row_of_x<E>(a, n0 + row), (const E*)a.down + ((size_t)sid * a.r + c) * a.K, a.K);
+            }
+            __syncthreads();
+        }
     }
     // the adapters, for all rows of the wave at once where they share one
     bool same = true;
@@ -379,6 +458,7 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
         const int b = flat ? 0 : n / a.T;
         return (E*)a.y + (size_t)b * a.sy[0] + (size_t)(n - b * a.T) * a.sy[1];
     };
+    float odd = 0.f;                                              // stays 0 while every result is finite
     auto finish = [&](auto tile_row) {
         constexpr int i = decltype(tile_row)::value;
         const int nt0 = n0 + (wr * MR + i) * 16, n = nt0 + col;    // 16 rows, one per lane column
@@ -416,6 +496,7 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 y[r] = acc[j][i][r] + bias[j][r];
+                odd = fmaf(0.f, y[r], odd);
                 if (id[i] >= a.n) y[r] = __builtin_nanf("");
                 if (a.relu) y[r] = relu_(y[r]);
             }
@@ -458,6 +539,14 @@ MP_KERNEL __launch_bounds__(64 * WR * WC, WR * WC >= 8 ? 2 : 1) void mp_adapt_ge
         }
     };
     each_of(finish, std::make_integer_sequence<int, MR>{});
+    if (__any(odd != 0.f)) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "agent");        // (the outputs are looked at again)
+#pragma unroll 1
+        for (int t = 0; t < MR * MC; ++t) {
+            const int n = n0 + (wr * MR + t % MR) * 16, m = m0 + (wc * MC + t / MR) * 16, row = min(n + col, n1 - 1);
+            if (n < n1 && m < a.M) plain_tile<E>(a, n, n1, m, FUSED ? zl + (row - n0) * G::kRowZ : a.ws + (size_t)row * rlen);
+        }
+    }
 }
 
 template <class E, int WR, int WC, int MR, int MC, int BK, bool TWO, bool FUSED = false, bool DIRECT = false>
