@@ -11,6 +11,7 @@
 // same step time; graph mode 1 means mode 2 (single-branch) unless the environment asks for the real thing (mp_handle.hip
 // multibranch_graphs_allowed).
 #include "mp_host.h"
+#include "mp_seq.h"
 
 // ================================================================================================ C ABI
 extern "C" {
@@ -160,7 +161,7 @@ int mp_rnn_forward_adapted(mp_handle* h, int module, const float* x_dev, const i
     const size_t need = mp_linear_adapted_workspace(B, T, r);
     if (need && (!ws_dev || ws_bytes < need || (uintptr_t)ws_dev % 16))
         return fail(h, MP_ERR_INVALID, "mp_rnn_forward_adapted: workspace of %zu bytes, %zu needed (16-byte aligned)", ws_bytes, need);
-    if ((int64_t)B * T > (int64_t)1 << 30 || (int64_t)B * T * r > (int64_t)0x7fffffff)
+    if (r && !mpseq::adapt_fits(B, T, 512, r))
         return fail(h, MP_ERR_INVALID, "mp_rnn_forward_adapted: %d x %d frames are too many for one call", B, T);
     if (use_x3(h, h->mod[module]))               // (its linear layers hand their rows over as pairs of halves)
         return fail(h, MP_ERR_INVALID, "mp_rnn_forward_adapted runs on exact-fp32 operands (LSTM mode 1 or 0)");

@@ -896,15 +896,23 @@ MP_KERNEL __launch_bounds__(256) void mp_delta_online(DeltaOnlineArgs a, int nti
     }
 }
 
+// 8 .. 32 threads side by side in a row of the state; 64 where they hold single columns: a row that two workgroups share is
+// written in parts of cache lines (77 streams, 6 heads of 96 x 41: 8.6 us against 12.0 with 32, 14.2 with 16) -- up to dk = 128,
+// where a thread holds 32 rows
+static bool online_vec(const DeltaOnlineArgs& a) { return a.dv % 4 == 0 && (uintptr_t)a.state % 16 == 0; }
+static int online_log_lanes(const DeltaOnlineArgs& a, int vec) {
+    int lg = 3;
+    while (lg < (vec == 1 && a.dk <= 128 ? 6 : 5) && (1 << lg) < (a.dv + vec - 1) / vec) ++lg;
+    return lg;
+}
+static int online_tiles(const DeltaOnlineArgs& a, int vec, int lg) { return (int)((((int64_t)a.dv + vec - 1) / vec + (1 << lg) - 1) >> lg); }
+int64_t delta_online_blocks(const DeltaOnlineArgs& a) {
+    const int vec = online_vec(a) ? 4 : 1;
+    return (int64_t)a.S * a.Hv * online_tiles(a, vec, online_log_lanes(a, vec));
+}
 template <class E, int VEC>
 static void online_for(const DeltaOnlineArgs& a, hipStream_t s) {
-    const int need = (a.dv + VEC - 1) / VEC;
-    // 8 .. 32 threads side by side in a row of the state; 64 where they hold single columns: a row that two workgroups share is
-    // written in parts of cache lines (77 streams, 6 heads of 96 x 41: 8.6 us against 12.0 with 32, 14.2 with 16) -- up to dk = 128,
-    // where a thread holds 32 rows
-    int lg = 3;
-    while (lg < (VEC == 1 && a.dk <= 128 ? 6 : 5) && (1 << lg) < need) ++lg;
-    const int ntile = (need + (1 << lg) - 1) >> lg, rows = 256 >> lg, nr = (a.dk + rows - 1) / rows;
+    const int lg = online_log_lanes(a, VEC), ntile = online_tiles(a, VEC, lg), rows = 256 >> lg, nr = (a.dk + rows - 1) / rows;
     const size_t lds = (2 * (size_t)a.dk + 8 * (size_t)(VEC << lg)) * sizeof(float);
     const dim3 grid((unsigned)((size_t)a.S * a.Hv * ntile)), block(256);
     if (nr <= 2) hipLaunchKernelGGL((mp_delta_online<E, VEC, 2>), grid, block, lds, s, a, ntile, lg);
@@ -914,7 +922,7 @@ static void online_for(const DeltaOnlineArgs& a, hipStream_t s) {
     else hipLaunchKernelGGL((mp_delta_online<E, VEC, 32>), grid, block, lds, s, a, ntile, lg);
 }
 bool launch_delta_online(const DeltaOnlineArgs& a, int dtype, hipStream_t s) {
-    const bool vec = a.dv % 4 == 0 && (uintptr_t)a.state % 16 == 0;
+    const bool vec = online_vec(a);
     if (dtype == kBF16) { if (vec) online_for<bf16raw, 4>(a, s); else online_for<bf16raw, 1>(a, s); }
     else { if (vec) online_for<float, 4>(a, s); else online_for<float, 1>(a, s); }
     return hipGetLastError() == hipSuccess;

@@ -45,6 +45,7 @@ struct DeltaOnlineArgs {
 };
 size_t delta_ws_floats(int B, int T, int Hv, int dk, int dv);
 bool launch_delta(const DeltaArgs& a, int dtype, hipStream_t s);
+int64_t delta_online_blocks(const DeltaOnlineArgs& a);        // workgroups of 256 threads
 bool launch_delta_online(const DeltaOnlineArgs& a, int dtype, hipStream_t s);
 
 // ---------------------------------------------------------------- linear layer with an adapter per sequence
@@ -63,6 +64,7 @@ struct AdaptArgs {
     int vec;                                     // (set by the launcher) columns of y that can be stored at once: 2: 16 bytes, 1: four, 0: one
 };
 size_t adapt_ws_floats(int B, int T, int r);
+bool adapt_fits(int B, int T, int M, int r);     // one call's launches can count these rows and columns
 bool launch_adapt(const AdaptArgs& a, int dtype, hipStream_t s);
 
 }  // namespace mpseq

@@ -7,7 +7,8 @@
 
 namespace {
 
-constexpr int64_t kMaxBlocks = 0x7fffffff;
+// A launch counts its threads in 32 bits: so many workgroups of 256 or of 64 threads.
+constexpr int64_t kMaxBlocks = (1 << 24) - 1, kMaxBlocks64 = (1 << 26) - 1;
 
 int bad_type(mp_handle* h, const char* what, int dtype) {
     return fail(h, MP_ERR_INVALID, "%s: dtype %d (MP_F32 = 0 or MP_BF16 = 1)", what, dtype);
@@ -37,7 +38,7 @@ int mp_delta_rule(mp_handle* h, int dtype, const void* q_dev, const void* k_dev,
     if (need && (!ws_dev || ws_bytes < need || (uintptr_t)ws_dev % 16))
         return fail(h, MP_ERR_INVALID, "mp_delta_rule: workspace of %zu bytes, %zu needed (16-byte aligned)", ws_bytes, need);
     const int64_t nchunk = ((int64_t)T + 31) / 32;
-    if ((int64_t)B * Hk * nchunk > kMaxBlocks || ((int64_t)B * Hk + 7) * (Hv / Hk) * (((int64_t)dv + 63) / 64) > kMaxBlocks ||
+    if ((int64_t)B * Hk * nchunk > kMaxBlocks64 || ((int64_t)B * Hk + 7) * (Hv / Hk) * (((int64_t)dv + 63) / 64) > kMaxBlocks ||
         (int64_t)Hv * dv > (1 << 24) - 1)
         return fail(h, MP_ERR_INVALID, "mp_delta_rule: batch of %d x %d frames, %d heads is too large for one call", B, T, Hv);
     ON_DEVICE(h);
@@ -69,8 +70,6 @@ int mp_delta_rule_online(mp_handle* h, int dtype, const void* q_dev, const void*
     if (!q_dev || !k_dev || !v_dev || !g_dev || !beta_dev || !strides || !o_dev || !state_dev || n_slots < 1)
         return fail(h, MP_ERR_INVALID, "mp_delta_rule_online: NULL buffer or no state");
     if (!slots_dev && S > n_slots) return fail(h, MP_ERR_INVALID, "mp_delta_rule_online: %d streams on %d states without slots", S, n_slots);
-    if ((int64_t)S * Hv * (((int64_t)dv + 7) / 8) > kMaxBlocks)
-        return fail(h, MP_ERR_INVALID, "mp_delta_rule_online: %d streams of %d heads are too many for one call", S, Hv);
     ON_DEVICE(h);
     mpseq::DeltaOnlineArgs a;
     a.q = q_dev; a.k = k_dev; a.v = v_dev; a.g = g_dev; a.beta = beta_dev;
@@ -79,6 +78,8 @@ int mp_delta_rule_online(mp_handle* h, int dtype, const void* q_dev, const void*
     }
     a.slots = slots_dev; a.S = S; a.n_slots = n_slots; a.Hk = Hk; a.Hv = Hv; a.dk = dk; a.dv = dv; a.scale = scale;
     a.o = o_dev; a.state = state_dev;
+    if (mpseq::delta_online_blocks(a) > kMaxBlocks)
+        return fail(h, MP_ERR_INVALID, "mp_delta_rule_online: %d streams of %d heads are too many for one call", S, Hv);
     if (!mpseq::launch_delta_online(a, dtype, (hipStream_t)stream)) return fail(h, MP_ERR_HIP, "mp_delta_rule_online: launch failed");
     return MP_OK;
 }
@@ -100,8 +101,7 @@ int mp_linear_adapted(mp_handle* h, int dtype, const void* x_dev, const int64_t 
     const size_t need = mp_linear_adapted_workspace(B, T, r);
     if (!ws_dev || ws_bytes < need || (uintptr_t)ws_dev % 16)
         return fail(h, MP_ERR_INVALID, "mp_linear_adapted: workspace of %zu bytes, %zu needed (16-byte aligned)", ws_bytes, need);
-    if ((int64_t)B * T > (int64_t)1 << 30 || (int64_t)B * T * r > (int64_t)kMaxBlocks || ((int64_t)M + 15) / 16 > 65535 ||
-        ((int64_t)B * T + 31) / 32 * (((int64_t)M + 31) / 32) > kMaxBlocks - 8)
+    if (!mpseq::adapt_fits(B, T, M, r))
         return fail(h, MP_ERR_INVALID, "mp_linear_adapted: %d x %d rows to %d columns are too many for one call", B, T, M);
     ON_DEVICE(h);
     mpseq::AdaptArgs a;

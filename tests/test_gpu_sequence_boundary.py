@@ -89,3 +89,32 @@ def test_operators_of_a_model_without_weights(ops):  # noqa: F811
         if i == 1:
             bare.load_state_dict(synthetic.make_weights(0))
     bare.close()
+
+
+def test_calls_with_more_threads_than_a_launch_counts_are_refused(ops):  # noqa: F811
+    """A launch counts its threads in 32 bits.  Calls that need more are refused before anything runs (their buffers here are a few
+    bytes), the ones below are not: 2^20 streams of 15 heads run."""
+    import torch
+    from mobileposer_amd import _lib
+    some = torch.zeros(1024, device="cuda")
+    p, lib, h = some.data_ptr(), ops._lib, ops._h
+    ids = torch.zeros(4, device="cuda", dtype=torch.int32).data_ptr()
+    st = (C.c_int64 * 15)(*[0] * 15)
+    at = C.addressof(st)
+    huge = 2 ** 40                                       # (a workspace's size is what the caller says)
+    refused = [lambda: lib.mp_delta_rule_online(h, 0, p, p, p, p, p, at, None, 2 ** 24, 2 ** 24, 1, 1, 4, 4, 1.0, p, p, None),
+               lambda: lib.mp_delta_rule_online(h, 0, p, p, p, p, p, at, None, 2 ** 20, 2 ** 20, 1, 16, 4, 4, 1.0, p, p, None),
+               lambda: lib.mp_delta_rule(h, 0, p, p, p, p, p, at, None, 2 ** 24, 1, 1, 1, 4, 4, 1.0, p, None, None, p, huge, None),
+               lambda: lib.mp_delta_rule(h, 0, p, p, p, p, p, at, None, 2 ** 20, 32 * 64, 1, 1, 4, 4, 1.0, p, None, None, p, huge, None),
+               lambda: lib.mp_linear_adapted(h, 0, p, at, p, p, p, p, p, ids, 2 ** 24, 1, 4, 4, 1, 1, 0, p, p, huge, None),
+               lambda: lib.mp_linear_adapted(h, 1, p, at, p, p, p, p, p, ids, 1, 2 ** 20, 4, 2 ** 20, 1, 1, 0, p, p, huge, None)]
+    for call in refused:
+        assert call() == _lib.MP_ERR_INVALID and "too" in _lib.last_error(h)
+    S, H = 2 ** 20, 15
+    q, k, v = (torch.randn(S, n, 4, device="cuda") for n in (1, 1, H))
+    g, beta, state = -torch.rand(S, H, device="cuda"), torch.rand(S, H, device="cuda"), torch.randn(S, H, 4, 4, device="cuda")
+    rows = torch.tensor([0, 1, 7, S // 2, S - 1], device="cuda")
+    part = state[rows].clone()
+    o = ops.delta_rule_online(q, k, v, g, beta, state)
+    want = ops.delta_rule_online(q[rows], k[rows], v[rows], g[rows], beta[rows], part)
+    assert torch.equal(o[rows], want) and torch.equal(state[rows], part)
