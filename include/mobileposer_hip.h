@@ -278,20 +278,23 @@ int mp_live_form_frames(mp_handle* h, const float* quat_dev, const float* acc_de
  * layers).  Inputs of two types; fp32 accumulation and state in both.  Unlike the network entry points these run on the
  * caller's stream itself and use no memory of the handle: calls on several streams are independent, a call can be captured
  * into the caller's graph (lengths, slots and ids are device memory and read on replay), every kind of handle serves them.
- * They return without waiting; an output buffer overlaps an input only where that is said.  Replaces: nothing in the
- * reference. */
+ * They return without waiting; an output buffer overlaps an input only where that is said.  bf16 operands enter the products as
+ * they are, fp32 ones (the state, and whatever is computed between two products, for both types) as three bf16 terms: all 24 bits.
+ * Calls whose launches would need more threads than 32 bits count are refused.  Replaces: nothing in the reference. */
 enum { MP_F32 = 0, MP_BF16 = 1 };
 
 /* Gated delta rule over B ragged sequences: per value head a state S [dk][dv] and per frame
  *     S <- e^g S;   u = beta (v - S^T k);   S <- S + k u^T;   o = scale S^T q.
  *   q_dev, k_dev [B,T,Hk,dk], v_dev [B,T,Hv,dv] (dtype), g_dev, beta_dev [B,T,Hv] (fp32); value head i uses key head
  *                i / (Hv / Hk).  g is the logarithm of the decay: g <= 0 (below -1e4 it counts as -1e4: the state is cleared).
- *   strides      15 values, in elements: (batch, frame, head) of q, k, v, g, beta; the last dimension of q, k, v is contiguous
- *   lengths_dev  [B] int32 or NULL (all T); values are clamped to 0..T.  Inputs behind a sequence's end are not read.
+ *   strides      15 values, in elements: (batch, frame, head) of q, k, v, g, beta; the last dimension of q, k, v is contiguous, frame
+ *                strides of q, k and v are 0 .. 2^24 - 1
+ *   lengths_dev  [B] int32 or NULL (all T); values are clamped to 0..T.  Inputs behind a sequence's end are not read (they need no memory).
  *   o_dev        [B,T,Hv,dv] (dtype), contiguous; frames behind a sequence's end are zeros (as pad_packed_sequence has them)
  *   state_in_dev [B,Hv,dk,dv] fp32 or NULL (zeros);  state_out_dev the same or NULL; both may be the same buffer
  *   ws_dev       mp_delta_rule_workspace(B, T, Hv, dk, dv) bytes, 16-byte aligned: the caller's until the call's work is done
- * dk is at most 256.  A value that is not finite reaches the outputs of its own and later frames only. */
+ * dk is at most 256.  A value that is not finite, or beyond 3.39e38, makes the outputs of its own and later frames NaN, and none before
+ * them (in v and in the state: those of its own column). */
 int mp_delta_rule(mp_handle* h, int dtype, const void* q_dev, const void* k_dev, const void* v_dev, const float* g_dev,
                   const float* beta_dev, const int64_t strides[15], const int32_t* lengths_dev, int B, int T, int Hk, int Hv,
                   int dk, int dv, float scale, void* o_dev, const float* state_in_dev, float* state_out_dev, void* ws_dev,
@@ -312,7 +315,8 @@ int mp_delta_rule_online(mp_handle* h, int dtype, const void* q_dev, const void*
  *   x_dev [B,T,K] (dtype; strides: (batch, frame) in elements, the last dimension contiguous), w_dev [M,K], bias_dev [M] or NULL,
  *   down_dev [n,r,K], up_dev [n,M,r] (dtype, contiguous), scale_dev [n] fp32 or NULL (1), ids_dev [B] int32: negative = the shared
  *   layer alone, >= n = the sequence's rows are NaN;  y_dev [B,T,M] (dtype, contiguous);  1 <= r <= 128.
- *   ws_dev: mp_linear_adapted_workspace(B, T, r) bytes, 16-byte aligned. */
+ *   ws_dev: mp_linear_adapted_workspace(B, T, r) bytes, 16-byte aligned.
+ * Infinities and NaN are what fp32 sums make of them (scale[a] belongs to the inner product, scale[a] (down[a] x)). */
 int mp_linear_adapted(mp_handle* h, int dtype, const void* x_dev, const int64_t strides[2], const void* w_dev, const void* bias_dev,
                       const void* down_dev, const void* up_dev, const float* scale_dev, const int32_t* ids_dev, int B, int T, int K,
                       int M, int n_adapters, int r, int relu, void* y_dev, void* ws_dev, size_t ws_bytes, void* stream);

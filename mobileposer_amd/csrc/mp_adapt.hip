@@ -31,7 +31,7 @@ static __device__ __forceinline__ const E* row_of_x(const AdaptArgs& a, int n) {
     return (const E*)a.x + (size_t)b * a.sx[0] + (size_t)(n - b * a.T) * a.sx[1];
 }
 template <class E>
-static __device__ __attribute__((noinline)) float plain_dot(const E* x, const E* w, int K) {
+static __device__ __forceinline__ float plain_dot(const E* x, const E* w, int K) {
     float s = 0.f;
     for (int k = 0; k < K; ++k) s = fmaf(load_f(x + k), load_f(w + k), s);
     return s;
@@ -41,7 +41,7 @@ static __device__ __attribute__((noinline)) float plain_dot(const E* x, const E*
 // A workgroup takes up to 16 RG frames of one sequence -- one adapter, so the product runs on the matrix units even where the rows
 // are one (a tick: the reads of Down bound it either way) --, K split over the four waves and joined through LDS; KB steps of
 // every wave are in flight together.  RT = r / 16 rounded up.  Bound by the latency of one pass for a tick (512 x 1, 1024, r 16: 6 us), by
-// the reads of x and Down together for long sequences (8 x 2048, 2048, r 32: 18 us, 67 MB of x and as many of Down, those from L2).
+// the reads of x and Down together for long sequences (8 x 2048, 2048, r 32: 18 .. 20 us, 67 MB of x and as many of Down, those from L2).
 template <class E, int RT, int RG>
 MP_KERNEL __launch_bounds__(256) void mp_adapt_down(AdaptArgs a, int per_seq) {
     constexpr int P = Arith<E>::P, KB = RT >= 4 ? 2 : 4, NR = 16 * RG;
@@ -122,7 +122,7 @@ MP_KERNEL __launch_bounds__(256) void mp_adapt_down(AdaptArgs a, int per_seq) {
 // multiplied.  BK is as long as the staging registers allow: a small tile is a chain of memory latencies.  FUSED: a row tile lies
 // inside one sequence, columns Mp .. Mp + r - 1 of the tile (Mp = M rounded up to 16) are that sequence's Down.  DIRECT (bf16, rows of
 // whole cache lines): tiles go from memory to LDS without registers, 8 rows x 128 bytes a wave and instruction, the pieces of a row
-// exchanged by its index; the fragments are read between the products.  8 x 2048, 2048 -> 2048, r 32: 126 us, 1090 TFLOP/s (the
+// exchanged by its index; the fragments are read between the products.  8 x 2048, 2048 -> 2048, r 32: 126 .. 137 us, 1090 .. 1000 TFLOP/s (the
 // library's product: 1180), 1.35 us per step of K beside 0.85 of products alone, 18 us for loads before and stores behind;
 // 256 x 125, 512 -> 96, r 8, fp32 (FUSED): 29 us, 2.8 TB/s, 1.4 us per step of K beside 0.64 of products alone (LDS and splitting the rest).
 template <class E, int WR, int WC, int MR, int MC, int BK, bool TWO, bool FUSED, bool DIRECT>

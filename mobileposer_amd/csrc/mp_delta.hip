@@ -12,9 +12,9 @@
 // cost the frames behind it their low bits if G were a float, and e^{G_i} / e^{G_j} would be 0 / 0.  g below -1e4 counts as -1e4
 // (e^-104 already is 0 in fp32).
 //
-// A value that is not finite reaches the frames behind it only, as in the recurrence: where a right-hand side holds one, the
-// rows from there on are taken out of the products (0 * NaN in a triangular matrix's zeros would reach the frames before it)
-// and their outputs and the column's state are NaN.
+// A value that is not finite (or too large for a first bf16 term, 3.396e38) reaches the frames behind it only, as in the recurrence: where a
+// right-hand side holds one, the rows from there on are taken out of the products (0 * NaN in a triangular matrix's zeros would
+// reach the frames before it) and their outputs and the column's state are NaN.
 #include "mp_seq_dev.h"
 
 namespace mpseq {
@@ -79,7 +79,7 @@ static __device__ __forceinline__ double lane_below(double x) {
 // (I + A)^{-1} by forward substitution on the two 16 x 16 diagonal blocks -- a lane of two groups of 16 solves a column; stable
 // where keys repeat and A is far from small, products of powers of A are not -- and T21 = -T22 A21 T11 on the fp32 matrix
 // instructions.  KB: steps of 32 components whose loads are in flight together.  Bound by memory, its own output being the larger part:
-// 8 x 2048 frames, 8 / 16 heads of 128, bf16 34 us (4.5 TB/s), 256 x 125 frames, 4 heads of 64, fp32 22 us.
+// 8 x 2048 frames, 8 / 16 heads of 128, bf16 36 us (149 MB, 4.1 TB/s), 256 x 125 frames, 4 heads of 64, fp32 22 us.
 template <class E, int MODE, int KB>
 MP_KERNEL __launch_bounds__(64) void mp_delta_prep(DeltaArgs a) {
     constexpr int P = Arith<E>::P, LS = kC + 4;
@@ -246,8 +246,8 @@ MP_KERNEL __launch_bounds__(64) void mp_delta_prep(DeltaArgs a) {
 // K^T comes from K's operands by the turning reads), the chunk's workspace, the 64 columns of V, whose place the outputs take --
 // and the next chunk is on its way through registers meanwhile, with no use of its values before this chunk's products are done.
 // Bound by the chain of a chunk -- products with S, U, products with U, the new S split into terms again -- whose steps overlap between
-// waves only: 8 x 2048 frames, 16 heads of 128, bf16 153 us, 2.4 us a chunk, the matrix units busy 18 % of it; 256 x 125, 4 heads of 64,
-// fp32 48 us.  Two waves per 16 columns (each half of dk) took as long: what they share goes through LDS once more.
+// waves only: 8 x 2048 frames, 16 heads of 128, bf16 165 us, 2.6 us a chunk, the matrix units busy 20 % of it; 256 x 125, 4 heads of 64,
+// fp32 48 us (17 %).  Two waves per 16 columns (each half of dk) took as long: what they share goes through LDS once more.
 constexpr int kFragK = kFrag + 256;               // K's operands: 64 bytes between the groups of eight components, or the 16 lanes of a
                                                   // turning read would meet in a quarter of the banks
 template <class E, int NK>
@@ -719,10 +719,11 @@ MP_KERNEL __launch_bounds__(KT <= 4 ? 256 : 512) void mp_delta_join(DeltaArgs a,
 }
 
 // Segments: as many as give the first pass two workgroups a CU, at least four chunks each; from four segments on they win (3 x the
-// work in 2 / segments of the steps): 1 x 512 frames, 4 heads of 64, bf16 35 -> 31 us (fp32 54 -> 41), 1 x 3000 161 -> 50 (262 -> 62),
-// 1 x 32768 1641 -> 144 (2726 -> 183).  Where that makes no more than eight, and two workgroups of this kernel share a CU, twice as
-// many: 2 x 4096, 32 heads of 64, bf16 147 -> 134 (fp32 236 -> 212), 4 x 4096, 16 heads of 128, bf16 320 -> 302 (fp32, one a CU, 567
-// -> 585); with more the join, whose steps are one after the other, takes what the passes gain (1 x 32768, 4 heads, 144 -> 199).
+// work in 2 / segments of the steps): 1 x 384 frames (three), 4 heads of 64, bf16 30.0 -> 31.3 us (fp32 41.9 -> 39.1), 1 x 512 36.3 -> 31.7
+// (51.7 -> 39.9), 1 x 3000 166 -> 46 (248 -> 56), 1 x 32768 1683 -> 129 (2566 -> 162).  Where that makes no more than eight, and two
+// workgroups of this kernel share a CU, twice as many: 2 x 4096, 32 heads of 64, bf16 160 -> 147 (fp32 247 -> 229), 4 x 4096, 16 heads of
+// 128, bf16 347 -> 350 (fp32, one a CU, 597 -> 645); with more the join, whose steps are one after the other, takes what the passes
+// gain (1 x 32768, 4 heads, 129 -> 160, fp32 162 -> 190).
 static DeltaPlan plan_of(int B, int T, int Hv, int dk, int dv, bool two) {
     DeltaPlan p = {1, (T + kC - 1) / kC, nullptr, nullptr, nullptr};
     const long per = (long)B * Hv * ((dv + 63) / 64 + (dk + 63) / 64);
@@ -797,8 +798,9 @@ bool launch_delta(const DeltaArgs& a, int dtype, hipStream_t s) {
 // ---------------------------------------------------------------- one frame per stream
 // A workgroup owns (stream, value head, tile of columns): its part of the state is read once into registers -- a thread holds
 // VEC columns of NR rows --, S^T k and S^T q are reduced together (o = e^g S^T q + (k . q) u needs no second pass), and the updated
-// state is written once.  HBM-bound: 8 dk dv bytes per stream and head (512 streams, 16 heads of 128 x 128: 217 us, 4.98 TB/s; a copy
-// reaches 5.08).
+// state is written once.  HBM-bound: 8 dk dv bytes per stream and head (512 streams, 16 heads of 128 x 128: 217 us, 4.94 TB/s, on one
+// set of states or on six in turn; a copy reaches 5.08).  With slots a stream looks through those of the streams before it, whose
+// number's square is nothing to 2048 streams (4 heads of 64 x 64: 48 us) and half of the call at 65536 (1.6 -> 3.5 ms).
 template <class E, int VEC, int NR>
 MP_KERNEL __launch_bounds__(256) void mp_delta_online(DeltaOnlineArgs a, int ntile, int log_lanes) {
     extern __shared__ float tick_lds[];               // k [dk] | q [dk] | partial sums [4 waves][2][lanes * VEC]

@@ -3,8 +3,8 @@
 // An fp32 value as three bf16 terms -- each the nearest to what the ones before it leave -- keeps all 24 bits, and a product of two
 // such values is six products of terms: the three left out are below 2^-26 of it.  With fp32 accumulation that is the accuracy of
 // an fp32 sum at 16 / 6 times the rate of the fp32 matrix instructions; beside a bf16 operand, which is its own only term, it is
-// three products.  (An infinite value, or one above the largest bf16 by half a step, 3.396e38, gives
-// NaN terms: inf - inf in the split.)
+// three products.  (An infinite value, or one above the largest bf16 by half a step, 3.396e38, gives NaN terms: inf - inf in the
+// split.)
 #pragma once
 #include "mp_seq.h"
 

@@ -95,7 +95,8 @@ class SequenceOps:
         """The gated delta rule over B ragged sequences: per value head a state S [dk, dv] and per frame
         ``S = exp(g) S; u = beta (v - S^T k); S = S + k u^T; o = scale S^T q``.
 
-        q, k [B, T, Hk, dk], v [B, T, Hv, dv] (fp32 or bf16; views of one projection's rows are fine), g (<= 0), beta [B, T, Hv]
+        q, k [B, T, Hk, dk], v [B, T, Hv, dv] (fp32 or bf16; views of one projection's rows are fine, frames less than 2^24 elements
+        apart; what lies behind a sequence's end is not read), g (<= 0), beta [B, T, Hv]
         fp32, ``input_lengths`` [B] (0..T; a list, or an int32 tensor on the device, whose values are clamped), ``state``
         [B, Hv, dk, dv] fp32 or None (zeros), ``scale`` (default dk ** -0.5).
         -> (o [B, T, Hv, dv], zeros behind a sequence's end; the state after each sequence's last frame, fp32)."""
