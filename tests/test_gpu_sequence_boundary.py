@@ -118,3 +118,42 @@ def test_calls_with_more_threads_than_a_launch_counts_are_refused(ops):  # noqa:
     o = ops.delta_rule_online(q, k, v, g, beta, state)
     want = ops.delta_rule_online(q[rows], k[rows], v[rows], g[rows], beta[rows], part)
     assert torch.equal(o[rows], want) and torch.equal(state[rows], part)
+
+
+def near(a, b):
+    """Within two roundings of the outputs' type and what 128-long fp32 sums in another order leave."""
+    return float((a.float() - b.float()).abs().max()) <= 2.0 ** -7 * float(b.float().abs().max())
+
+
+def test_buffers_of_more_than_2_31_elements(ops):  # noqa: F811
+    """Rows, frames and states whose offsets pass 32 bits: the last ones are what a small call gives for them (4 to 10 GB a buffer)."""
+    import torch
+    bf = torch.bfloat16
+    gen = torch.Generator(device="cuda").manual_seed(12)
+    rn = lambda *s, dtype=bf: torch.randn(*s, generator=gen, device="cuda", dtype=dtype)
+    x, w, down, up = rn(9, 130000, 2048), rn(2048, 2048), rn(3, 8, 2048), rn(3, 2048, 8)
+    assert x.numel() > 2 ** 31
+    ids = torch.tensor([2, 0, 1, -1, 2, 0, 1, -1, 2], device="cuda", dtype=torch.int32)
+    y = ops.linear_adapted(x, w, None, down, up, None, ids)
+    for b in (0, 7, 8):
+        assert near(y[b, -300:], ops.linear_adapted(x[b:b + 1, -300:], w, None, down, up, None, ids[b:b + 1])[0])
+    del x, y
+    B, T, Hk, Hv, d = 70, 16000, 2, 16, 128
+    q, k, v = rn(B, T, Hk, d), rn(B, T, Hk, d), rn(B, T, Hv, d)
+    q, k = q / q.norm(dim=-1, keepdim=True), k / k.norm(dim=-1, keepdim=True)
+    g, beta = -torch.rand(B, T, Hv, generator=gen, device="cuda"), torch.rand(B, T, Hv, generator=gen, device="cuda")
+    assert v.numel() > 2 ** 31
+    o, s = ops.delta_rule(q, k, v, g, beta)
+    # (the state forgets within some 30 frames: the last 640 from zero give the same last 128)
+    tail = [t[-1:, -640:] for t in (q, k, v, g, beta)]
+    ot, st = ops.delta_rule(*tail)
+    assert near(o[-1, -128:], ot[0, -128:]) and near(s[-1], st[0])
+    del q, k, v, g, beta, o, s
+    n, S = 8200, 5
+    state = torch.empty(n, Hv, d, d, device="cuda")
+    assert state.numel() > 2 ** 31
+    slots = torch.tensor([n - 1, 0, n - 2, 7, 8192], device="cuda", dtype=torch.int32)
+    state[slots.long()] = rn(S, Hv, d, d, dtype=torch.float32)
+    few = state[slots.long()].clone()
+    args = rn(S, Hk, d), rn(S, Hk, d), rn(S, Hv, d), -torch.rand(S, Hv, device="cuda"), torch.rand(S, Hv, device="cuda")
+    assert torch.equal(ops.delta_rule_online(*args, state, slots), ops.delta_rule_online(*args, few)) and torch.equal(state[slots.long()], few)
