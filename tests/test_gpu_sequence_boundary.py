@@ -157,3 +157,38 @@ def test_buffers_of_more_than_2_31_elements(ops):  # noqa: F811
     few = state[slots.long()].clone()
     args = rn(S, Hk, d), rn(S, Hk, d), rn(S, Hv, d), -torch.rand(S, Hv, device="cuda"), torch.rand(S, Hv, device="cuda")
     assert torch.equal(ops.delta_rule_online(*args, state, slots), ops.delta_rule_online(*args, few)) and torch.equal(state[slots.long()], few)
+
+
+@pytest.mark.parametrize("shape", [(3, 1000, 1, 2, 64, 40), (2, 300, 8, 16, 64, 64)], ids=str)
+def test_delta_rule_in_place_captured(ops, shape):  # noqa: F811
+    """A captured call that carries its state in place, in segments and whole: every replay goes on from the state the last one left, with
+    the inputs and lengths of its time (out of range ones are held to 0..T)."""
+    import torch
+    B, T = shape[:2]
+    q, k, v, g, beta, state = (t.cuda() for t in F.delta_inputs(13, *shape, torch.bfloat16))
+    lens = torch.tensor([T, 129, 0][:B], device="cuda", dtype=torch.int32)
+    own, eager = state.clone(), state.clone()
+    call = lambda s: delta_call(ops, q, k, v, g, beta, lens, s, s, 0.3, shape)
+    call(own)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(own)
+    torch.cuda.current_stream().wait_stream(side)
+    _, Hk, Hv, dk, dv = shape[1:]
+    o = torch.empty(B, T, Hv, dv, device="cuda", dtype=q.dtype)
+    need = ops._lib.mp_delta_rule_workspace(B, T, Hv, dk, dv)
+    ws = torch.empty(need, device="cuda", dtype=torch.uint8)
+    st = (C.c_int64 * 15)(*[s for t in (q, k, v, g, beta) for s in t.stride()[:3]])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops._check(ops._lib.mp_delta_rule(ops._h, 1, *(t.data_ptr() for t in (q, k, v, g, beta)), C.addressof(st), lens.data_ptr(), B, T, Hk, Hv, dk, dv, 0.3,
+                                          o.data_ptr(), own.data_ptr(), own.data_ptr(), ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream))
+    own.copy_(state)
+    for i, n in enumerate(([T, 129, 0], [161, T, 5], [T + 7, -1, T], [33, 257, 128])):
+        lens.copy_(torch.tensor(n[:B], dtype=torch.int32))
+        v.mul_(0.5)
+        graph.replay()
+        want = call(eager)
+        torch.cuda.synchronize()
+        assert torch.equal(o, want) and torch.equal(own, eager), i
