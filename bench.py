@@ -931,11 +931,11 @@ def main():
     # (2*FETCH_SIZE + WRITE_SIZE)*1024, corrected as MI355X_MICROARCH.md prescribes.  A PMC pass cannot run inside this timed
     # process, so the figure is quoted from the committed profile -- and ONLY while the library that just ran is the binary
     # that was profiled (the summary records its md5): a changed kernel must not inherit a stale counter.  null otherwise.
-    traffic, traffic_src = None, "no PMC summary of this library (profiles/r06_pmc_summary.json absent, or profiled from other sources / another binary)"
+    traffic, traffic_src = None, "no PMC summary of this library (profiles/headline_pmc_summary.json absent, or profiled from other sources / another binary)"
     import hashlib
     lib_md5 = hashlib.md5(open(__graft_entry__.LIB, "rb").read()).hexdigest()
     src_md5 = __graft_entry__.source_md5()       # (a rebuild of the same sources gives the same device code, another .so md5)
-    for prof in ("r06_pmc_summary.json", "r05_pmc_summary.json", "r04_pmc_summary.json"):
+    for prof in ("headline_pmc_summary.json", "r06_pmc_summary.json", "r05_pmc_summary.json", "r04_pmc_summary.json"):
         try:
             summ = json.load(open(os.path.join(REPO, "profiles", prof)))
             if summ.get("lib_md5") != lib_md5 and summ.get("src_md5") != src_md5:

@@ -294,7 +294,7 @@ enum { MP_F32 = 0, MP_BF16 = 1 };
  *   state_in_dev [B,Hv,dk,dv] fp32 or NULL (zeros);  state_out_dev the same or NULL; both may be the same buffer
  *   ws_dev       mp_delta_rule_workspace(B, T, Hv, dk, dv) bytes, 16-byte aligned: the caller's until the call's work is done
  * dk is at most 256.  A value that is not finite, or beyond 3.39e38, makes the outputs of its own and later frames NaN, and none before
- * them (in v and in the state: those of its own column). */
+ * them (in q: those of its own frame; in v and in the state: those of its own column). */
 int mp_delta_rule(mp_handle* h, int dtype, const void* q_dev, const void* k_dev, const void* v_dev, const float* g_dev,
                   const float* beta_dev, const int64_t strides[15], const int32_t* lengths_dev, int B, int T, int Hk, int Hv,
                   int dk, int dv, float scale, void* o_dev, const float* state_in_dev, float* state_out_dev, void* ws_dev,

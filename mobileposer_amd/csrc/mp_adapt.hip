@@ -17,8 +17,8 @@ namespace mpseq {
 
 size_t adapt_ws_floats(int B, int T, int r) { return (size_t)B * T * r; }
 // 32-bit row and z indexes; workgroups of up to 512 threads in a launch that counts its threads in 32 bits: one per 16 frames of a
-// sequence (Down), one per 128 of them (one launch), tiles of 128 from 192 or 384 of them on (at most three times as many of 64 or 32
-// in front of that)
+// sequence (Down), one per 128 of them (one launch), tiles of 128 or 256 from 192 or 384 of 128 on (the smaller tiles in front of that
+// are a few thousand)
 bool adapt_fits(int B, int T, int M, int r) {
     const int64_t rows = (int64_t)B * T, most = (1 << 23) - 8;
     return rows <= 1 << 30 && rows * r <= 0x7fffffff && (int64_t)B * ((T + 15) / 16) <= most && (rows + 127) / 128 * (((int64_t)M + 127) / 128) <= most;
